@@ -400,6 +400,99 @@ int rbh_sksy_tri_ex_f32(char layout, char side, char uplo, char A_fmt, int64_t d
                         int64_t ro_s, int64_t co_s, const float *A, int64_t lda, float beta, float *B, int64_t ldb,
                         const rbh_options *opt, void *stream);
 
+/* 4-bit microscaled matrices (no reference counterpart). The format is MXFP4 of the Open Compute
+ * Project's Microscaling Formats v1.0: an element is sign, 2 exponent bits and 1 mantissa bit (0, 0.5,
+ * 1, 1.5, 2, 3, 4, 6), and 32 consecutive elements of a row share a scale 2^(s - 127), stored as the
+ * byte s (255: NaN, the whole block is NaN). Row r of the matrix is
+ *   codes + r * ld_codes:   16 bytes a block, two elements a byte, the even column in the low half;
+ *   scales + r * ld_scales: one byte a block.
+ * The codes of the last block past n_cols are zero (rbh_mx4_quantize_* writes them so); bytes between
+ * rows are never read for a result nor written. codes and ld_codes are multiples of 16, scales may have
+ * any alignment (multiples of 4 for both scales and ld_scales spare a product a copy of them); ld_codes
+ * and ld_scales are at most 2^23. Device
+ * or host memory, as for every matrix; all device arrays of a call are on one device. */
+typedef struct rbh_mx4 {
+    int64_t n_rows, n_cols;
+    uint8_t *codes;
+    int64_t ld_codes;
+    uint8_t *scales;
+    int64_t ld_scales;
+} rbh_mx4;
+
+/* A workspace for one call. ptr == NULL: the call only writes the bytes it needs and returns. Otherwise
+ * ptr is device memory, a multiple of 256, of at least that many bytes. A call without one (NULL) takes
+ * what it needs from the stream's workspaces, except on a stream that is captured into a graph, where a
+ * call that needs bytes and is given none fails: a graph would share the block with all later calls. */
+typedef struct rbh_work {
+    void *ptr;
+    int64_t bytes;
+} rbh_work;
+
+/* Rounding. RBH_ROUND_NEAREST: a block's scale is the power of two 2^e with e = floor(log2 max|x|) - 2,
+ * x 2^-e goes to the nearest element, ties to even, above 6 to 6. RBH_ROUND_STOCHASTIC: e is one more
+ * where max|x| > 6 * 2^e, so that nothing is cut, and x 2^-e goes to one of its two neighbours with
+ * probabilities that make the result's mean x: up iff w < floor(part * 2^32), part its place between
+ * them and w the word c & 3 of the generator's block at counter + r * ceil(n_cols / 4) + (c >> 2) -- the
+ * words rbh_fill_dense_* reads for entry (r, c) of an operator with rows of n_cols. e is kept in
+ * [-127, 125]. A block with an infinity or a NaN gets scale 255 and zero codes. */
+#define RBH_ROUND_NEAREST 0
+#define RBH_ROUND_STOCHASTIC 1
+
+/* Q (n_rows x n_cols) = op(A). seed: for stochastic rounding only; next_state (may be NULL): the state
+ * after the words that were read. f16 and bf16 are passed as their 16 bits. */
+int rbh_mx4_quantize_f64(char layout, char op, int64_t n_rows, int64_t n_cols, const double *A, int64_t lda,
+                         const rbh_mx4 *Q, int rounding, const rbh_state *seed, rbh_state *next_state, void *stream);
+int rbh_mx4_quantize_f32(char layout, char op, int64_t n_rows, int64_t n_cols, const float *A, int64_t lda,
+                         const rbh_mx4 *Q, int rounding, const rbh_state *seed, rbh_state *next_state, void *stream);
+int rbh_mx4_quantize_f16(char layout, char op, int64_t n_rows, int64_t n_cols, const uint16_t *A, int64_t lda,
+                         const rbh_mx4 *Q, int rounding, const rbh_state *seed, rbh_state *next_state, void *stream);
+int rbh_mx4_quantize_bf16(char layout, char op, int64_t n_rows, int64_t n_cols, const uint16_t *A, int64_t lda,
+                          const rbh_mx4 *Q, int rounding, const rbh_state *seed, rbh_state *next_state, void *stream);
+
+/* op(A) = submat(Q), n_rows x n_cols at (ro, co), co a multiple of 32. */
+int rbh_mx4_dequantize_f64(char layout, char op, int64_t n_rows, int64_t n_cols, const rbh_mx4 *Q, int64_t ro,
+                           int64_t co, double *A, int64_t lda, void *stream);
+int rbh_mx4_dequantize_f32(char layout, char op, int64_t n_rows, int64_t n_cols, const rbh_mx4 *Q, int64_t ro,
+                           int64_t co, float *A, int64_t lda, void *stream);
+int rbh_mx4_dequantize_f16(char layout, char op, int64_t n_rows, int64_t n_cols, const rbh_mx4 *Q, int64_t ro,
+                           int64_t co, uint16_t *A, int64_t lda, void *stream);
+int rbh_mx4_dequantize_bf16(char layout, char op, int64_t n_rows, int64_t n_cols, const rbh_mx4 *Q, int64_t ro,
+                            int64_t co, uint16_t *A, int64_t lda, void *stream);
+
+/* C (m x n) = alpha op(A) op(B) + beta C, sums in 32 bits. right: B is submat(B) of a 4-bit matrix at
+ * (ro_b, co_b), as the sparse factor of rbh_spmm_right_*; left: A is; both: both are, and their blocks
+ * have to lie along the contraction (opA = 'N', opB = 'T'). Column offsets are multiples of 32. The
+ * dense factor and C have one type; the dense factor enters the sums with all its bits. The gradient of
+ * a product's dense factor is the product of C's gradient with op flipped on the 4-bit one. C overlaps
+ * no other array. */
+int rbh_mxmm_right_f32(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const float *A,
+                       int64_t lda, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta, float *C, int64_t ldc,
+                       rbh_work *work, void *stream);
+int rbh_mxmm_right_f16(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha,
+                       const uint16_t *A, int64_t lda, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta,
+                       uint16_t *C, int64_t ldc, rbh_work *work, void *stream);
+int rbh_mxmm_right_bf16(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha,
+                        const uint16_t *A, int64_t lda, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta,
+                        uint16_t *C, int64_t ldc, rbh_work *work, void *stream);
+int rbh_mxmm_left_f32(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const rbh_mx4 *A,
+                      int64_t ro_a, int64_t co_a, const float *B, int64_t ldb, float beta, float *C, int64_t ldc,
+                      rbh_work *work, void *stream);
+int rbh_mxmm_left_f16(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const rbh_mx4 *A,
+                      int64_t ro_a, int64_t co_a, const uint16_t *B, int64_t ldb, float beta, uint16_t *C, int64_t ldc,
+                      rbh_work *work, void *stream);
+int rbh_mxmm_left_bf16(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const rbh_mx4 *A,
+                       int64_t ro_a, int64_t co_a, const uint16_t *B, int64_t ldb, float beta, uint16_t *C, int64_t ldc,
+                       rbh_work *work, void *stream);
+int rbh_mxmm_both_f32(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const rbh_mx4 *A,
+                      int64_t ro_a, int64_t co_a, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta, float *C,
+                      int64_t ldc, rbh_work *work, void *stream);
+int rbh_mxmm_both_f16(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const rbh_mx4 *A,
+                      int64_t ro_a, int64_t co_a, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta, uint16_t *C,
+                      int64_t ldc, rbh_work *work, void *stream);
+int rbh_mxmm_both_bf16(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const rbh_mx4 *A,
+                       int64_t ro_a, int64_t co_a, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta,
+                       uint16_t *C, int64_t ldc, rbh_work *work, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

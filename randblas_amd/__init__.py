@@ -66,6 +66,16 @@ class PlanC(ctypes.Structure):
     _fields_ = [("kernel", ctypes.c_int32), ("splitk", ctypes.c_int32), ("tiles", c_i64), ("workgroups", c_i64)]
 
 
+class MX4MatrixC(ctypes.Structure):
+    # rbh_mx4 (include/randblas_hip.h)
+    _fields_ = [("n_rows", c_i64), ("n_cols", c_i64), ("codes", c_vp), ("ld_codes", c_i64), ("scales", c_vp),
+                ("ld_scales", c_i64)]
+
+
+class WorkC(ctypes.Structure):
+    _fields_ = [("ptr", c_vp), ("bytes", c_i64)]
+
+
 class RandBLASError(RuntimeError):
     """RandBLAS::exceptions::Error equivalent (RandBLAS/exceptions.hh:45-70)."""
 
@@ -161,6 +171,19 @@ for _t, _ct in (("f64", ctypes.c_double), ("f32", ctypes.c_float)):
     getattr(lib, f"rbh_sketch_symmetric_ex_{_t}").argtypes = \
         getattr(lib, f"rbh_sketch_symmetric_{_t}").argtypes[:-1] + [P(OptionsC), c_vp]
     getattr(lib, f"rbh_sksy_tri_ex_{_t}").argtypes = getattr(lib, f"rbh_sksy_tri_{_t}").argtypes[:-1] + [P(OptionsC), c_vp]
+
+for _t in ("f64", "f32", "f16", "bf16"):
+    getattr(lib, f"rbh_mx4_quantize_{_t}").argtypes = [c_char, c_char, c_i64, c_i64, c_vp, c_i64, P(MX4MatrixC),
+                                                       ctypes.c_int, P(RNGStateC), P(RNGStateC), c_vp]
+    getattr(lib, f"rbh_mx4_dequantize_{_t}").argtypes = [c_char, c_char, c_i64, c_i64, P(MX4MatrixC), c_i64, c_i64,
+                                                         c_vp, c_i64, c_vp]
+for _t in ("f32", "f16", "bf16"):
+    _mmh = [c_char, c_char, c_char, c_i64, c_i64, c_i64, ctypes.c_float]
+    _mmd, _mmq = [c_vp, c_i64], [P(MX4MatrixC), c_i64, c_i64]
+    _mmt = [ctypes.c_float, c_vp, c_i64, P(WorkC), c_vp]
+    getattr(lib, f"rbh_mxmm_right_{_t}").argtypes = _mmh + _mmd + _mmq + _mmt
+    getattr(lib, f"rbh_mxmm_left_{_t}").argtypes = _mmh + _mmq + _mmd + _mmt
+    getattr(lib, f"rbh_mxmm_both_{_t}").argtypes = _mmh + _mmq + _mmq + _mmt
 
 # --------------------------------------------------------------------------------------------
 # Python mirror of the reference's types
@@ -691,6 +714,126 @@ def spmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
                                                     _stream(C, stream)))
 
 
+# --------------------------------------------------------------------------------------------
+# 4-bit microscaled matrices (MXFP4; no reference counterpart)
+# --------------------------------------------------------------------------------------------
+_MX4_TAGS = {"float64": "f64", "float32": "f32", "float16": "f16", "bfloat16": "bf16"}
+ROUNDINGS = {"nearest": 0, "stochastic": 1}   # RBH_ROUND_*
+
+
+def _mx4_tag(x) -> str:
+    tag = _MX4_TAGS.get(str(x.dtype).removeprefix("torch."))
+    if tag is None:
+        raise TypeError(f"unsupported dtype {x.dtype}")
+    return tag
+
+
+def _bytes_2d(x, name, rows, width):
+    """The bytes between rows of a uint8 array of at least rows x width, checked."""
+    if str(x.dtype) not in ("uint8", "torch.uint8") or len(x.shape) != 2:
+        raise TypeError(f"{name} must be a 2-D uint8 array")
+    strides = x.strides if isinstance(x, np.ndarray) else x.stride()
+    if rows == 0 or width == 0:
+        return width
+    if x.shape[0] < rows or x.shape[1] < width or (x.shape[1] > 1 and strides[1] != 1):
+        raise ValueError(f"{name} must hold {rows} rows of {width} consecutive bytes")
+    return strides[0] if rows > 1 else max(strides[0], width)
+
+
+@dataclass(frozen=True)
+class MX4Matrix:
+    """A 4-bit microscaled matrix (rbh_mx4, include/randblas_hip.h): n_rows x n_cols E2M1 elements, blocks
+    of 32 along a row, one E8M0 scale a block. codes: uint8, n_rows x 16 bytes a block, two elements a
+    byte, the even column in the low half. scales: uint8, n_rows x one byte a block. Device tensors or
+    host arrays; rows may be further apart than they are long (codes: by multiples of 16)."""
+
+    n_rows: int
+    n_cols: int
+    codes: object
+    scales: object
+    _c: MX4MatrixC = field(default=None, repr=False, compare=False)
+
+    def __post_init__(self):
+        nb = (self.n_cols + 31) // 32
+        c = MX4MatrixC(self.n_rows, self.n_cols, _ptr(self.codes), _bytes_2d(self.codes, "codes", self.n_rows, 16 * nb),
+                       _ptr(self.scales), _bytes_2d(self.scales, "scales", self.n_rows, nb))
+        object.__setattr__(self, "_c", c)
+
+
+def mx4_empty(n_rows: int, n_cols: int, device=None) -> MX4Matrix:
+    """An uninitialised MX4Matrix of device tensors (device: the current one by default); rows of scales
+    start at multiples of 4 bytes."""
+    nb = (n_cols + 31) // 32
+    device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
+    return MX4Matrix(n_rows, n_cols, torch.empty(n_rows, 16 * nb, dtype=torch.uint8, device=device),
+                     torch.empty(n_rows, (nb + 3) // 4 * 4, dtype=torch.uint8, device=device))
+
+
+def mx4_quantize(layout, op, n_rows, n_cols, A, lda, Q: MX4Matrix, rounding="nearest",
+                 seed: Optional[RNGState] = None, stream=None) -> Optional[RNGState]:
+    """Q = op(A), n_rows x n_cols, in 4 bits with blocks along op(A)'s rows (rbh_mx4_quantize). rounding
+    "nearest" (ties to even) or "stochastic" (unbiased; reads the words of seed that fill_dense reads
+    for a row-major n_rows x n_cols operator, and returns the state after them)."""
+    if rounding not in ROUNDINGS:
+        raise ValueError(f"rounding must be one of {sorted(ROUNDINGS)}, not {rounding!r}")
+    if rounding == "stochastic" and seed is None:
+        raise ValueError("stochastic rounding needs a seed state")
+    sr = rounding == "stochastic"
+    nxt = RNGStateC()
+    _check(getattr(lib, f"rbh_mx4_quantize_{_mx4_tag(A)}")(
+        _b(layout), _b(op), n_rows, n_cols, _ptr(A), lda, ctypes.byref(Q._c), ROUNDINGS[rounding],
+        ctypes.byref(seed.c()) if sr else None, ctypes.byref(nxt) if sr else None, _stream(A, stream)))
+    return RNGState.from_c(nxt) if sr else None
+
+
+def mx4_dequantize(layout, op, n_rows, n_cols, Q: MX4Matrix, A, lda, ro=0, co=0, stream=None) -> None:
+    """op(A) = submat(Q), n_rows x n_cols at (ro, co), co a multiple of 32 (rbh_mx4_dequantize). Exact in
+    every type but f16, which rounds to nearest even."""
+    _check(getattr(lib, f"rbh_mx4_dequantize_{_mx4_tag(A)}")(_b(layout), _b(op), n_rows, n_cols, ctypes.byref(Q._c),
+                                                             ro, co, _ptr(A), lda, _stream(A, stream)))
+
+
+def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, stream=None) -> None:
+    """C (m x n) = alpha * op(A) * op(B) + beta * C with one or two 4-bit factors, called as spmm is:
+      mxmm(layout, opA, opB, m, n, k, alpha, A_mx4, ro_a, co_a, B, ldb, beta, C, ldc)
+      mxmm(layout, opA, opB, m, n, k, alpha, A, lda, B_mx4, ro_b, co_b, beta, C, ldc)
+      mxmm(layout, opA, opB, m, n, k, alpha, A_mx4, ro_a, co_a, B_mx4, ro_b, co_b, beta, C, ldc)
+    The dense factor and C are of one type, f32, f16 or bf16; sums are formed in 32 bits. Two 4-bit
+    factors need opA = "N" and opB = "T" (blocks along the contraction). The gradient of the dense
+    factor is the product of C's gradient with op flipped on the 4-bit one.
+
+    On a stream that a graph captures, a call that needs a workspace allocates it from the graph's own
+    memory (torch's allocator), so captured calls share none."""
+    if isinstance(X, MX4Matrix):
+        ro_a, co_a = x_off_r, x_off_c_or_ld
+        if isinstance(Y, MX4Matrix):
+            side, (ro_b, co_b, beta, C, ldc) = "both", args
+            factors, dense = [ctypes.byref(X._c), ro_a, co_a, ctypes.byref(Y._c), ro_b, co_b], None
+        else:
+            side, (ldb, beta, C, ldc) = "left", args
+            factors, dense = [ctypes.byref(X._c), ro_a, co_a, _ptr(Y), ldb], Y
+    else:
+        A, lda, B = X, x_off_r, x_off_c_or_ld
+        if not isinstance(B, MX4Matrix):
+            raise TypeError("mxmm needs an MX4Matrix")
+        side, (ro_b, co_b, beta, C, ldc) = "right", (Y,) + args
+        factors, dense = [_ptr(A), lda, ctypes.byref(B._c), ro_b, co_b], A
+    t = _mx4_tag(C)
+    if t == "f64" or (dense is not None and dense.dtype != C.dtype):
+        raise TypeError("mxmm: C and the dense factor must both be f32, both f16 or both bf16")
+    fn, st = getattr(lib, f"rbh_mxmm_{side}_{t}"), _stream(C, stream)
+    head = (_b(layout), _b(opA), _b(opB), m, n, k, alpha, *factors, beta, _ptr(C), ldc)
+    if torch is None or not getattr(C, "is_cuda", False) or not torch.cuda.is_current_stream_capturing():
+        return _check(fn(*head, None, st))
+    work = WorkC()
+    _check(fn(*head, ctypes.byref(work), st))
+    if work.bytes == 0:
+        return _check(fn(*head, None, st))
+    block = torch.empty(work.bytes, dtype=torch.uint8, device=C.device)
+    work.ptr = block.data_ptr()
+    _check(fn(*head, ctypes.byref(work), st))
+
+
 def kernel_timing(on: bool) -> None:
     """Enable/disable HIP-event timing of each call's dominant kernel (diagnostics)."""
     lib.rbh_kernel_timing_enable(1 if on else 0)
@@ -742,5 +885,6 @@ __all__ = [
     "LIB_PATH", "kernel_timing", "kernel_times_ms", "sketch_vector", "sketch_vector_full", "COOMatrix",
     "CSRMatrix", "CSCMatrix", "sketch_sparse", "sketch_sparse_left", "sketch_sparse_right", "spmm",
     "sketch_symmetric_tri", "release_workspaces", "unpack_shards", "Options", "Plan", "plan_left", "plan_right",
-    "sketch_symmetric_last_path", "fill_sparse_op", "sparse_last_path",
+    "sketch_symmetric_last_path", "fill_sparse_op", "sparse_last_path", "MX4Matrix", "mx4_empty", "mx4_quantize",
+    "mx4_dequantize", "mxmm",
 ]

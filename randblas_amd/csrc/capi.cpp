@@ -16,11 +16,13 @@
 #include <cstdio>
 #include <cstdlib>
 #include <cstring>
+#include <new>
 #include <string>
 #include <vector>
 
 #include "../../include/randblas_hip.h"
 #include "common.hpp"
+#include "mx4.hpp"
 #include "saso.hpp"
 
 using namespace rbh;
@@ -1828,4 +1830,321 @@ int rbh_rskge3_plan_st_f32(char layout, char opA, char opS, int64_t m, int64_t d
                              seed);
 }
 
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------
+// 4-bit microscaled matrices (mx4.hip, mx4_gemm.hip)
+// ---------------------------------------------------------------------------------------------
+namespace {
+
+// The device a call's arrays are on becomes the current one for the call: launches, workspaces and a
+// NULL stream belong to it. All device arrays of a call have to be on one device.
+struct DeviceOf {
+    int before = -1, want = -1;
+    bool differ = false;
+    void look(const void *p) {
+        hipPointerAttribute_t a;
+        if (!p) return;
+        if (hipPointerGetAttributes(&a, p) != hipSuccess) { (void)hipGetLastError(); return; }
+        if (a.type != hipMemoryTypeDevice) return;   // managed memory is reached from every device
+        if (want >= 0 && a.device != want) differ = true;
+        want = a.device;
+    }
+    hipError_t enter() {
+        if (want < 0) return hipSuccess;
+        int cur = 0;
+        hipError_t e = hipGetDevice(&cur);
+        if (e != hipSuccess || cur == want) return e;
+        e = hipSetDevice(want);
+        if (e == hipSuccess) before = cur;
+        return e;
+    }
+    ~DeviceOf() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+};
+
+// A workspace of one call: the caller's block, or the stream's arena
+struct CallWork {
+    void *p = nullptr;
+    bool owned = false;
+    hipStream_t s;
+    explicit CallWork(hipStream_t st) : s(st) {}
+    ~CallWork() {
+        if (owned) (void)ws_free(p, s);
+    }
+};
+
+bool mx4_ok(const rbh_mx4 *Q) {
+    return Q != nullptr && Q->n_rows >= 0 && Q->n_cols >= 0 &&
+           (Q->n_rows == 0 || Q->n_cols == 0 || (Q->codes != nullptr && Q->scales != nullptr));
+}
+// the window of rows x cols of Q at (ro, co), staged
+int mx4_window(Stager &st, const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t rows, int64_t cols, bool out, Mx4View &v) {
+    v = Mx4View{};
+    v.rows = rows;
+    v.cols = cols;
+    v.ldq = Q->ld_codes;
+    v.lds = Q->ld_scales;
+    if (rows == 0 || cols == 0) return RBH_OK;
+    const int64_t nb = mx4_blocks(cols);
+    uint8_t *q = Q->codes + ro * Q->ld_codes + co / 2, *sc = Q->scales + ro * Q->ld_scales + co / MX4_BLOCK;
+    RBH_HIP(st.map_window(q, (size_t)extent('R', rows, nb * 16, Q->ld_codes), !out, out, (size_t)(nb * 16), (size_t)rows,
+                          (size_t)Q->ld_codes, (void **)&v.codes));
+    RBH_HIP(st.map_window(sc, (size_t)extent('R', rows, nb, Q->ld_scales), !out, out, (size_t)nb, (size_t)rows,
+                          (size_t)Q->ld_scales, (void **)&v.scales));
+    return RBH_OK;
+}
+
+// what a 4-bit matrix of any call has to satisfy (window at (ro, co), rows x cols)
+#define RBH_REQUIRE_MX4(Q, rows, cols, ro, co)                          \
+    RBH_REQUIRE(mx4_ok(Q));                                             \
+    RBH_REQUIRE((ro) >= 0 && (co) >= 0 && (co) % 32 == 0);              \
+    RBH_REQUIRE((Q)->n_rows >= (rows) + (ro));                          \
+    RBH_REQUIRE((Q)->n_cols >= (cols) + (co));                          \
+    RBH_REQUIRE((Q)->ld_codes % 16 == 0 && (Q)->ld_codes <= (1 << 23)); \
+    RBH_REQUIRE((Q)->ld_scales <= (1 << 23));                           \
+    RBH_REQUIRE((Q)->ld_codes >= 16 * mx4_blocks((Q)->n_cols));         \
+    RBH_REQUIRE((Q)->ld_scales >= mx4_blocks((Q)->n_cols));             \
+    RBH_REQUIRE((uintptr_t)(Q)->codes % 16 == 0)
+
+int mx4_quantize(int type, char layout, char op, int64_t n_rows, int64_t n_cols, const void *A, int64_t lda,
+                 const rbh_mx4 *Q, int rounding, const rbh_state *seed, rbh_state *next_state, void *stream) {
+    RBH_REQUIRE(layout == 'C' || layout == 'R');
+    RBH_REQUIRE(op == 'N' || op == 'T');
+    RBH_REQUIRE(n_rows >= 0 && n_cols >= 0);
+    const int64_t rows_A = op == 'N' ? n_rows : n_cols, cols_A = op == 'N' ? n_cols : n_rows;
+    RBH_REQUIRE(lda >= (layout == 'C' ? rows_A : cols_A));
+    RBH_REQUIRE_MX4(Q, n_rows, n_cols, 0, 0);
+    RBH_REQUIRE(Q->n_rows == n_rows && Q->n_cols == n_cols);
+    RBH_REQUIRE(rounding == RBH_ROUND_NEAREST || rounding == RBH_ROUND_STOCHASTIC);
+    if (rounding == RBH_ROUND_STOCHASTIC) {
+        RBH_REQUIRE(seed != nullptr);
+        RBH_REQUIRE(seed->rng == RBH_RNG_PHILOX4X32 || seed->rng == RBH_RNG_THREEFRY4X32);
+    }
+    const bool empty = n_rows == 0 || n_cols == 0;
+    RBH_REQUIRE(empty || A != nullptr);
+    DeviceOf dev;
+    dev.look(A);
+    dev.look(Q->codes);
+    dev.look(Q->scales);
+    RBH_REQUIRE_AS(!dev.differ, "all arrays on one device", __func__);
+    RBH_HIP(dev.enter());
+    hipStream_t s = (hipStream_t)stream;
+    Stager st(s);
+    void *dA;
+    RBH_HIP(st.map(A, (size_t)mx4_size(type) * (size_t)extent(layout, rows_A, cols_A, lda), true, false, &dA));
+    Mx4View v;
+    const int rc = mx4_window(st, Q, 0, 0, n_rows, n_cols, true, v);
+    if (rc) return rc;
+    const bool along = (layout == 'R') == (op == 'N');   // a row of op(A) is contiguous
+    const Mx4Dense a{dA, along ? lda : 1, along ? 1 : lda, type};
+    Mx4Random rnd{};
+    if (rounding == RBH_ROUND_STOCHASTIC) {
+        memcpy(rnd.ctr, seed->counter, sizeof rnd.ctr);
+        memcpy(rnd.key, seed->key, sizeof rnd.key);
+        rnd.rng = seed->rng == RBH_RNG_THREEFRY4X32 ? rb::RNG_THREEFRY : rb::RNG_PHILOX;
+        rnd.quads = (uint64_t)((n_cols + 3) / 4);
+        if (next_state) {
+            const rbh_state from = *seed;
+            *next_state = from;
+            rb::ctr_add(from.counter, (uint64_t)n_rows * rnd.quads, next_state->counter);
+        }
+    }
+    RBH_HIP(launch_mx4_quantize(a, v, rounding == RBH_ROUND_STOCHASTIC ? &rnd : nullptr, s));
+    RBH_HIP(st.finish());
+    return RBH_OK;
+}
+
+int mx4_dequantize(int type, char layout, char op, int64_t n_rows, int64_t n_cols, const rbh_mx4 *Q, int64_t ro,
+                   int64_t co, void *A, int64_t lda, void *stream) {
+    RBH_REQUIRE(layout == 'C' || layout == 'R');
+    RBH_REQUIRE(op == 'N' || op == 'T');
+    RBH_REQUIRE(n_rows >= 0 && n_cols >= 0);
+    const int64_t rows_A = op == 'N' ? n_rows : n_cols, cols_A = op == 'N' ? n_cols : n_rows;
+    RBH_REQUIRE(lda >= (layout == 'C' ? rows_A : cols_A));
+    RBH_REQUIRE_MX4(Q, n_rows, n_cols, ro, co);
+    const bool empty = n_rows == 0 || n_cols == 0;
+    RBH_REQUIRE(empty || A != nullptr);
+    DeviceOf dev;
+    dev.look(A);
+    dev.look(Q->codes);
+    dev.look(Q->scales);
+    RBH_REQUIRE_AS(!dev.differ, "all arrays on one device", __func__);
+    RBH_HIP(dev.enter());
+    hipStream_t s = (hipStream_t)stream;
+    Stager st(s);
+    void *dA;
+    RBH_HIP(st.map_out(A, (size_t)mx4_size(type), layout, rows_A, cols_A, lda, false, &dA));
+    Mx4View v;
+    const int rc = mx4_window(st, Q, ro, co, n_rows, n_cols, false, v);
+    if (rc) return rc;
+    const bool along = (layout == 'R') == (op == 'N');
+    const Mx4Dense a{dA, along ? lda : 1, along ? 1 : lda, type};
+    RBH_HIP(launch_mx4_dequantize(v, a, s));
+    RBH_HIP(st.finish());
+    return RBH_OK;
+}
+
+// C = alpha op(A) op(B) + beta C. side 'R': B is 4-bit, 'L': A is, 'B': both. In the canonical problem Y
+// is a 4-bit factor whose rows (yt = 0) or columns (yt = 1) are the second index of the result.
+int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha,
+         const void *D, int64_t ldd, const rbh_mx4 *QA, int64_t ro_a, int64_t co_a, const rbh_mx4 *QB, int64_t ro_b,
+         int64_t co_b, float beta, void *C, int64_t ldc, rbh_work *work, void *stream) {
+    RBH_REQUIRE(layout == 'C' || layout == 'R');
+    RBH_REQUIRE(opA == 'N' || opA == 'T');
+    RBH_REQUIRE(opB == 'N' || opB == 'T');
+    RBH_REQUIRE(m >= 0 && n >= 0 && k >= 0);
+    const int64_t rows_A = opA == 'N' ? m : k, cols_A = opA == 'N' ? k : m;
+    const int64_t rows_B = opB == 'N' ? k : n, cols_B = opB == 'N' ? n : k;
+    RBH_REQUIRE(ldc >= (layout == 'C' ? m : n));
+    if (side == 'R') RBH_REQUIRE(ldd >= (layout == 'C' ? rows_A : cols_A));
+    if (side == 'L') RBH_REQUIRE(ldd >= (layout == 'C' ? rows_B : cols_B));
+    if (side != 'R') { RBH_REQUIRE_MX4(QA, rows_A, cols_A, ro_a, co_a); }
+    if (side != 'L') { RBH_REQUIRE_MX4(QB, rows_B, cols_B, ro_b, co_b); }
+    // two 4-bit factors: blocks along the contraction in both (dequantise one of them otherwise)
+    if (side == 'B') RBH_REQUIRE(opA == 'N' && opB == 'T');
+    const bool empty = m == 0 || n == 0, reads = !empty && k > 0 && alpha != 0.f;
+    RBH_REQUIRE(empty || C != nullptr);
+    if (side != 'B') RBH_REQUIRE(!reads || D != nullptr);
+    if (work) RBH_REQUIRE(work->bytes >= 0);
+
+    DeviceOf dev;
+    dev.look(C);
+    if (side != 'B') dev.look(D);
+    if (side != 'R') dev.look(QA->codes), dev.look(QA->scales);
+    if (side != 'L') dev.look(QB->codes), dev.look(QB->scales);
+    if (work) dev.look(work->ptr);
+    RBH_REQUIRE_AS(!dev.differ, "all arrays on one device", __func__);
+    RBH_HIP(dev.enter());
+    const bool query = work && !work->ptr;
+    hipStream_t s = (hipStream_t)stream;
+    Stager st(s);
+    Mx4Product p{};
+    p.type = type;
+    p.alpha = reads ? alpha : 0.f;
+    p.beta = beta;
+    p.K = k;
+    p.both = side == 'B';
+    void *dC = C, *dD = const_cast<void *>(D);
+    if (!query) {
+        RBH_HIP(st.map_out(C, (size_t)mx4_size(type), layout, m, n, ldc, beta != 0.f, &dC));
+        if (side != 'B' && reads) {
+            const int64_t r = side == 'R' ? rows_A : rows_B, c = side == 'R' ? cols_A : cols_B;
+            RBH_HIP(st.map(D, (size_t)mx4_size(type) * (size_t)extent(layout, r, c, ldd), true, false, &dD));
+        }
+    }
+    p.C = dC;
+    auto view = [&](const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t rows, int64_t cols, Mx4View &v) -> int {
+        if (query || !reads) {
+            v = Mx4View{Q->codes + ro * Q->ld_codes + co / 2, Q->scales + ro * Q->ld_scales + co / MX4_BLOCK, Q->ld_codes,
+                        Q->ld_scales, rows, cols};
+            return RBH_OK;
+        }
+        return mx4_window(st, Q, ro, co, rows, cols, false, v);
+    };
+    const int64_t cr = layout == 'C' ? 1 : ldc, cc = layout == 'C' ? ldc : 1;   // strides of C along rows, columns
+    int rc;
+    if (side == 'L') {   // C^T (n x m) = op(B)^T op(A)^T: the dense factor's rows are C's columns
+        p.M = n; p.N = m; p.ci = cc; p.cj = cr;
+        const bool along = (layout == 'R') == (opB == 'T');   // op(B)^T has contiguous rows
+        p.X = Mx4Dense{dD, along ? ldd : 1, along ? 1 : ldd, type};
+        p.yt = opA == 'T';
+        rc = view(QA, ro_a, co_a, rows_A, cols_A, p.Y);
+    } else {
+        p.M = m; p.N = n; p.ci = cr; p.cj = cc;
+        if (side == 'R') {
+            const bool along = (layout == 'R') == (opA == 'N');
+            p.X = Mx4Dense{dD, along ? ldd : 1, along ? 1 : ldd, type};
+        } else {
+            rc = view(QA, ro_a, co_a, rows_A, cols_A, p.XQ);
+            if (rc) return rc;
+        }
+        p.yt = opB == 'N';
+        rc = view(QB, ro_b, co_b, rows_B, cols_B, p.Y);
+    }
+    if (rc) return rc;
+    const size_t need = empty ? 0 : mx4_product_work(p);
+    if (query) {
+        work->bytes = (int64_t)need;
+        return RBH_OK;
+    }
+    CallWork ws(s);
+    if (need) {
+        if (work) {
+            RBH_REQUIRE(work->bytes >= (int64_t)need && (uintptr_t)work->ptr % 256 == 0);
+            RBH_REQUIRE(is_device_ptr(work->ptr));
+            ws.p = work->ptr;
+        } else {
+            // a graph would keep the arena's block, which later calls and other graphs use as well
+            hipStreamCaptureStatus cs = hipStreamCaptureStatusNone;
+            RBH_HIP(hipStreamIsCapturing(s, &cs));
+            RBH_REQUIRE_AS(cs == hipStreamCaptureStatusNone, "a workspace of the caller's in a captured call", __func__);
+            RBH_HIP(ws_alloc(&ws.p, need, s));
+            ws.owned = true;
+        }
+    }
+    RBH_HIP(launch_mx4_product(p, ws.p, s));
+    RBH_HIP(st.finish());
+    return RBH_OK;
+}
+
+// no C++ exception leaves a C entry (std::vector and std::map of the staging and the arenas may throw)
+template <typename F> int guarded(F f) {
+    try {
+        return f();
+    } catch (const std::bad_alloc &) {
+        return set_error(RBH_ERR_HIP, "out of host memory");
+    } catch (...) {
+        return set_error(RBH_ERR_HIP, "unexpected C++ exception");
+    }
+}
+}  // namespace
+
+extern "C" {
+#define RBH_MX4_CONVERT(SUF, TYPE, T)                                                                                   \
+    int rbh_mx4_quantize_##SUF(char layout, char op, int64_t n_rows, int64_t n_cols, const T *A, int64_t lda,           \
+                               const rbh_mx4 *Q, int rounding, const rbh_state *seed, rbh_state *next_state,            \
+                               void *stream) {                                                                          \
+        return guarded([&] {                                                                                            \
+            return mx4_quantize(TYPE, layout, op, n_rows, n_cols, A, lda, Q, rounding, seed, next_state, stream);       \
+        });                                                                                                             \
+    }                                                                                                                   \
+    int rbh_mx4_dequantize_##SUF(char layout, char op, int64_t n_rows, int64_t n_cols, const rbh_mx4 *Q, int64_t ro,    \
+                                 int64_t co, T *A, int64_t lda, void *stream) {                                         \
+        return guarded([&] { return mx4_dequantize(TYPE, layout, op, n_rows, n_cols, Q, ro, co, A, lda, stream); });    \
+    }
+RBH_MX4_CONVERT(f64, MX4_F64, double)
+RBH_MX4_CONVERT(f32, MX4_F32, float)
+RBH_MX4_CONVERT(f16, MX4_F16, uint16_t)
+RBH_MX4_CONVERT(bf16, MX4_BF16, uint16_t)
+
+#define RBH_MXMM(SUF, TYPE, T)                                                                                          \
+    int rbh_mxmm_right_##SUF(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const T *A, \
+                             int64_t lda, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta, T *C, int64_t ldc,  \
+                             rbh_work *work, void *stream) {                                                            \
+        return guarded([&] {                                                                                            \
+            return mxmm(TYPE, 'R', layout, opA, opB, m, n, k, alpha, A, lda, nullptr, 0, 0, B, ro_b, co_b, beta, C,     \
+                        ldc, work, stream);                                                                             \
+        });                                                                                                             \
+    }                                                                                                                   \
+    int rbh_mxmm_left_##SUF(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha,              \
+                            const rbh_mx4 *A, int64_t ro_a, int64_t co_a, const T *B, int64_t ldb, float beta, T *C,    \
+                            int64_t ldc, rbh_work *work, void *stream) {                                                \
+        return guarded([&] {                                                                                            \
+            return mxmm(TYPE, 'L', layout, opA, opB, m, n, k, alpha, B, ldb, A, ro_a, co_a, nullptr, 0, 0, beta, C,     \
+                        ldc, work, stream);                                                                             \
+        });                                                                                                             \
+    }                                                                                                                   \
+    int rbh_mxmm_both_##SUF(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha,              \
+                            const rbh_mx4 *A, int64_t ro_a, int64_t co_a, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, \
+                            float beta, T *C, int64_t ldc, rbh_work *work, void *stream) {                              \
+        return guarded([&] {                                                                                            \
+            return mxmm(TYPE, 'B', layout, opA, opB, m, n, k, alpha, nullptr, 0, A, ro_a, co_a, B, ro_b, co_b, beta, C, \
+                        ldc, work, stream);                                                                             \
+        });                                                                                                             \
+    }
+RBH_MXMM(f32, MX4_F32, float)
+RBH_MXMM(f16, MX4_F16, uint16_t)
+RBH_MXMM(bf16, MX4_BF16, uint16_t)
 }  // extern "C"

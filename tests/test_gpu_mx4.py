@@ -1,0 +1,529 @@
+"""GPU tests of the 4-bit microscaled operators (mx4_quantize, mx4_dequantize, mxmm) against 64-bit numpy.
+
+Tolerances. Quantisation and its inverse are exact: codes, scales and values are compared bitwise. A
+product whose dense factor holds small integers and whose scales are 2^0 .. 2^3 has sums below 2^24, so
+every order of summation is exact: compared bitwise as well. Products of random numbers: a sum of k
+products in 32 bits is within (k + 2) 2^-24 of the sum of magnitudes, whatever the order (k - 1 additions
+and the product's own rounding, one each for alpha and for the final addition of beta C), and the result
+is rounded once to its type, half a step (eps / 2).
+"""
+import numpy as np
+import pytest
+import torch
+
+import mx4_reference as R
+import randblas_amd as rb
+
+pytestmark = pytest.mark.gpu
+
+TORCH = {"f64": torch.float64, "f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def stored(a, layout, op, pad, cuda, fill=float("nan")):
+    """A buffer that holds A with op(A) = a (a tensor of the type under test), rows padded by `pad`, and lda."""
+    t = a if (layout == "R") == (op == "N") else a.t()
+    buf = torch.full((t.shape[0], t.shape[1] + pad), fill, dtype=a.dtype)
+    buf[:, : t.shape[1]] = t
+    return buf.to(cuda).view(-1), t.shape[1] + pad
+
+
+def unstored(buf, ld, rows, cols, layout, op):
+    """op(A) of a host copy of a buffer, and the padding."""
+    straight = (layout == "R") == (op == "N")
+    r, c = (rows, cols) if straight else (cols, rows)
+    m = buf.cpu().view(r, ld)
+    return (m[:, :c] if straight else m[:, :c].t()), m[:, c:]
+
+
+def inputs(rows, cols, t, seed):
+    g = torch.Generator().manual_seed(seed)
+    a = torch.randn(rows, cols, generator=g, dtype=torch.float64)
+    a = a * torch.exp2(torch.randint(-6, 7, (rows, 1), generator=g).double())
+    # ties and exact values too
+    pick = torch.rand(rows, cols, generator=g) < 0.3
+    a = torch.where(pick, torch.round(4 * a) / 4, a)
+    return a.to(TORCH[t])
+
+
+def empty(rows, cols, cuda, pad_codes=0, pad_scales=0):
+    nb = (cols + 31) // 32
+    return rb.MX4Matrix(rows, cols, torch.full((rows, 16 * (nb + pad_codes)), 0xAA, dtype=torch.uint8, device=cuda),
+                        torch.full((rows, nb + pad_scales), 0xAA, dtype=torch.uint8, device=cuda))
+
+
+def check_quantized(Q, x, words=None):
+    code, scale = R.quantize(x, words)
+    nb = scale.shape[1]
+    got_c, got_s = Q.codes.cpu().numpy(), Q.scales.cpu().numpy()
+    assert np.array_equal(got_s[:, :nb], scale)
+    assert np.array_equal(got_c[:, : 16 * nb], R.pack(code))
+    assert np.all(got_c[:, 16 * nb:] == 0xAA) and np.all(got_s[:, nb:] == 0xAA)   # padding untouched
+
+
+@pytest.mark.parametrize("rounding", ["nearest", "stochastic"])
+@pytest.mark.parametrize("layout,op", [("R", "N"), ("R", "T"), ("C", "N"), ("C", "T")])
+@pytest.mark.parametrize("t", ["f64", "f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols,pad", [(1, 1, 0), (3, 31, 0), (5, 64, 0), (70, 100, 3), (129, 257, 7), (64, 1024, 8)])
+def test_quantize(cuda, rows, cols, pad, t, layout, op, rounding):
+    a = inputs(rows, cols, t, rows + cols)
+    buf, lda = stored(a, layout, op, pad, cuda)
+    Q = empty(rows, cols, cuda, pad_codes=1 if pad else 0, pad_scales=pad)
+    seed = rb.RNGState(11, counter=(2 ** 32 - 3, 0, 0, 0)) if rounding == "stochastic" else None
+    nxt = rb.mx4_quantize(layout, op, rows, cols, buf, lda, Q, rounding=rounding, seed=seed)
+    torch.cuda.synchronize()
+    words = None
+    if seed:
+        words = R.philox_words(rows, cols, 11, 2 ** 32 - 3)
+        at = 2 ** 32 - 3 + rows * ((cols + 3) // 4)
+        assert nxt.counter == (at & 0xFFFFFFFF, at >> 32, 0, 0) and nxt.key == 11
+    check_quantized(Q, a.double().numpy(), words)
+
+
+@pytest.mark.parametrize("offset", [1, 3, 8])
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_quantize_unaligned(cuda, t, offset):
+    a = inputs(9, 90, t, 5)
+    buf = torch.zeros(9 * 90 + offset, dtype=TORCH[t], device=cuda)
+    buf[offset:] = a.view(-1).to(cuda)
+    Q = empty(9, 90, cuda)
+    rb.mx4_quantize("R", "N", 9, 90, buf[offset:], 90, Q)
+    check_quantized(Q, a.double().numpy())
+
+
+@pytest.mark.parametrize("layout", ["R", "C"])
+@pytest.mark.parametrize("rounding", ["nearest", "stochastic"])
+@pytest.mark.parametrize("t", ["f64", "f32", "f16", "bf16"])
+def test_quantize_special_values(cuda, t, rounding, layout):
+    """Zero and subnormal blocks, the largest numbers, every tie, infinities and NaNs, signs of zeros."""
+    big, tiny = torch.finfo(TORCH[t]).max, torch.finfo(TORCH[t]).smallest_normal
+    x = torch.zeros(14, 64, dtype=torch.float64)
+    x[1, :5] = torch.tensor([tiny, -tiny, tiny / 2, tiny / 4, tiny * 1.5])
+    x[2, :3] = torch.tensor([big, -big, big / 2])
+    x[3, 3] = float("inf")
+    x[4, 40] = float("nan")
+    x[4, :32] = 1.0
+    x[5, 0], x[5, 33] = -float("inf"), 2.0
+    x[6, :32] = torch.arange(32) / 4 - 4.0
+    x[7] = -0.0
+    x[8, :4] = torch.tensor([6.0, 6.03125, 7.96875, 5.96875])
+    x[9, :4] = torch.tensor([1e-30, 1e-38, 1e-20, 1e-39])
+    x[10, :4] = torch.tensor([4.0, 3.984375, 2.0, 1.0])
+    x[11, :3] = torch.tensor([2.0 ** -126, 2.0 ** -127, 2.0 ** -128])
+    x[12, :3] = torch.tensor([2.0 ** -149, 2.0 ** -140, -2.0 ** -149])
+    if t == "f64":
+        x[13, :5] = torch.tensor([1e300, 2.0 ** 200, 2.0 ** 127, 1.0, -1e300], dtype=torch.float64)
+        x[6, 31] = 0.25 + 2.0 ** -50   # just above a tie: a rounding to 32 bits on the way would lose it
+        x[6, 30] = 0.25 - 2.0 ** -50
+        x[6, 29] = -1e-300
+    a = x.to(TORCH[t])
+    buf, lda = stored(a, layout, "N", 0, cuda)
+    Q = empty(14, 64, cuda)
+    seed = rb.RNGState(5) if rounding == "stochastic" else None
+    rb.mx4_quantize(layout, "N", 14, 64, buf, lda, Q, rounding=rounding, seed=seed)
+    check_quantized(Q, a.double().numpy(), R.philox_words(14, 64, 5) if seed else None)
+
+
+def test_quantize_threefry_words(cuda):
+    import oracle_lib as O
+
+    a = inputs(6, 40, "f32", 8)
+    Q = empty(6, 40, cuda)
+    st = rb.RNGState(21, key_hi=4, rng="threefry", key_ext=(9, 8))
+    rb.mx4_quantize("R", "N", 6, 40, a.to(cuda).view(-1), 40, Q, rounding="stochastic", seed=st)
+    words = np.array([[O.threefry([r * 10 + c // 4, 0, 0, 0], [21, 4, 9, 8])[c % 4] for c in range(40)] for r in range(6)])
+    check_quantized(Q, a.double().numpy(), words)
+
+
+@pytest.mark.parametrize("layout,op", [("R", "N"), ("R", "T"), ("C", "N"), ("C", "T")])
+@pytest.mark.parametrize("t", ["f64", "f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols,ro,co,pad", [(1, 1, 0, 0, 0), (40, 70, 0, 0, 0), (33, 129, 5, 32, 3), (64, 512, 1, 64, 8)])
+def test_dequantize(cuda, rows, cols, ro, co, pad, t, layout, op):
+    rng = np.random.default_rng(rows * cols + ro)
+    low, high = (112, 140) if t == "f16" else (0, 252)
+    codes, scales = R.random_mx4(rng, rows + ro, cols + co, low, high)
+    scales[0, 0] = 255
+    Q = rb.MX4Matrix(rows + ro, cols + co, torch.from_numpy(codes).to(cuda), torch.from_numpy(scales).to(cuda))
+    exp = torch.from_numpy(R.values(codes, scales, cols + co)[ro:, co:])
+    buf, lda = stored(torch.zeros(rows, cols, dtype=TORCH[t]), layout, op, pad, cuda, fill=7.0)
+    buf.fill_(7.0)
+    rb.mx4_dequantize(layout, op, rows, cols, Q, buf, lda, ro=ro, co=co)
+    got, padding = unstored(buf, lda, rows, cols, layout, op)
+    # exact in f64, f32 and bf16; f16 rounds to nearest even
+    assert torch.equal(torch.nan_to_num(got.double(), nan=123.0), torch.nan_to_num(exp.to(TORCH[t]).double(), nan=123.0))
+    assert torch.equal(torch.signbit(got), torch.signbit(exp.to(TORCH[t]))) or torch.isnan(exp).any()
+    assert torch.all(padding == 7.0)
+
+
+def test_dequantize_extreme_scales(cuda):
+    """2^-127 (a subnormal) to 2^127: 64-bit values are exact, 32-bit ones overflow to infinity."""
+    codes = np.tile(np.arange(0, 256, 16, dtype=np.uint8), (3, 1))
+    scales = np.array([[0], [254], [255]], np.uint8)
+    Q = rb.MX4Matrix(3, 32, torch.from_numpy(codes).to(cuda), torch.from_numpy(scales).to(cuda))
+    exp = torch.from_numpy(R.values(codes, scales, 32))
+    for t in ("f64", "f32", "bf16"):
+        out = torch.empty(96, dtype=TORCH[t], device=cuda)
+        rb.mx4_dequantize("R", "N", 3, 32, Q, out, 32)
+        assert torch.equal(torch.nan_to_num(out.cpu().double().view(3, 32), nan=5.0),
+                           torch.nan_to_num(exp.to(TORCH[t]).double(), nan=5.0)), t
+
+
+def test_large_offsets(cuda):
+    """Elements beyond 2^31: the last rows of a matrix of 2.2e9 elements."""
+    rows, cols = 140_000, 16_000
+    a = torch.zeros(rows * cols, dtype=torch.bfloat16, device=cuda)
+    tail = inputs(3, cols, "bf16", 1)
+    a[-3 * cols:] = tail.to(cuda).view(-1)
+    Q = rb.mx4_empty(rows, cols, device=cuda)
+    rb.mx4_quantize("R", "N", rows, cols, a, cols, Q)
+    code, scale = R.quantize(tail.double().numpy())
+    assert np.array_equal(Q.codes[-3:].cpu().numpy(), R.pack(code))
+    assert np.array_equal(Q.scales[-3:, : cols // 32].cpu().numpy(), scale)
+    a.fill_(1.0)
+    rb.mx4_dequantize("R", "N", rows, cols, Q, a, cols)
+    assert np.array_equal(a[-3 * cols:].cpu().double().numpy().reshape(3, cols), R.values(R.pack(code), scale, cols))
+    assert not a[: cols].any()
+
+
+# ---------------------------------------------------------------------------------------------
+# products
+# ---------------------------------------------------------------------------------------------
+def mx4(rng, rows, cols, cuda, low=127, high=130, scale_pad=None):
+    codes, scales = R.random_mx4(rng, rows, cols, low, high)
+    nb = scales.shape[1]
+    wide = np.full((rows, nb + (-nb % 4 if scale_pad is None else scale_pad)), 255, np.uint8)   # padding: NaN scales
+    wide[:, :nb] = scales
+    Q = rb.MX4Matrix(rows, cols, torch.from_numpy(codes).to(cuda), torch.from_numpy(wide).to(cuda))
+    return Q, R.values(codes, scales, cols)
+
+
+class Case:
+    """One product: factors, the call and its expected value in 64 bits."""
+
+    def __init__(self, cuda, side, m, n, k, t, layout, opA, opB, seed, integers, alpha=1.0, beta=0.0, pad=0, ro=0, co=0,
+                 low=127, high=130, scale_pad=None):
+        rng = np.random.default_rng(seed)
+        self.m, self.n, self.k, self.t, self.layout = m, n, k, t, layout
+        self.head = (layout, opA, opB, m, n, k, alpha)
+
+        def dense(rows, cols, op):
+            x = rng.integers(-4, 5, (rows, cols)).astype(np.float64) if integers else rng.standard_normal((rows, cols))
+            x = torch.from_numpy(x).to(TORCH[t])
+            buf, ld = stored(x, layout, op, pad, cuda)
+            return buf, ld, x.double().numpy()
+
+        def quantised(rows, cols, op):
+            r, c = (rows, cols) if op == "N" else (cols, rows)
+            Q, v = mx4(rng, r + ro, c + co, cuda, low, high, scale_pad)
+            v = v[ro:, co:]
+            return Q, (v if op == "N" else v.T)
+
+        if side == "right":
+            bufA, lda, a = dense(m, k, opA)
+            Q, b = quantised(k, n, opB)
+            self.factors = (bufA, lda, Q, ro, co)
+        elif side == "left":
+            Q, a = quantised(m, k, opA)
+            bufB, ldb, b = dense(k, n, opB)
+            self.factors = (Q, ro, co, bufB, ldb)
+        else:
+            QA, a = quantised(m, k, opA)
+            QB, b = quantised(k, n, opB)
+            self.factors = (QA, ro, co, QB, ro, co)
+        c0 = rng.integers(-4, 5, (m, n)).astype(np.float64)
+        self.beta, self.pad = beta, pad
+        self.c0 = torch.from_numpy(c0).to(TORCH[t])
+        self.exact = alpha * (a @ b) + (beta * c0 if beta else 0.0)
+        self.size = abs(alpha) * (np.abs(a) @ np.abs(b)) + abs(beta) * np.abs(c0)
+        self.new(cuda)
+
+    def new(self, cuda):
+        c = self.c0 if self.beta else torch.full_like(self.c0, float("nan"))   # beta = 0 reads nothing
+        self.C, self.ldc = stored(c, self.layout, "N", self.pad, cuda, fill=9.0)
+
+    def run(self, **kw):
+        rb.mxmm(*self.head, *self.factors, self.beta, self.C, self.ldc, **kw)
+
+    def result(self):
+        torch.cuda.synchronize()
+        got, padding = unstored(self.C, self.ldc, self.m, self.n, self.layout, "N")
+        assert torch.all(padding == 9.0)
+        return got
+
+    def check_bitwise(self):
+        got = self.result()
+        exp = torch.from_numpy(np.ascontiguousarray(self.exact)).to(TORCH[self.t])
+        bad = (got != exp).nonzero()
+        assert len(bad) == 0, (len(bad), bad[:5].tolist(), got[tuple(bad[0])], exp[tuple(bad[0])])
+
+    def check_close(self):
+        got = self.result().double().numpy()
+        bound = (self.k + 2) * 2.0 ** -24 * self.size
+        bound = bound + torch.finfo(TORCH[self.t]).eps / 2 * (np.abs(self.exact) + bound) + torch.finfo(TORCH[self.t]).smallest_normal
+        assert np.all(np.abs(got - self.exact) <= bound), np.max(np.abs(got - self.exact) / bound)
+
+
+SIZES = [(1, 1, 1), (1, 16, 32), (1, 300, 100), (2, 33, 257), (7, 64, 512), (16, 130, 96), (17, 48, 1000), (33, 200, 64),
+         (64, 64, 160), (100, 257, 130), (130, 70, 520), (257, 300, 288)]
+
+
+@pytest.mark.parametrize("side", ["right", "left"])
+@pytest.mark.parametrize("layout", ["R", "C"])
+@pytest.mark.parametrize("opA,opB", [("N", "N"), ("T", "N"), ("N", "T"), ("T", "T")])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_mixed_products_exact(cuda, t, opA, opB, layout, side):
+    """Integers: every sum is exact (|x y| <= 4 * 6 * 2^3, k <= 1000), so the results are bitwise."""
+    for i, (m, n, k) in enumerate(SIZES):
+        if side == "left":
+            m, n = n, m
+        pad, off = (0, 8, 3)[i % 3], i % 2
+        c = Case(cuda, side, m, n, k, t, layout, opA, opB, i, True, pad=pad, ro=off, co=32 * off)
+        c.run()
+        c.check_bitwise()
+
+
+@pytest.mark.parametrize("layout", ["R", "C"])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+def test_both_products_exact(cuda, t, layout):
+    """|x y| <= 36 * 2^6 in quarters, k <= 1000: sums are multiples of 1/4 below 2^22."""
+    for i, (m, n, k) in enumerate(SIZES):
+        for mm, nn in ((m, n), (n, m)):
+            c = Case(cuda, "both", mm, nn, k, t, layout, "N", "T", i, True, pad=(0, 8, 3)[i % 3], ro=i % 2, co=32 * (i % 2))
+            c.run()
+            c.check_bitwise()
+
+
+@pytest.mark.parametrize("side,opA,opB", [("right", "N", "T"), ("right", "T", "N"), ("left", "N", "T"), ("both", "N", "T")])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("alpha,beta", [(1.0, 0.0), (0.5, 1.0), (-1.25, 0.75)])
+@pytest.mark.parametrize("m,n,k", [(1, 513, 2100), (13, 200, 4096), (40, 120, 333), (200, 190, 1500)])
+def test_products_close(cuda, m, n, k, alpha, beta, t, side, opA, opB):
+    """Random numbers, scales 2^-7 .. 2^3, alpha and beta, within the bound of 32-bit sums."""
+    c = Case(cuda, side, m, n, k, t, "R", opA, opB, m + k, False, alpha=alpha, beta=beta, low=120, high=130)
+    c.run()
+    c.check_close()
+
+
+@pytest.mark.parametrize("scale_pad", [0, 1, 3])
+@pytest.mark.parametrize("side,opB", [("right", "T"), ("right", "N"), ("both", "T")])
+def test_scales_of_any_alignment(cuda, side, opB, scale_pad):
+    c = Case(cuda, side, 70, 150, 300, "bf16", "R", "N", opB, 3, True, scale_pad=scale_pad)
+    c.run()
+    c.check_bitwise()
+
+
+@pytest.mark.parametrize("opB", ["T", "N"])
+@pytest.mark.parametrize("m", [1, 20, 150])
+def test_all_bits_of_the_dense_factor(cuda, m, opB):
+    """A 4-bit factor with one +-2^e a column copies the dense one: every bit of 32 has to arrive, from
+    subnormals to the largest numbers, and an infinity or a NaN stays in its row."""
+    k = n = 96
+    rng = np.random.default_rng(m)
+    code = np.zeros((k, n), np.uint8)
+    perm = rng.permutation(k)
+    sign = rng.integers(0, 2, n)
+    code[perm, np.arange(n)] = 2 + 8 * sign   # +-1
+    q = code if opB == "N" else code.T
+    scales = np.full((q.shape[0], 3), 127, np.uint8)
+    Q = rb.MX4Matrix(*q.shape, torch.from_numpy(R.pack(np.ascontiguousarray(q))).to(cuda), torch.from_numpy(scales).to(cuda))
+    bits = rng.integers(0, 2 ** 32, (m, k), dtype=np.uint64).astype(np.uint32)
+    x = bits.view(np.float32).copy()
+    x[~np.isfinite(x)] = 1.0
+    x[np.abs(x) < 2.0 ** -110] = 3.0   # the third part of a smaller one is below the smallest 16-bit number
+    x[0, 0], x[0, 1] = np.finfo(np.float32).max, -np.finfo(np.float32).max
+    C = torch.empty(m * n, dtype=torch.float32, device=cuda)
+    rb.mxmm("R", "N", opB, m, n, k, 1.0, torch.from_numpy(x).to(cuda).view(-1), k, Q, 0, 0, 0.0, C, n)
+    exp = x[:, perm] * np.where(sign, np.float32(-1), np.float32(1))
+    assert np.array_equal(C.cpu().numpy().reshape(m, n), exp)
+    # an infinite entry: its row is +-inf in its column and NaN elsewhere (inf * 0), other rows are as before
+    if m > 1:
+        x[1, perm[5]] = np.inf
+        rb.mxmm("R", "N", opB, m, n, k, 1.0, torch.from_numpy(x).to(cuda).view(-1), k, Q, 0, 0, 0.0, C, n)
+        got = C.cpu().numpy().reshape(m, n)
+        assert np.array_equal(np.delete(got, 1, 0), np.delete(exp, 1, 0))
+        assert np.isinf(got[1, 5]) and np.all(np.isnan(np.delete(got[1], 5)))
+
+
+@pytest.mark.parametrize("side,opB", [("right", "T"), ("right", "N"), ("both", "T")])
+@pytest.mark.parametrize("m", [3, 140])
+def test_nan_scale_reaches_its_outputs_only(cuda, m, side, opB):
+    c = Case(cuda, side, m, 90, 200, "f32", "R", "N", opB, 4, True)
+    Q = c.factors[-3] if side == "both" else c.factors[2]
+    Q.scales[7, 2] = 255   # row 7, columns 64 .. 95
+    c.run()
+    got, exp = c.result().numpy(), c.exact.copy()
+    if opB == "T":
+        exp[:, 7] = np.nan
+    else:
+        exp[:, 64:90] = np.nan
+    assert np.array_equal(np.isnan(got), np.isnan(exp))
+    assert np.array_equal(got[~np.isnan(exp)], exp[~np.isnan(exp)].astype(np.float32))
+
+
+@pytest.mark.parametrize("side", ["right", "left", "both"])
+def test_alpha_zero_and_empty_contraction(cuda, side):
+    """alpha = 0 or k = 0: C = beta C, factors unread (NaN in them does not show), beta = 0 writes zeros."""
+    for k, alpha in ((64, 0.0), (0, 1.0)):
+        for beta in (0.0, 2.0):
+            c = Case(cuda, side, 5, 9, k, "f32", "C", "N", "T", 1, True, alpha=alpha, beta=beta, pad=2)
+            if side != "both" and k:
+                (c.factors[0] if side == "right" else c.factors[3]).fill_(float("nan"))
+            c.run()
+            c.check_bitwise()
+
+
+def test_large_products_agree_with_64_bits(cuda):
+    """Several tiles in each direction and a long contraction, 64-bit sums on the device."""
+    for side, m, n, k, t, opB in (("right", 500, 1000, 4128, "bf16", "T"), ("right", 700, 900, 2000, "f32", "N"),
+                                  ("both", 900, 1100, 4128, "f32", "T"), ("right", 16, 2048, 8192, "f16", "T")):
+        c = Case(cuda, side, m, n, k, t, "R", "N", opB, 2, False, low=120, high=130)
+        c.run()
+        c.check_close()
+
+
+def test_another_stream(cuda):
+    c = Case(cuda, "right", 150, 260, 500, "f32", "R", "N", "T", 6, True)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        c.run()
+    torch.cuda.current_stream().wait_stream(side)
+    c.check_bitwise()
+    c.new(cuda)
+    torch.cuda.synchronize()
+    c.run(stream=side.cuda_stream)
+    c.check_bitwise()
+
+
+@pytest.mark.parametrize("side,t,opB,m", [("right", "bf16", "T", 1), ("right", "f32", "T", 150), ("right", "f16", "N", 150),
+                                          ("right", "f32", "N", 9), ("left", "f32", "T", 150), ("both", "bf16", "T", 150),
+                                          ("both", "f32", "T", 5)])
+def test_captured_and_replayed(cuda, side, t, opB, m):
+    """Two graphs of the same stream, replayed in turn with eager calls and new inputs between them, share
+    no workspace: every replay gives the eager result."""
+    cases = [Case(cuda, side, m, 260, 1056, t, "R", "N", opB, s, True) for s in (1, 2)]
+    st, graphs = torch.cuda.Stream(), []
+    torch.cuda.synchronize()
+    for c in cases:
+        with torch.cuda.stream(st):
+            c.run()
+        torch.cuda.synchronize()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=st):
+            c.run()
+        graphs.append(g)
+    other = torch.cuda.Stream()
+    for rep in range(4):
+        for c in cases:
+            c.C.view(-1, c.ldc).fill_(float("nan") if rep % 2 else 3.0)
+        torch.cuda.synchronize()
+        with torch.cuda.stream(st):
+            graphs[0].replay()
+        with torch.cuda.stream(other):
+            graphs[1].replay()
+        torch.cuda.synchronize()
+        for c in cases:
+            c.check_bitwise()
+            c.run()
+            c.check_bitwise()
+
+
+def test_captured_call_without_a_workspace_is_refused(cuda):
+    """The C ABI without a caller's workspace, where the call needs one: an error, and the capture ends well."""
+    import ctypes
+
+    c = Case(cuda, "right", 150, 260, 1056, "f32", "R", "N", "T", 1, True)
+    A, lda, Q = c.factors[:3]
+    fn = rb.lib.rbh_mxmm_right_f32
+    head = (b"R", b"N", b"T", 150, 260, 1056, 1.0, A.data_ptr(), lda, ctypes.byref(Q._c), 0, 0, 0.0, c.C.data_ptr(), c.ldc)
+    work = rb.WorkC()
+    assert fn(*head, ctypes.byref(work), None) == rb.RBH_OK
+    st = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        rc = fn(*head, None, st.cuda_stream)
+        c.C.zero_()
+    if work.bytes:
+        assert rc == rb.RBH_ERR_REQUIRE
+        small = rb.WorkC(A.data_ptr() // 256 * 256, work.bytes - 1)
+        assert fn(*head, ctypes.byref(small), None) == rb.RBH_ERR_REQUIRE
+    else:
+        assert rc == rb.RBH_OK
+    c.run()
+    c.check_bitwise()
+
+
+def test_host_arrays(cuda):
+    """Host arrays are staged: the call is synchronous, windows are copied back."""
+    rng = np.random.default_rng(0)
+    a = rng.standard_normal((40, 70)).astype(np.float32)
+    Q = rb.MX4Matrix(40, 70, np.full((40, 64), 7, np.uint8), np.full((40, 5), 7, np.uint8))
+    if Q._c.codes % 16:
+        pytest.skip("numpy gave an unaligned block")
+    rb.mx4_quantize("R", "N", 40, 70, a.ravel(), 70, Q)
+    code, scale = R.quantize(a.astype(np.float64))
+    assert np.array_equal(Q.codes[:, :48], R.pack(code)) and np.array_equal(Q.scales[:, :3], scale)
+    assert np.all(Q.codes[:, 48:] == 7) and np.all(Q.scales[:, 3:] == 7)
+    x = rng.integers(-3, 4, (5, 70)).astype(np.float32)
+    C = np.full((5, 44), 9.0, np.float32)
+    rb.mxmm("R", "N", "T", 5, 40, 70, 1.0, x.ravel(), 70, Q, 0, 0, 0.0, C, 44)
+    v = R.values(R.pack(code), scale, 70)
+    bound = 72 * 2.0 ** -24 * (np.abs(x) @ np.abs(v.T)) * 1.01
+    assert np.all(np.abs(C[:, :40] - x @ v.T) <= bound) and np.all(C[:, 40:] == 9.0)
+    out = np.zeros((70, 40), np.float64)
+    rb.mx4_dequantize("C", "N", 40, 70, Q, out, 40)
+    assert np.array_equal(out.T, v)
+
+
+@pytest.mark.parametrize("opB", ["T", "N"])
+def test_gradient_of_the_dense_factor(cuda, opB):
+    """C = A op(B): with G the gradient of C, A's is G op(B)^T, the product with op flipped. C is linear in
+    A, so the difference quotient along D is the product of D itself; both are integers, hence exact."""
+    m, n, k = 50, 180, 140
+    rng = np.random.default_rng(3)
+    Q, v = mx4(rng, *((n, k) if opB == "T" else (k, n)), cuda)
+    a, d, g = (rng.integers(-3, 4, s).astype(np.float64) for s in ((m, k), (m, k), (m, n)))
+
+    def product(x, rows, cols, inner, op):
+        c = torch.empty(rows * cols, dtype=torch.float32, device=cuda)
+        rb.mxmm("R", "N", op, rows, cols, inner, 1.0, torch.from_numpy(x).float().to(cuda).view(-1), inner, Q, 0, 0, 0.0, c, cols)
+        return c.cpu().double().numpy().reshape(rows, cols)
+
+    grad = product(g, m, k, n, "N" if opB == "T" else "T")
+    assert np.array_equal(grad, g @ (v if opB == "T" else v.T))
+    difference = product(a + d, m, n, k, opB) - product(a, m, n, k, opB)
+    assert (g * difference).sum() == (grad * d).sum()
+
+
+def test_run_together(cuda):
+    """Two data matrices sketched by one operator, the sketches made 4-bit without bias, multiplied in 4
+    bits, and the same product with one sketch kept in 32 bits: (S A1)^T (S A2)."""
+    d, m, n1, n2 = 256, 1000, 90, 120
+    rng = np.random.default_rng(1)
+    S = rb.DenseSkOp(rb.DenseDist(d, m), rb.RNGState(7))
+    B, Q, state = [], [], S.next_state
+    for n in (n1, n2):
+        A = torch.from_numpy(rng.standard_normal(m * n).astype(np.float32)).to(cuda)
+        b = torch.empty(d * n, dtype=torch.float32, device=cuda)
+        rb.sketch_general("C", "N", "N", d, n, m, 1.0, S, A, m, 0.0, b, d)
+        q = rb.mx4_empty(n, d, device=cuda)
+        state = rb.mx4_quantize("C", "T", n, d, b, d, q, rounding="stochastic", seed=state)   # op T: a sketch's columns
+        B.append(b)
+        Q.append(q)
+    C = torch.empty(n1 * n2, dtype=torch.float32, device=cuda)
+    rb.mxmm("C", "N", "T", n1, n2, d, 1.0 / d, Q[0], 0, 0, Q[1], 0, 0, 0.0, C, n1)
+    M = torch.empty(n1 * n2, dtype=torch.float32, device=cuda)
+    rb.mxmm("C", "T", "T", n1, n2, d, 1.0 / d, B[0], d, Q[1], 0, 0, 0.0, M, n1)
+    b1, b2 = (b.cpu().double().numpy().reshape(n, d) for b, n in zip(B, (n1, n2)))
+    q1, q2 = (R.values(q.codes.cpu().numpy(), q.scales.cpu().numpy()[:, : d // 32], d) for q in Q)
+    for got, x, y in ((C, q1, q2), (M, b1, q2)):
+        got = got.cpu().double().numpy().reshape(n2, n1).T
+        assert np.all(np.abs(got - x @ y.T / d) <= (d + 2) * 2.0 ** -24 * (np.abs(x) @ np.abs(y.T)) / d + 1e-30)
+    # the words of the second matrix follow those of the first
+    at = list(S.next_state.counter)
+    first = (at[0] + (at[1] << 32)) + n1 * (d // 4)
+    code, scale = R.quantize(b2, R.philox_words(n2, d, 7, first))
+    assert np.array_equal(Q[1].codes.cpu().numpy(), R.pack(code))
+    # unbiased rounding: an element is off by less than a gap of its block (at most 2 units)
+    unit = np.repeat(2.0 ** (scale.astype(np.float64) - 127), 32, 1)
+    assert np.all(np.abs(q2 - b2) < 2 * unit)

@@ -1,0 +1,182 @@
+"""CPU tests of the 4-bit microscaled operators: the reference itself, the handle and every refusal of the
+C ABI (all of them come before any GPU work)."""
+import ctypes
+
+import numpy as np
+import pytest
+
+import mx4_reference as R
+import oracle_lib as O
+import randblas_amd as rb
+
+
+def handle(rows, cols, ld_codes=None, ld_scales=None):
+    nb = (cols + 31) // 32
+    codes = np.zeros((rows, ld_codes or max(16, 16 * nb)) if rows else (0, 16), np.uint8)
+    # numpy aligns large arrays only to 16 bytes; take an aligned start in a larger block
+    block = np.zeros(codes.size + 64, np.uint8)
+    start = -block.ctypes.data % 64
+    codes = block[start:start + codes.size].reshape(codes.shape)
+    return rb.MX4Matrix(rows, cols, codes, np.zeros((rows, ld_scales or max(1, nb)), np.uint8))
+
+
+def refused(fragment, fn, *args, **kw):
+    with pytest.raises(rb.RandBLASError) as ei:
+        fn(*args, **kw)
+    assert ei.value.code == rb.RBH_ERR_REQUIRE and fragment in str(ei.value), str(ei.value)
+
+
+def test_reference_rounds_to_nearest_even():
+    x = np.zeros((1, 32))
+    x[0, :16] = [6, 0.25, 0.26, 0.75, 0.74, 1.25, 1.26, 1.75, 2.5, 2.51, 3.5, 3.49, 5, 5.01, -0.25, -5]
+    code, scale = R.quantize(x)
+    assert scale[0, 0] == 127
+    got = R.values(R.pack(code), scale, 32)[0, :16]
+    assert got.tolist() == [6, 0, 0.5, 1, 0.5, 1, 1.5, 2, 2, 3, 4, 3, 4, 6, 0, -4]
+    assert np.signbit(got[14])
+
+
+def test_reference_words_are_the_oracles_philox():
+    w = R.philox_words(3, 10, 77)
+    for r, c in ((0, 0), (1, 3), (2, 9)):
+        assert w[r, c] == O.philox([r * 3 + c // 4, 0, 0, 0], [77, 0])[c % 4]
+
+
+def test_reference_stochastic_rounding_has_the_right_mean():
+    # 4096 rows of one row: the mean of a value between neighbours `gap` apart is off by at most
+    # 6 standard deviations of gap / 2 / sqrt(4096)
+    row = np.linspace(-7.3, 7.9, 32)
+    x = np.tile(row, (4096, 1))
+    code, scale = R.quantize(x, R.philox_words(4096, 32, 5))
+    mean = R.values(R.pack(code), scale, 32).mean(0)
+    unit = 2.0 ** (int(scale[0, 0]) - 127)
+    assert np.abs(np.abs(row) / unit).max() <= 6
+    gap = np.where(np.abs(row) / unit < 2, 0.5, np.where(np.abs(row) / unit < 4, 1.0, 2.0)) * unit
+    assert np.all(np.abs(mean - row) <= 6 * gap / 2 / 64)
+
+
+@pytest.mark.parametrize("t", ["f64", "f32"])
+def test_quantize_refusals(t):
+    dt = np.float64 if t == "f64" else np.float32
+    A = np.zeros(40 * 70, dt)
+    q = rb.mx4_quantize
+    refused("layout == 'C' || layout == 'R'", q, "X", "N", 40, 70, A, 70, handle(40, 70))
+    refused("op == 'N' || op == 'T'", q, "R", "C", 40, 70, A, 70, handle(40, 70))
+    refused("n_rows >= 0", q, "R", "N", -1, 70, A, 70, handle(40, 70))
+    refused("lda >=", q, "R", "N", 40, 70, A, 69, handle(40, 70))
+    refused("lda >=", q, "C", "N", 40, 70, A, 39, handle(40, 70))
+    refused("lda >=", q, "R", "T", 40, 70, A, 39, handle(40, 70))
+    refused("Q->n_rows == n_rows", q, "R", "N", 40, 70, A, 70, handle(41, 70))
+    refused("n_cols >= (n_cols)", q, "R", "N", 40, 70, A, 70, handle(40, 69))
+    refused("ld_codes % 16 == 0", q, "R", "N", 40, 70, A, 70, handle(40, 70, ld_codes=56))
+    refused("A != nullptr", q, "R", "N", 40, 70, Null(dt), 70, handle(40, 70))
+    with pytest.raises(ValueError):
+        q("R", "N", 40, 70, A, 70, handle(40, 70), rounding="up")
+    with pytest.raises(ValueError):
+        q("R", "N", 40, 70, A, 70, handle(40, 70), rounding="stochastic")
+    with pytest.raises(TypeError):
+        q("R", "N", 40, 70, np.zeros(2800, np.int32), 70, handle(40, 70))
+
+
+class Null:
+    """An array of a type whose address is NULL."""
+
+    def __init__(self, dtype):
+        self.dtype = np.dtype(dtype)
+
+    def data_ptr(self):
+        return 0
+
+
+def test_quantize_refusals_of_the_c_abi():
+    A = np.zeros(64, np.float32)
+    Q = handle(2, 32)
+    fn = rb.lib.rbh_mx4_quantize_f32
+    head = (b"R", b"N", 2, 32, A.ctypes.data, 32)
+    assert fn(*head, None, 0, None, None, None) == rb.RBH_ERR_REQUIRE
+    assert fn(*head, ctypes.byref(Q._c), 2, None, None, None) == rb.RBH_ERR_REQUIRE
+    assert fn(*head, ctypes.byref(Q._c), 1, None, None, None) == rb.RBH_ERR_REQUIRE
+    seed = rb.RNGState(1).c()
+    seed.rng = 7
+    assert fn(*head, ctypes.byref(Q._c), 1, ctypes.byref(seed), None, None) == rb.RBH_ERR_REQUIRE
+    for change in (dict(codes=Q._c.codes + 8), dict(codes=None), dict(scales=None), dict(ld_codes=0),
+                   dict(ld_codes=1 << 24), dict(ld_scales=0), dict(ld_scales=1 << 24), dict(n_rows=-1)):
+        c = rb.MX4MatrixC(2, 32, Q._c.codes, 16, Q._c.scales, 1)
+        for k, v in change.items():
+            setattr(c, k, v)
+        assert fn(*head, ctypes.byref(c), 0, None, None, None) == rb.RBH_ERR_REQUIRE, change
+
+
+def test_dequantize_refusals():
+    A = np.zeros(40 * 70, np.float32)
+    d = rb.mx4_dequantize
+    refused("layout == 'C'", d, "x", "N", 40, 70, handle(40, 70), A, 70)
+    refused("lda >=", d, "R", "N", 40, 70, handle(40, 70), A, 69)
+    refused("n_rows >= (n_rows) + (ro)", d, "R", "N", 40, 70, handle(40, 70), A, 70, ro=1)
+    refused("n_cols >= (n_cols) + (co)", d, "R", "N", 40, 70, handle(40, 70), A, 70, co=32)
+    refused("(co) % 32 == 0", d, "R", "N", 40, 8, handle(40, 70), A, 70, co=16)
+    refused("(ro) >= 0", d, "R", "N", 40, 8, handle(40, 70), A, 70, ro=-1)
+    refused("A != nullptr", d, "R", "N", 40, 70, handle(40, 70), Null(np.float32), 70)
+
+
+def test_product_refusals():
+    A, C = np.zeros(5 * 64, np.float32), np.zeros(5 * 9, np.float32)
+    B = handle(9, 64)
+    mm = rb.mxmm
+    refused("layout == 'C'", mm, "x", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 9)
+    refused("opA == 'N'", mm, "R", "x", "T", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 9)
+    refused("opB == 'N'", mm, "R", "N", "x", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 9)
+    refused("m >= 0", mm, "R", "N", "T", -5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 9)
+    refused("ldc >=", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 8)
+    refused("ldd >=", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 63, B, 0, 0, 0.0, C, 9)
+    refused("n_cols >= (cols_B) + (co_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 32, 0.0, C, 9)
+    refused("n_rows >= (rows_B) + (ro_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 1, 0, 0.0, C, 9)
+    refused("(co_b) % 32 == 0", mm, "R", "N", "T", 5, 9, 32, 1.0, A, 64, B, 0, 8, 0.0, C, 9)
+    refused("n_rows >= (rows_A) + (ro_a)", mm, "R", "N", "N", 10, 5, 64, 1.0, B, 0, 0, A, 5, 0.0, np.zeros(50, np.float32), 5)
+    refused("D != nullptr", mm, "R", "N", "T", 5, 9, 64, 1.0, Null(np.float32), 64, B, 0, 0, 0.0, C, 9)
+    refused("opA == 'N' && opB == 'T'", mm, "R", "N", "N", 9, 64, 9, 1.0, handle(9, 9), 0, 0, B, 0, 0, 0.0,
+            np.zeros(9 * 64, np.float32), 64)
+    with pytest.raises(TypeError):   # no 64-bit products
+        mm("R", "N", "T", 5, 9, 64, 1.0, A.astype(np.float64), 64, B, 0, 0, 0.0, C.astype(np.float64), 9)
+    with pytest.raises(TypeError):   # one type
+        mm("R", "N", "T", 5, 9, 64, 1.0, A.astype(np.float16), 64, B, 0, 0, 0.0, C, 9)
+    with pytest.raises(TypeError):   # a 4-bit factor
+        mm("R", "N", "T", 5, 9, 64, 1.0, A, 64, A, 0, 0, 0.0, C, 9)
+
+
+def test_null_result_is_refused():
+    A, B = np.zeros(5 * 64, np.float32), handle(9, 64)
+    refused("C != nullptr", rb.mxmm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, Null(np.float32), 9)
+
+
+def test_handle_checks_its_arrays():
+    ok = np.zeros((4, 48), np.uint8)
+    with pytest.raises(TypeError):
+        rb.MX4Matrix(4, 70, ok.astype(np.int8), ok)
+    with pytest.raises(TypeError):
+        rb.MX4Matrix(4, 70, ok.ravel(), ok)
+    with pytest.raises(ValueError):
+        rb.MX4Matrix(4, 97, ok, ok)
+    with pytest.raises(ValueError):
+        rb.MX4Matrix(5, 70, ok, np.zeros((5, 3), np.uint8))
+    with pytest.raises(ValueError):
+        rb.MX4Matrix(4, 70, ok, np.zeros((4, 2), np.uint8))
+    with pytest.raises(ValueError):
+        rb.MX4Matrix(4, 20, np.zeros((4, 64), np.uint8)[:, ::2], ok)
+    assert rb.MX4Matrix(4, 70, np.zeros((4, 64), np.uint8), ok)._c.ld_codes == 64
+    one = np.zeros((1, 16), np.uint8)[:, :16]
+    assert rb.MX4Matrix(1, 32, one, one)._c.ld_codes == 16
+
+
+def test_next_state_of_stochastic_rounding_carries():
+    # an empty matrix reads no words and needs no GPU
+    st = rb.mx4_quantize("R", "N", 0, 70, np.zeros(0, np.float32), 70, handle(0, 70), rounding="stochastic",
+                         seed=rb.RNGState(3, counter=(5, 0, 0, 0)))
+    assert st.counter == (5, 0, 0, 0) and st.key == 3
+
+
+@pytest.mark.parametrize("m,n,k", [(0, 9, 64), (5, 0, 64), (0, 0, 0)])
+def test_empty_products(m, n, k):
+    C = np.full(64, 7.0, np.float32)
+    rb.mxmm("R", "N", "T", m, n, k, 1.0, np.zeros(512, np.float32), max(k, 1), handle(n, k), 0, 0, 0.0, C, max(n, 1))
+    assert np.all(C == 7.0)
