@@ -408,9 +408,10 @@ int rbh_sksy_tri_ex_f32(char layout, char side, char uplo, char A_fmt, int64_t d
  *   scales + r * ld_scales: one byte a block.
  * The codes of the last block past n_cols are zero (rbh_mx4_quantize_* writes them so); bytes between
  * rows are never read for a result nor written. codes and ld_codes are multiples of 16, scales may have
- * any alignment (multiples of 4 for both scales and ld_scales spare a product a copy of them); ld_codes
- * and ld_scales are at most 2^23. Device
- * or host memory, as for every matrix; all device arrays of a call are on one device. */
+ * any alignment. (Where scales and ld_scales are multiples of 4, products read whole words of 4 scales,
+ * otherwise they copy them first.) ld_codes
+ * and ld_scales are at most 2^22. Device or host memory, as for every matrix; all device arrays
+ * of a call are on one device. */
 typedef struct rbh_mx4 {
     int64_t n_rows, n_cols;
     uint8_t *codes;

@@ -1902,8 +1902,8 @@ int mx4_window(Stager &st, const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t row
     RBH_REQUIRE((ro) >= 0 && (co) >= 0 && (co) % 32 == 0);              \
     RBH_REQUIRE((Q)->n_rows >= (rows) + (ro));                          \
     RBH_REQUIRE((Q)->n_cols >= (cols) + (co));                          \
-    RBH_REQUIRE((Q)->ld_codes % 16 == 0 && (Q)->ld_codes <= (1 << 23)); \
-    RBH_REQUIRE((Q)->ld_scales <= (1 << 23));                           \
+    RBH_REQUIRE((Q)->ld_codes % 16 == 0 && (Q)->ld_codes <= (1 << 22)); \
+    RBH_REQUIRE((Q)->ld_scales <= (1 << 22));                           \
     RBH_REQUIRE((Q)->ld_codes >= 16 * mx4_blocks((Q)->n_cols));         \
     RBH_REQUIRE((Q)->ld_scales >= mx4_blocks((Q)->n_cols));             \
     RBH_REQUIRE((uintptr_t)(Q)->codes % 16 == 0)
