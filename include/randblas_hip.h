@@ -463,7 +463,7 @@ int rbh_mx4_dequantize_bf16(char layout, char op, int64_t n_rows, int64_t n_cols
 /* C (m x n) = alpha op(A) op(B) + beta C, sums in 32 bits. right: B is submat(B) of a 4-bit matrix at
  * (ro_b, co_b), as the sparse factor of rbh_spmm_right_*; left: A is; both: both are, and their blocks
  * have to lie along the contraction (opA = 'N', opB = 'T'). Column offsets are multiples of 32. The
- * dense factor and C have one type; the dense factor enters the sums with all its bits. The gradient of
+ * dense factor and C have one type, k is at most 2^21; the dense factor enters the sums with all its bits. The gradient of
  * a product's dense factor is the product of C's gradient with op flipped on the 4-bit one. C overlaps
  * no other array. */
 int rbh_mxmm_right_f32(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const float *A,

@@ -1994,7 +1994,7 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
     RBH_REQUIRE(layout == 'C' || layout == 'R');
     RBH_REQUIRE(opA == 'N' || opA == 'T');
     RBH_REQUIRE(opB == 'N' || opB == 'T');
-    RBH_REQUIRE(m >= 0 && n >= 0 && k >= 0);
+    RBH_REQUIRE(m >= 0 && n >= 0 && k >= 0 && k <= (1 << 21));
     const int64_t rows_A = opA == 'N' ? m : k, cols_A = opA == 'N' ? k : m;
     const int64_t rows_B = opB == 'N' ? k : n, cols_B = opB == 'N' ? n : k;
     RBH_REQUIRE(ldc >= (layout == 'C' ? m : n));

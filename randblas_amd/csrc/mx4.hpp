@@ -14,7 +14,7 @@ enum Mx4Type : int { MX4_F64 = 0, MX4_F32 = 1, MX4_F16 = 2, MX4_BF16 = 3 };
 inline int mx4_size(int type) { return type == MX4_F64 ? 8 : type == MX4_F32 ? 4 : 2; }
 
 constexpr int MX4_BLOCK = 32;
-inline int64_t mx4_blocks(int64_t cols) { return (cols + MX4_BLOCK - 1) / MX4_BLOCK; }
+__host__ __device__ inline int64_t mx4_blocks(int64_t cols) { return (cols + MX4_BLOCK - 1) / MX4_BLOCK; }
 
 // rows x cols window of a 4-bit matrix that starts at a block; ldq / lds: bytes between rows
 struct Mx4View {

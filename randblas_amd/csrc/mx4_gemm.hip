@@ -1,4 +1,6 @@
 // mx4_gemm.hip -- products with 4-bit microscaled matrices (gfx950).
+#include <type_traits>
+
 #include "common.hpp"
 #include "mx4.hpp"
 
@@ -9,58 +11,6 @@ template <int TYPE> struct Elem;
 template <> struct Elem<MX4_F32> { typedef float mem; };
 template <> struct Elem<MX4_F16> { typedef _Float16 mem; };
 template <> struct Elem<MX4_BF16> { typedef __bf16 mem; };
-
-__device__ __forceinline__ float scale_f32(uint32_t s) {
-    return __builtin_bit_cast(float, s == 255 ? 0x7FC00000u : s == 0 ? 0x00400000u : s << 23);
-}
-__device__ __forceinline__ float value(const Mx4View &Q, int64_t r, int64_t c) {
-    const uint32_t byte = Q.codes[r * Q.ldq + (c >> 1)], code = (c & 1) ? byte >> 4 : byte & 15u;
-    const uint32_t m = code & 7u;
-    // 0, 0.5, 1, 1.5, 2, 3, 4, 6 in halves, 4 bits each
-    const float v = 0.5f * (float)((0xC8643210u >> (4 * m)) & 15u);
-    return (code & 8u ? -v : v) * scale_f32(Q.scales[r * Q.lds + (c >> 5)]);
-}
-
-// One 64 x 64 tile of C a workgroup, 4 x 4 entries a thread, both factors decoded to 32 bits in LDS, one
-// block of 32 at a time; a block's sum is formed apart and added to the total.
-template <int TYPE>
-__global__ __launch_bounds__(256) void product_plain_kernel(Mx4Product p) {
-    typedef typename Elem<TYPE>::mem T;
-    __shared__ float xs[32][65], ys[32][65];
-    const int64_t i0 = (int64_t)blockIdx.x * 64, j0 = (int64_t)blockIdx.y * 64;
-    const int ti = threadIdx.x & 15, tj = threadIdx.x >> 4;
-    float acc[4][4] = {};
-    const T *x = (const T *)p.X.ptr;
-    for (int64_t k0 = 0; k0 < p.K; k0 += 32) {
-        for (int t = threadIdx.x; t < 64 * 32; t += 256) {
-            const int o = t & 63, kk = t >> 6;
-            const int64_t i = i0 + o, j = j0 + o, k = k0 + kk;
-            float xv = 0.f, yv = 0.f;
-            if (i < p.M && k < p.K) xv = (float)x[i * p.X.sr + k * p.X.sc];
-            if (j < p.N && k < p.K) yv = p.yt ? value(p.Y, k, j) : value(p.Y, j, k);
-            xs[kk][o] = xv;
-            ys[kk][o] = yv;
-        }
-        __syncthreads();
-        float part[4][4] = {};
-        for (int kk = 0; kk < 32; ++kk)
-            for (int a = 0; a < 4; ++a)
-                for (int b = 0; b < 4; ++b) part[a][b] += xs[kk][ti + 16 * a] * ys[kk][tj + 16 * b];
-        for (int a = 0; a < 4; ++a)
-            for (int b = 0; b < 4; ++b) acc[a][b] += part[a][b];
-        __syncthreads();
-    }
-    T *C = (T *)p.C;
-    for (int a = 0; a < 4; ++a)
-        for (int b = 0; b < 4; ++b) {
-            const int64_t i = i0 + ti + 16 * a, j = j0 + tj + 16 * b;
-            if (i >= p.M || j >= p.N) continue;
-            T &c = C[i * p.ci + j * p.cj];
-            float v = p.alpha * acc[a][b];
-            if (p.beta != 0.f) v += p.beta * (float)c;
-            c = (T)v;
-        }
-}
 
 // ---------------------------------------------------------------------------------------------
 // Two 4-bit factors on the scaled matrix instruction
@@ -106,6 +56,12 @@ template <typename T> __device__ __forceinline__ void store4(const Out &o, int64
         for (int i = 0; i < 4; ++i)
             if (p + i < o.np) c[i] = (T)(o.beta != 0.f ? o.alpha * v[i] + o.beta * (float)c[i] : o.alpha * v[i]);
     }
+}
+
+// partial sums (f32) where there are any, the result otherwise
+template <typename T> __device__ __forceinline__ void put4(const Out &o, const float *partial, int64_t p, int64_t q, v4f v) {
+    if (partial) store4<float>(o, p, q, v);
+    else store4<T>(o, p, q, v);
 }
 
 // A range of memory for loads straight to LDS (16 bytes a lane, lane after lane from `lds`, which is the
@@ -297,6 +253,319 @@ template <int TYPE> hipError_t both_t(const Mx4Product &q, uint8_t *work, hipStr
     return launch_both_tile<T, 128, 128, 64, 64>(P, O, out, s);
 }
 
+// ---------------------------------------------------------------------------------------------
+// One dense and one 4-bit factor on the bf16 matrix instruction
+// ---------------------------------------------------------------------------------------------
+// A product of E2M1 and a power of two is a bf16 number, so the 4-bit factor enters exactly. The dense one
+// enters as a sum of bf16 planes with all its bits: bf16 is one plane, f16 two (11 bits), f32 three (24
+// bits, cut off from the top 8 at a time: each remainder is exact, and 3 bf16 products at 2.5 PFLOP/s are
+// 5 times the f32 instruction's rate). Sums are f32.
+typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
+typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
+
+__device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
+}
+// 8 codes as bf16 times the scale, a float of which the exponent counts (0: 2^-127, 255: NaN)
+__device__ __forceinline__ v4u decode_bf16(uint32_t w, float scale) {
+    v4u r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
+    r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
+    r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+    return r;
+}
+
+template <typename T> struct Planes { static constexpr int N = 1; };
+template <> struct Planes<_Float16> { static constexpr int N = 2; };
+template <> struct Planes<float> { static constexpr int N = 3; };
+
+// x as a sum of bf16 numbers (their bits); an infinity or a NaN is the first one alone
+template <int PL> __device__ __forceinline__ void split(float x, uint32_t *b) {
+    const uint32_t u = __builtin_bit_cast(uint32_t, x);
+    const bool finite = (u & 0x7F800000u) != 0x7F800000u;
+    b[0] = u >> 16;
+    if (!finite && (u & 0x7FFFFFu)) b[0] |= 0x40u;   // a NaN stays one without its low bits
+    float r = x - __builtin_bit_cast(float, u & 0xFFFF0000u);
+#pragma unroll
+    for (int i = 1; i < PL; ++i) {
+        const uint32_t v = __builtin_bit_cast(uint32_t, r);
+        b[i] = finite ? v >> 16 : 0u;
+        r = r - __builtin_bit_cast(float, v & 0xFFFF0000u);
+    }
+}
+__device__ __forceinline__ uint32_t bf16_bits(__bf16 x) { return __builtin_bit_cast(unsigned short, x); }
+
+// The planes of a dense factor in a workspace: plane i of element (r, c) at out[(i * rows + r) * ld + c], ld a
+// multiple of 64, zeros behind the last column. One thread makes 8 columns of a row; with COLS the rows
+// are contiguous in memory, and lanes go along them.
+template <typename T, bool COLS>
+__global__ __launch_bounds__(256) void planes_kernel(const T *__restrict__ x, int64_t stride, int64_t rows, int64_t cols,
+                                                     int64_t ld, uint16_t *__restrict__ out) {
+    constexpr int PL = Planes<T>::N;
+    const int64_t n8 = ld / 8;
+    int64_t r, c8;
+    if (COLS) {
+        r = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
+        c8 = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
+    } else {
+        r = blockIdx.y;
+        c8 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    }
+    for (; COLS ? r < rows && c8 < n8 : r < rows && c8 < n8;) {
+        uint32_t b[8][PL];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int64_t c = c8 * 8 + i;
+            const T v = c < cols ? (COLS ? x[c * stride + r] : x[r * stride + c]) : (T)0.f;
+            if constexpr (PL == 1) b[i][0] = bf16_bits(v);
+            else split<PL>((float)v, b[i]);
+        }
+#pragma unroll
+        for (int q = 0; q < PL; ++q) {
+            v4u w;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = b[2 * i][q] | b[2 * i + 1][q] << 16;
+            *(v4u *)(out + ((int64_t)q * rows + r) * ld + c8 * 8) = w;
+        }
+        if (COLS) c8 += (int64_t)gridDim.y * 4;
+        else r += gridDim.y;
+    }
+}
+
+// A dense factor as the product kernels read it: bf16 planes, rows of `chunks` 16-byte pieces, ld elements apart
+struct Dense16 {
+    const uint16_t *ptr;
+    int64_t rows, ld, plane;
+    int chunks;
+};
+
+// BQ rows (YT: columns) of the 4-bit factor x BD rows of the dense one a workgroup, WQ x WD a wave; 64
+// elements of the contraction a step, loaded straight to LDS, double-buffered.
+//
+// A step's two matrix instructions take their 32 elements from all over the 64: lane group g holds
+// elements 16 g + 8 t .. + 7 of both factors for instruction t, so a lane's 16 codes lie in one word pair
+// and under one scale.
+//   dense: rows of 128 bytes, 16-byte pieces at place piece ^ (row / 2 & 7), a plane after the other
+//   codes, blocks along the contraction: rows of 32 bytes, halves exchanged in 8 of 16 rows; scales: words
+//   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes a word (8 columns 8 c .. +
+//     7) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 8
+//     operands are then columns 8 c + f, and the operand f of the wave is columns f, f + 8, .. -- an order of
+//     the result's rows or columns that the stores undo. Scales are kept as the upper halves of floats.
+template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, bool QFIRST>
+__global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
+                                                                                   Out out, float *partial) {
+    constexpr int NW = (BQ / WQ) * (BD / WD), NT = NW * 64;
+    constexpr int FQ = WQ / 16, FD = WD / 16;
+    constexpr int LD = BD * 8 / NT;
+    static_assert(BD * 8 % NT == 0 && NT / 8 % 16 == 0, "whole loads of the dense rows");
+    static_assert(BQ * 2 == NT, "one load of codes a thread");
+    static_assert(!YT || WQ == 128, "8 columns a lane");
+    constexpr int DENSE = PL * BD * 128;
+    constexpr int PITCH = YT ? (BQ == 256 ? 1056 : 1088) : 1024;   // 64 lanes' codes; lane groups on different banks
+    constexpr int CODES = NW * PITCH;
+    constexpr int SCALES = YT ? BQ / 32 * 128 : BQ * 4;
+    constexpr int STAGE = DENSE + CODES + SCALES;
+    static_assert(2 * STAGE <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) uint8_t lds0[STAGE], lds1[STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    const int64_t nq = YT ? Y.cols : Y.rows;
+    uint32_t iq, id;
+    tile_of(blockIdx.x, (uint32_t)((nq + BQ - 1) / BQ), (uint32_t)((D.rows + BD - 1) / BD), iq, id);
+    const int64_t q0 = (int64_t)iq * BQ, d0 = (int64_t)id * BD;
+    const int wq = wave % (BQ / WQ), wd = wave / (BQ / WQ);
+    const int nd = (int)(D.rows - d0 < BD ? D.rows - d0 : BD), mq = (int)(nq - q0 < BQ ? nq - q0 : BQ);
+    const int steps = (int)((K + 63) / 64), s0 = blockIdx.y * steps_z, s1 = s0 + steps_z < steps ? s0 + steps_z : steps;
+
+    Buffer db[PL];
+#pragma unroll
+    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane + d0 * D.ld, (uint32_t)((nd - 1) * D.ld * 2 + D.chunks * 16));
+    const int piece = (tid & 7) ^ ((tid >> 4) & 7);
+    const uint32_t vd = (uint32_t)((tid >> 3) * D.ld * 2) + piece * 16, rd = (uint32_t)(D.ld * 2) * (NT / 8);
+    // codes and scales
+    const int nb = (int)mx4_blocks(YT ? mq : Y.cols);   // blocks a row (YT: of this tile)
+    Buffer qb, sb;
+    uint32_t vq, vs;
+    int qpart;
+    if constexpr (YT) {
+        constexpr int PR = BQ / 32;                       // pieces a row
+        qpart = lane % PR;
+        vq = (uint32_t)((wave * (64 / PR) + lane / PR) * Y.ldq) + qpart * 16;
+        vs = 0;
+    } else {
+        qb = buffer(Y.codes + q0 * Y.ldq, (uint32_t)((mq - 1) * Y.ldq + nb * 16));
+        sb = buffer(Y.scales + q0 * Y.lds, (uint32_t)((mq - 1) * Y.lds + (nb + 3) / 4 * 4));
+        qpart = (lane & 1) ^ ((lane >> 4) & 1);           // rows 8-15 of 16: halves exchanged
+        vq = (uint32_t)((wave * 32 + (lane >> 1)) * Y.ldq) + qpart * 16;
+        vs = (uint32_t)((wave * 64 + lane) * Y.lds);
+    }
+    uint32_t sreg = 0;   // YT: 4 scales of a row on their way to LDS
+    auto load = [&](int step, uint8_t *lds) {
+        if constexpr (YT) {
+            const int64_t k0 = (int64_t)step * 64;
+            const int64_t left = K - k0 < 64 ? K - k0 : 64;
+            const uint32_t rows = left > 0 ? (uint32_t)left : 0u;
+            const uint32_t have = rows ? 1u : 0u;
+            // past the last step the range is empty, and reads zeros
+            const Buffer cb = buffer(Y.codes + q0 / 2 + (have ? k0 : 0) * Y.ldq, have * ((rows - 1) * (uint32_t)Y.ldq + nb * 16));
+            const Buffer kb = buffer(Y.scales + q0 / 32 + (have ? k0 : 0) * Y.lds, have * ((rows - 1) * (uint32_t)Y.lds + (nb + 3) / 4 * 4));
+            constexpr int WR = BQ / 128;                  // words of scales a row
+            if (tid < 64 * WR) {
+                const int w = tid % WR;
+                sreg = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, w * 4 < nb ? (int)((tid / WR) * Y.lds + w * 4) : (int)OUTSIDE, 0, 0);
+            }
+            load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
+        } else {
+            load_lds16(qb, lds + DENSE + wave * PITCH, step * 2 + qpart < nb ? vq : OUTSIDE, step * 32);
+            if (wave < BQ / 64) load_lds4(sb, lds + DENSE + CODES + wave * 256, step * 2 < nb ? vs : OUTSIDE, step * 2 / 4 * 4);
+        }
+        const bool in = step * 8 + piece < D.chunks;
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int i = 0; i < LD; ++i)
+                load_lds16(db[p], lds + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
+    };
+    auto put_scales = [&](uint8_t *lds) {
+        if constexpr (YT) {
+            constexpr int WR = BQ / 128;
+            if (tid < 64 * WR) {
+                uint16_t *s = (uint16_t *)(lds + DENSE + CODES) + (tid % WR) * 4 * 64 + tid / WR;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i * 64] = (uint16_t)(((sreg >> (8 * i)) & 255u) << 7);
+            }
+        }
+    };
+    // the loads have arrived (for YT the scales of the next step too), every wave is done with this step
+    auto next = [&](uint8_t *lds) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        put_scales(lds);
+        __syncthreads();
+    };
+
+    v4f acc[FQ][FD];
+#pragma unroll
+    for (int a = 0; a < FQ; ++a)
+#pragma unroll
+        for (int b = 0; b < FD; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    int dat[2];
+#pragma unroll
+    for (int t = 0; t < 2; ++t) dat[t] = wd * WD * 128 + r16 * 128 + ((g * 2 + t) ^ ((r16 >> 1) & 7)) * 16;
+    auto compute = [&](int step, const uint8_t *lds) {
+        v2u raw[YT ? 1 : FQ];
+        float scale[YT ? 1 : FQ];
+        if constexpr (!YT) {
+            const uint8_t *cq = lds + (DENSE + (wq * WQ + r16) * 32 + ((g * 8) ^ ((r16 >> 3) * 16)));
+            const uint8_t *sq = lds + (DENSE + CODES + (wq * WQ + r16) * 4);
+            const int bit = (step & 1) * 16 + (g >> 1) * 8;
+            const uint32_t width = step * 2 + (g >> 1) < nb ? 8 : 0;   // past the last block, whatever is there, as 0
+#pragma unroll
+            for (int f = 0; f < FQ; ++f) {
+                raw[f] = *(const v2u *)(cq + f * 16 * 32);
+                scale[f] = __builtin_bit_cast(float, __builtin_amdgcn_ubfe(*(const uint32_t *)(sq + f * 16 * 4), bit, width) << 23);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            v4u d[PL][FD];
+            const uint8_t *dp = lds + dat[t];
+#pragma unroll
+            for (int p = 0; p < PL; ++p)
+#pragma unroll
+                for (int f = 0; f < FD; ++f) d[p][f] = *(const v4u *)(dp + (p * BD + f * 16) * 128);
+            v4u q[FQ];
+            if constexpr (YT) {
+                constexpr int ROW = BQ / 2;               // bytes of codes a row; rows 16 g + 8 t .. + 7 are in one piece
+                const uint8_t *cq = lds + (DENSE + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 64 + r16 * 4);
+                const uint8_t *sq = lds + (DENSE + CODES + (wq * 4 + (r16 >> 2)) * 128 + g * 32 + t * 16);
+                const v4u sc = *(const v4u *)sq;
+                v4u row[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const uint32_t half = (j & 1) ? sc[j >> 1] & 0xFFFF0000u : sc[j >> 1] << 16;
+                    row[j] = decode_bf16(*(const uint32_t *)(cq + j * ROW), __builtin_bit_cast(float, half));
+                }
+#pragma unroll
+                for (int f = 0; f < FQ; ++f)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)           // rows 2 j, 2 j + 1 of column f
+                        q[f][j] = __builtin_amdgcn_perm(row[2 * j + 1][f >> 1], row[2 * j][f >> 1], (f & 1) ? 0x07060302u : 0x05040100u);
+            } else {
+#pragma unroll
+                for (int f = 0; f < FQ; ++f) q[f] = decode_bf16(raw[f][t], scale[f]);
+            }
+#pragma unroll
+            for (int fq = 0; fq < FQ; ++fq)
+#pragma unroll
+                for (int p = 0; p < PL; ++p)
+#pragma unroll
+                    for (int fd = 0; fd < FD; ++fd)
+                        acc[fq][fd] = QFIRST ? mfma_bf16(q[fq], d[p][fd], acc[fq][fd]) : mfma_bf16(d[p][fd], q[fq], acc[fq][fd]);
+        }
+    };
+    load(s0, lds0);
+    next(lds0);
+    int st = s0;
+    for (; st + 1 < s1; st += 2) {
+        load(st + 1, lds1);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(st, lds0);
+        next(lds1);
+        load(st + 2, lds0);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(st + 1, lds1);
+        next(lds0);
+    }
+    if (st < s1) compute(st, lds0);
+
+    // entry i of a lane's 4: QFIRST: 4-bit index 4 g + i, dense r16; otherwise the other way round
+    const Out to = partial ? Out{partial + (int64_t)blockIdx.y * out.np * out.no, out.np, out.np, out.no, 1.f, 0.f, out.np % 4 == 0} : out;
+#pragma unroll
+    for (int fd = 0; fd < FD; ++fd)
+#pragma unroll
+        for (int fq = 0; fq < FQ; ++fq) {
+            const int64_t dd = d0 + wd * WD + fd * 16;
+            if constexpr (!YT) {
+                const int64_t qq = q0 + wq * WQ + fq * 16;
+                if constexpr (QFIRST) put4<T>(to, partial, qq + 4 * g, dd + r16, acc[fq][fd]);
+                else put4<T>(to, partial, dd + 4 * g, qq + r16, acc[fq][fd]);
+            } else if constexpr (!QFIRST) {
+                put4<T>(to, partial, dd + 4 * g, q0 + wq * WQ + r16 * 8 + fq, acc[fq][fd]);
+            }
+        }
+    if constexpr (YT && QFIRST) {   // columns 8 (4 g + i) + fq: 8 operands make 8 consecutive ones
+#pragma unroll
+        for (int fd = 0; fd < FD; ++fd)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const v4f v{acc[4 * h][fd][i], acc[4 * h + 1][fd][i], acc[4 * h + 2][fd][i], acc[4 * h + 3][fd][i]};
+                    put4<T>(to, partial, q0 + wq * WQ + (4 * g + i) * 8 + 4 * h, d0 + wd * WD + fd * 16 + r16, v);
+                }
+    }
+}
+
+// C = alpha * (the sum of the slices' partial sums, in their order) + beta * C
+template <typename T>
+__global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, int slices, Out out) {
+    const int64_t n4 = (out.np + 3) / 4, plane = out.np * out.no;
+    for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n4 * out.no; t += (int64_t)gridDim.x * 256) {
+        const int64_t q = t / n4, p = (t - q * n4) * 4;
+        const float *x = partial + q * out.np + p;
+        v4f sum{0.f, 0.f, 0.f, 0.f};
+        for (int z = 0; z < slices; ++z)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (p + i < out.np) sum[i] += x[z * plane + i];
+        store4<T>(out, p, q, sum);
+    }
+}
+
 // C = beta C (beta = 0: zeros, whatever C holds)
 template <int TYPE> __global__ __launch_bounds__(256) void scale_kernel(Mx4Product p, int64_t inner, int64_t outer, int64_t ld) {
     typedef typename Elem<TYPE>::mem T;
@@ -308,6 +577,97 @@ template <int TYPE> __global__ __launch_bounds__(256) void scale_kernel(Mx4Produ
     }
 }
 
+// How a mixed product runs
+struct MixedPlan {
+    bool direct;         // the dense factor is read as it is
+    int64_t ld;          // of its planes otherwise
+    int bq, bd;          // tile
+    int slices, steps_z; // of the contraction, and steps of 64 in each
+    size_t planes, partials, scales;   // workspace bytes
+};
+constexpr size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+MixedPlan mixed_plan(const Mx4Product &p) {
+    MixedPlan m{};
+    const int esz = mx4_size(p.type), pl = p.type == MX4_F32 ? 3 : p.type == MX4_F16 ? 2 : 1;
+    // 16-byte pieces of 8 elements, whole ones only, rows within reach of a 32-bit offset
+    m.direct = p.type == MX4_BF16 && p.X.sc == 1 && (uintptr_t)p.X.ptr % 16 == 0 && p.X.sr % 8 == 0 && p.K % 8 == 0 &&
+               p.X.sr <= (1 << 21);
+    m.ld = (p.K + 63) / 64 * 64;
+    if (!m.direct) m.planes = round256((size_t)pl * p.M * m.ld * 2);
+    m.scales = scales_work(p.Y);
+    const int64_t nq = p.N, nd = p.M;
+    auto tiles = [&](int64_t q, int64_t d) { return ((nq + q - 1) / q) * ((nd + d - 1) / d); };
+    m.bq = 256;
+    m.bd = 128;
+    if (pl == 1 && tiles(256, 256) >= 256) m.bd = 256;
+    else if (tiles(256, 128) < 256) m.bq = 128;
+    const int64_t steps = (p.K + 63) / 64, t = tiles(m.bq, m.bd);
+    int64_t z = 1;
+    while (t * z * 2 <= 256 && steps / (z * 2) >= 8) z *= 2;
+    m.steps_z = (int)((steps + z - 1) / z);
+    m.slices = (int)((steps + m.steps_z - 1) / m.steps_z);
+    if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
+    return m;
+}
+
+template <typename T, bool YT, int BQ, int BD, int WQ, int WD>
+hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, const MixedPlan &m, const Out &out, float *partial,
+                             bool qfirst, hipStream_t s) {
+    constexpr int PL = Planes<T>::N;
+    const int64_t nq = YT ? Y.cols : Y.rows;
+    const dim3 grid((unsigned)(((nq + BQ - 1) / BQ) * ((D.rows + BD - 1) / BD)), (unsigned)m.slices);
+    constexpr int NT = (BQ / WQ) * (BD / WD) * 64;
+    if (qfirst)
+        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, true>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+    else
+        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, false>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+    return hipGetLastError();
+}
+
+template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipStream_t s) {
+    typedef typename Elem<TYPE>::mem T;
+    const MixedPlan m = mixed_plan(q);
+    Mx4Product p = q;
+    hipError_t e = align_scales(p.Y, work, s);
+    if (e != hipSuccess) return e;
+    Dense16 D{(const uint16_t *)p.X.ptr, p.M, p.X.sr, 0, (int)(p.K / 8)};
+    if (!m.direct) {
+        uint16_t *planes = (uint16_t *)work;
+        work += m.planes;
+        const T *x = (const T *)p.X.ptr;
+        const int64_t n8 = m.ld / 8;
+        if (p.X.sc == 1)
+            hipLaunchKernelGGL((planes_kernel<T, false>), dim3((unsigned)((n8 + 255) / 256), (unsigned)(p.M < 65535 ? p.M : 65535)),
+                               dim3(256), 0, s, x, p.X.sr, p.M, p.K, m.ld, planes);
+        else
+            hipLaunchKernelGGL((planes_kernel<T, true>),
+                               dim3((unsigned)((p.M + 63) / 64), (unsigned)((n8 + 3) / 4 < 65535 ? (n8 + 3) / 4 : 65535)), dim3(256), 0, s, x,
+                               p.X.sc, p.M, p.K, m.ld, planes);
+        e = hipGetLastError();
+        if (e != hipSuccess) return e;
+        D = Dense16{planes, p.M, m.ld, p.M * m.ld, (int)n8};
+    }
+    const bool qfirst = p.cj == 1;   // the 4-bit factor's index is the contiguous one of C
+    const int64_t ld = qfirst ? p.ci : p.cj;
+    const Out out{p.C, ld, qfirst ? p.N : p.M, qfirst ? p.M : p.N, p.alpha, p.beta,
+                  (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
+    float *partial = m.slices > 1 ? (float *)work : nullptr;
+    auto go = [&](auto yt) -> hipError_t {
+        constexpr bool YT = decltype(yt)::value;
+        if constexpr (Planes<T>::N == 1)
+            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, YT ? 128 : 64, YT ? 64 : 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        return launch_mixed_tile<T, YT, 128, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+    };
+    e = p.yt ? go(std::true_type{}) : go(std::false_type{});
+    if (e != hipSuccess || !partial) return e;
+    const int64_t n = (out.np + 3) / 4 * out.no;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256 < 65536 ? (n + 255) / 256 : 65536)), dim3(256), 0, s, partial,
+                       m.slices, out);
+    return hipGetLastError();
+}
+
 template <int TYPE> hipError_t product_t(const Mx4Product &p, void *work, hipStream_t s) {
     if (p.K <= 0 || p.alpha == 0.f) {
         const int64_t inner = p.ci == 1 ? p.M : p.N, outer = p.ci == 1 ? p.N : p.M;
@@ -315,17 +675,16 @@ template <int TYPE> hipError_t product_t(const Mx4Product &p, void *work, hipStr
                            dim3(256), 0, s, p, inner, outer, p.ci == 1 ? p.cj : p.ci);
         return hipGetLastError();
     }
-    if (p.both) return both_t<TYPE>(p, (uint8_t *)work, s);
-    const dim3 grid((unsigned)((p.M + 63) / 64), (unsigned)((p.N + 63) / 64));
-    hipLaunchKernelGGL((product_plain_kernel<TYPE>), grid, dim3(256), 0, s, p);
-    return hipGetLastError();
+    return p.both ? both_t<TYPE>(p, (uint8_t *)work, s) : mixed_t<TYPE>(p, (uint8_t *)work, s);
 }
 
 }  // namespace
 
 size_t mx4_product_work(const Mx4Product &p) {
     if (p.K <= 0 || p.alpha == 0.f) return 0;
-    return p.both ? scales_work(p.XQ) + scales_work(p.Y) : 0;
+    if (p.both) return scales_work(p.XQ) + scales_work(p.Y);
+    const MixedPlan m = mixed_plan(p);
+    return m.scales + m.planes + m.partials;
 }
 
 hipError_t launch_mx4_product(const Mx4Product &p, void *work, hipStream_t s) {
