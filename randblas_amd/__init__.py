@@ -717,25 +717,39 @@ def spmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
 # --------------------------------------------------------------------------------------------
 # 4-bit microscaled matrices (MXFP4; no reference counterpart)
 # --------------------------------------------------------------------------------------------
-_MX4_TAGS = {"float64": "f64", "float32": "f32", "float16": "f16", "bfloat16": "bf16"}
+_MX4_TAGS = {np.dtype(np.float64): "f64", np.dtype(np.float32): "f32", np.dtype(np.float16): "f16"}
+_MX4_BYTES = [np.dtype(np.uint8)]
+if torch is not None:
+    _MX4_TAGS.update({torch.float64: "f64", torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"})
+    _MX4_BYTES.append(torch.uint8)
 ROUNDINGS = {"nearest": 0, "stochastic": 1}   # RBH_ROUND_*
+_MX4_QUANTIZE = {t: getattr(lib, f"rbh_mx4_quantize_{t}") for t in ("f64", "f32", "f16", "bf16")}
+_MX4_DEQUANTIZE = {t: getattr(lib, f"rbh_mx4_dequantize_{t}") for t in ("f64", "f32", "f16", "bf16")}
+_MXMM = {(side, t): getattr(lib, f"rbh_mxmm_{side}_{t}") for side in ("right", "left", "both") for t in ("f32", "f16", "bf16")}
 
 
 def _mx4_tag(x) -> str:
-    tag = _MX4_TAGS.get(str(x.dtype).removeprefix("torch."))
+    tag = _MX4_TAGS.get(x.dtype)
     if tag is None:
         raise TypeError(f"unsupported dtype {x.dtype}")
     return tag
 
 
+def _mx4_stream(x, stream):
+    """_stream without the objects it makes on the way: these calls may take less time than they do."""
+    if stream is None and getattr(x, "is_cuda", False):
+        return torch._C._cuda_getCurrentRawStream(x.device.index)
+    return stream
+
+
 def _bytes_2d(x, name, rows, width):
     """The bytes between rows of a uint8 array of at least rows x width, checked."""
-    if str(x.dtype) not in ("uint8", "torch.uint8") or len(x.shape) != 2:
+    if x.dtype not in _MX4_BYTES or x.ndim != 2:
         raise TypeError(f"{name} must be a 2-D uint8 array")
-    strides = x.strides if isinstance(x, np.ndarray) else x.stride()
+    strides, (have, wide) = x.strides if isinstance(x, np.ndarray) else x.stride(), x.shape
     if rows == 0 or width == 0:
         return width
-    if x.shape[0] < rows or x.shape[1] < width or (x.shape[1] > 1 and strides[1] != 1):
+    if have < rows or wide < width or (wide > 1 and strides[1] != 1):
         raise ValueError(f"{name} must hold {rows} rows of {width} consecutive bytes")
     return strides[0] if rows > 1 else max(strides[0], width)
 
@@ -778,19 +792,19 @@ def mx4_quantize(layout, op, n_rows, n_cols, A, lda, Q: MX4Matrix, rounding="nea
         raise ValueError(f"rounding must be one of {sorted(ROUNDINGS)}, not {rounding!r}")
     if rounding == "stochastic" and seed is None:
         raise ValueError("stochastic rounding needs a seed state")
-    sr = rounding == "stochastic"
-    nxt = RNGStateC()
-    _check(getattr(lib, f"rbh_mx4_quantize_{_mx4_tag(A)}")(
-        _b(layout), _b(op), n_rows, n_cols, _ptr(A), lda, ctypes.byref(Q._c), ROUNDINGS[rounding],
-        ctypes.byref(seed.c()) if sr else None, ctypes.byref(nxt) if sr else None, _stream(A, stream)))
-    return RNGState.from_c(nxt) if sr else None
+    state = nxt = None
+    if rounding == "stochastic":
+        state, nxt = seed.c(), RNGStateC()
+    _check(_MX4_QUANTIZE[_mx4_tag(A)](_b(layout), _b(op), n_rows, n_cols, _ptr(A), lda, Q._c, ROUNDINGS[rounding], state,
+                                      nxt, _mx4_stream(A, stream)))
+    return RNGState.from_c(nxt) if nxt is not None else None
 
 
 def mx4_dequantize(layout, op, n_rows, n_cols, Q: MX4Matrix, A, lda, ro=0, co=0, stream=None) -> None:
     """op(A) = submat(Q), n_rows x n_cols at (ro, co), co a multiple of 32 (rbh_mx4_dequantize). Exact in
     every type but f16, which rounds to nearest even."""
-    _check(getattr(lib, f"rbh_mx4_dequantize_{_mx4_tag(A)}")(_b(layout), _b(op), n_rows, n_cols, ctypes.byref(Q._c),
-                                                             ro, co, _ptr(A), lda, _stream(A, stream)))
+    _check(_MX4_DEQUANTIZE[_mx4_tag(A)](_b(layout), _b(op), n_rows, n_cols, Q._c, ro, co, _ptr(A), lda,
+                                        _mx4_stream(A, stream)))
 
 
 def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, stream=None) -> None:
@@ -808,20 +822,20 @@ def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
         ro_a, co_a = x_off_r, x_off_c_or_ld
         if isinstance(Y, MX4Matrix):
             side, (ro_b, co_b, beta, C, ldc) = "both", args
-            factors, dense = [ctypes.byref(X._c), ro_a, co_a, ctypes.byref(Y._c), ro_b, co_b], None
+            factors, dense = [X._c, ro_a, co_a, Y._c, ro_b, co_b], None
         else:
             side, (ldb, beta, C, ldc) = "left", args
-            factors, dense = [ctypes.byref(X._c), ro_a, co_a, _ptr(Y), ldb], Y
+            factors, dense = [X._c, ro_a, co_a, _ptr(Y), ldb], Y
     else:
         A, lda, B = X, x_off_r, x_off_c_or_ld
         if not isinstance(B, MX4Matrix):
             raise TypeError("mxmm needs an MX4Matrix")
         side, (ro_b, co_b, beta, C, ldc) = "right", (Y,) + args
-        factors, dense = [_ptr(A), lda, ctypes.byref(B._c), ro_b, co_b], A
+        factors, dense = [_ptr(A), lda, B._c, ro_b, co_b], A
     t = _mx4_tag(C)
     if t == "f64" or (dense is not None and dense.dtype != C.dtype):
         raise TypeError("mxmm: C and the dense factor must both be f32, both f16 or both bf16")
-    fn, st = getattr(lib, f"rbh_mxmm_{side}_{t}"), _stream(C, stream)
+    fn, st = _MXMM[side, t], _mx4_stream(C, stream)
     head = (_b(layout), _b(opA), _b(opB), m, n, k, alpha, *factors, beta, _ptr(C), ldc)
     if torch is None or not getattr(C, "is_cuda", False) or not torch.cuda.is_current_stream_capturing():
         return _check(fn(*head, None, st))

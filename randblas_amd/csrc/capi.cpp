@@ -1842,13 +1842,16 @@ namespace {
 struct DeviceOf {
     int before = -1, want = -1;
     bool differ = false;
-    void look(const void *p) {
+    // whether p is device (or managed) memory
+    bool look(const void *p) {
         hipPointerAttribute_t a;
-        if (!p) return;
-        if (hipPointerGetAttributes(&a, p) != hipSuccess) { (void)hipGetLastError(); return; }
-        if (a.type != hipMemoryTypeDevice) return;   // managed memory is reached from every device
+        if (!p) return false;
+        if (hipPointerGetAttributes(&a, p) != hipSuccess) { (void)hipGetLastError(); return false; }
+        if (a.type == hipMemoryTypeManaged) return true;   // reached from every device
+        if (a.type != hipMemoryTypeDevice) return false;
         if (want >= 0 && a.device != want) differ = true;
         want = a.device;
+        return true;
     }
     hipError_t enter() {
         if (want < 0) return hipSuccess;

@@ -550,6 +550,233 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     }
 }
 
+// Few dense rows (at most 16 DF): a workgroup takes NQ columns of the result over one slice of the
+// contraction, its 8 waves take the slice's units in turn, and each wave streams its codes from memory
+// straight to registers, so nothing but the codes' bytes bounds it: every load of a unit is issued before the
+// one before it is used, and no barrier stands between them. The waves' sums are added in LDS, in order.
+//   blocks along the contraction: unit of 256 elements; lane (r, g) holds blocks 2 g, 2 g + 1 of row r
+//   blocks across it (YT): unit of 32 rows and 256 columns; lane (c, g) holds columns 16 c .. + 15 of rows
+//     8 g .. + 7 (128 bytes of a row, whole lines, are read by 16 lanes together)
+// entry (q, d) of the result at ptr[q * sq + d * sd]; partial sums where `partial` is set
+struct RowsOut {
+    void *ptr;
+    int64_t sq, sd, nq, nd;
+    float alpha, beta;
+    float *partial;
+};
+template <typename T> __device__ __forceinline__ void put1(const RowsOut &o, int64_t q, int64_t d, float v) {
+    if (q >= o.nq || d >= o.nd) return;
+    if (o.partial) {
+        o.partial[(int64_t)blockIdx.y * o.nq * o.nd + q * o.sq + d * o.sd] = v;
+    } else {
+        T *c = (T *)o.ptr + q * o.sq + d * o.sd;
+        *c = (T)(o.beta != 0.f ? o.alpha * v + o.beta * (float)*c : o.alpha * v);
+    }
+}
+
+constexpr int ROWS_WAVES = 8;
+
+// adds the 8 waves' N operands and hands each sum to f(operand, lane, value)
+template <int N, typename F> __device__ __forceinline__ void add_waves(const v4f *acc, v4f *lds, int lane, int wave, F &&f) {
+    constexpr int C = N < 8 ? N : 8;
+    static_assert(N % C == 0, "whole rounds");
+#pragma unroll
+    for (int r = 0; r < N; r += C) {
+        if (r) __syncthreads();
+#pragma unroll
+        for (int i = 0; i < C; ++i) lds[(wave * C + i) * 64 + lane] = acc[r + i];
+        __syncthreads();
+        if (wave < C) {
+            v4f sum = lds[wave * 64 + lane];
+#pragma unroll
+            for (int w = 1; w < ROWS_WAVES; ++w) sum += lds[(w * C + wave) * 64 + lane];
+            f(r + wave, lane, sum);
+        }
+    }
+}
+
+template <typename T, int NF, int DF>
+__global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_kernel(Dense16 D, Mx4View Y, bool pairs, RowsOut out) {
+    constexpr int PL = Planes<T>::N;
+    __shared__ v4f sums[ROWS_WAVES * (NF * DF < 8 ? NF * DF : 8) * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
+    const int64_t q0 = (int64_t)blockIdx.x * (NF * 16);
+    const int nb = (int)mx4_blocks(Y.cols);
+    const int units = (nb + 7) / 8, stride = ROWS_WAVES * gridDim.y;
+    const uint8_t *cp[NF], *sp[NF];
+#pragma unroll
+    for (int f = 0; f < NF; ++f) {
+        const int64_t r = q0 + f * 16 + r16 < Y.rows ? q0 + f * 16 + r16 : Y.rows - 1;
+        cp[f] = Y.codes + r * Y.ldq + 32 * g;
+        sp[f] = Y.scales + r * Y.lds + 2 * g;
+    }
+    struct Codes {
+        v4u c[NF][2];
+        uint32_t s[NF];
+    };
+    auto load = [&](int u, Codes &x) {
+        const int b = u * 8 + 2 * g;
+#pragma unroll
+        for (int f = 0; f < NF; ++f) {
+            x.c[f][0] = b < nb ? *(const v4u *)(cp[f] + (int64_t)u * 128) : v4u{0, 0, 0, 0};
+            x.c[f][1] = b + 1 < nb ? *(const v4u *)(cp[f] + (int64_t)u * 128 + 16) : v4u{0, 0, 0, 0};
+            const uint8_t *s = sp[f] + (int64_t)u * 8;
+            if (pairs && b + 1 < nb) x.s[f] = *(const uint16_t *)s;
+            else x.s[f] = (b < nb ? s[0] : 0u) | (b + 1 < nb ? s[1] : 0u) << 8;
+        }
+    };
+    v4f acc[NF * DF];
+#pragma unroll
+    for (int i = 0; i < NF * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    // the dense rows of this lane, and how many pieces of 8 elements it may read of them
+    const uint16_t *xp[DF];
+    int have[DF];
+#pragma unroll
+    for (int d = 0; d < DF; ++d) {
+        have[d] = d * 16 + r16 < D.rows ? D.chunks : 0;
+        xp[d] = D.ptr + (have[d] ? (d * 16 + r16) * D.ld : 0);
+    }
+    auto dense = [&](int piece, v4u (&d)[DF][PL]) {
+#pragma unroll
+        for (int e = 0; e < DF; ++e)
+#pragma unroll
+            for (int i = 0; i < PL; ++i)
+                d[e][i] = piece < have[e] ? *(const v4u *)(xp[e] + i * D.plane + piece * 8) : v4u{0, 0, 0, 0};
+    };
+    auto compute = [&](int u, const Codes &x) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                v4u d[DF][PL];
+                dense(u * 32 + g * 8 + h * 4 + t, d);
+#pragma unroll
+                for (int f = 0; f < NF; ++f) {
+                    const v4u q = decode_bf16(x.c[f][h][t], __builtin_bit_cast(float, __builtin_amdgcn_ubfe(x.s[f], 8 * h, 8) << 23));
+#pragma unroll
+                    for (int e = 0; e < DF; ++e)
+#pragma unroll
+                        for (int i = 0; i < PL; ++i) acc[f * DF + e] = mfma_bf16(q, d[e][i], acc[f * DF + e]);
+                }
+            }
+        }
+    };
+    // a unit past the last is zeros
+    Codes a, b;
+    int u = blockIdx.y * ROWS_WAVES + wave;
+    load(u, a);
+    for (; u < units; u += 2 * stride) {
+        load(u + stride, b);
+        compute(u, a);
+        load(u + 2 * stride, a);
+        compute(u + stride, b);
+    }
+    add_waves<NF * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (i / DF) * 16 + 4 * (l >> 4) + j, (i % DF) * 16 + (l & 15), v[j]);
+    });
+}
+
+template <typename T, int DF>
+__global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense16 D, Mx4View Y, bool words, int K, RowsOut out) {
+    constexpr int PL = Planes<T>::N;
+    __shared__ v4f sums[ROWS_WAVES * 8 * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
+    const int64_t q0 = (int64_t)blockIdx.x * 256;
+    const int nb = (int)(mx4_blocks(Y.cols) - q0 / 32);   // blocks of a row from this workgroup's first
+    const int units = (K + 31) / 32, stride = ROWS_WAVES * gridDim.y;
+    // a wave's scales of a unit, by block and row, as upper halves of floats: 8 blocks x 32 rows (in the place
+    // of its sums, which come after the last unit)
+    uint16_t *scales = (uint16_t *)&sums[wave * 8 * 64];
+    const uint8_t *cp = Y.codes + q0 / 2 + 8 * r16, *sp = Y.scales + q0 / 32;
+    struct Codes {
+        v2u c[8];
+        uint32_t s;
+    };
+    auto load = [&](int u, Codes &x) {
+        const int64_t k0 = u * 32 + 8 * g;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+            x.c[j] = k0 + j < K && (r16 >> 1) < nb ? *(const v2u *)(cp + (k0 + j) * Y.ldq) : v2u{0, 0};
+        // lane: row lane / 2, 4 blocks
+        const int64_t k = u * 32 + (lane >> 1);
+        const int b = (lane & 1) * 4;
+        x.s = 0;
+        if (k < K) {
+            const uint8_t *s = sp + k * Y.lds + b;
+            if (words && b + 4 <= nb) {
+                x.s = *(const uint32_t *)s;
+            } else {
+                for (int i = 0; i < 4; ++i)
+                    if (b + i < nb) x.s |= (uint32_t)s[i] << (8 * i);
+            }
+        }
+    };
+    v4f acc[16 * DF];
+#pragma unroll
+    for (int i = 0; i < 16 * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    // the dense rows of this lane, and how many pieces of 8 elements it may read of them
+    const uint16_t *xp[DF];
+    int have[DF];
+#pragma unroll
+    for (int d = 0; d < DF; ++d) {
+        have[d] = d * 16 + r16 < D.rows ? D.chunks : 0;
+        xp[d] = D.ptr + (have[d] ? (d * 16 + r16) * D.ld : 0);
+    }
+    auto dense = [&](int piece, v4u (&d)[DF][PL]) {
+#pragma unroll
+        for (int e = 0; e < DF; ++e)
+#pragma unroll
+            for (int i = 0; i < PL; ++i)
+                d[e][i] = piece < have[e] ? *(const v4u *)(xp[e] + i * D.plane + piece * 8) : v4u{0, 0, 0, 0};
+    };
+    auto compute = [&](int u, const Codes &x) {
+        v4u d[DF][PL];
+        dense(u * 4 + g, d);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) scales[((lane & 1) * 4 + i) * 32 + (lane >> 1)] = (uint16_t)(((x.s >> (8 * i)) & 255u) << 7);
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        v4u sc8;
+        __builtin_memcpy(&sc8, __builtin_assume_aligned(&scales[(r16 >> 1) * 32 + g * 8], 16), sizeof sc8);
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {   // 8 columns a word
+            v4u row[8];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const uint32_t half = (j & 1) ? sc8[j >> 1] & 0xFFFF0000u : sc8[j >> 1] << 16;
+                row[j] = decode_bf16(x.c[j][w], __builtin_bit_cast(float, half));
+            }
+#pragma unroll
+            for (int f = 0; f < 8; ++f) {
+                v4u q;
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    q[j] = __builtin_amdgcn_perm(row[2 * j + 1][f >> 1], row[2 * j][f >> 1], (f & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+                for (int e = 0; e < DF; ++e)
+#pragma unroll
+                    for (int i = 0; i < PL; ++i) acc[(w * 8 + f) * DF + e] = mfma_bf16(q, d[e][i], acc[(w * 8 + f) * DF + e]);
+            }
+        }
+    };
+    // a unit past the last is zeros
+    Codes a, b;
+    int u = blockIdx.y * ROWS_WAVES + wave;
+    load(u, a);
+    for (; u < units; u += 2 * stride) {
+        load(u + stride, b);
+        compute(u, a);
+        load(u + 2 * stride, a);
+        compute(u + stride, b);
+    }
+    add_waves<16 * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (4 * (l >> 4) + j) * 16 + i / DF, (i % DF) * 16 + (l & 15), v[j]);
+    });
+}
+
 // C = alpha * (the sum of the slices' partial sums, in their order) + beta * C
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, int slices, Out out) {
@@ -579,6 +806,7 @@ template <int TYPE> __global__ __launch_bounds__(256) void scale_kernel(Mx4Produ
 
 // How a mixed product runs
 struct MixedPlan {
+    int rows;            // dense rows / 16 of the kernel for few rows, 0 for the tiles
     bool direct;         // the dense factor is read as it is
     int64_t ld;          // of its planes otherwise
     int bq, bd;          // tile
@@ -595,6 +823,19 @@ MixedPlan mixed_plan(const Mx4Product &p) {
                p.X.sr <= (1 << 21);
     m.ld = (p.K + 63) / 64 * 64;
     if (!m.direct) m.planes = round256((size_t)pl * p.M * m.ld * 2);
+    if (p.M <= 32) {
+        m.rows = p.M <= 16 ? 1 : 2;
+        const int64_t groups = p.yt ? (p.N + 255) / 256 : (p.N + 63) / 64;
+        const int64_t units = p.yt ? (p.K + 31) / 32 : (p.K + 255) / 256;
+        // 64 columns a workgroup where that makes 256 of them, else fewer (a dense row is read by each)
+        // (64 x 32 in three planes does not fit the registers)
+        m.bq = p.yt ? 256 : p.N >= 64 * 256 && !(pl == 3 && m.rows == 2) ? 64 : p.N >= 32 * 256 ? 32 : 16;
+        m.slices = 1;
+        if (p.yt)
+            while (groups * m.slices * 2 <= 512 && units / (m.slices * 2) >= 2 * ROWS_WAVES) m.slices *= 2;
+        if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
+        return m;
+    }
     m.scales = scales_work(p.Y);
     const int64_t nq = p.N, nd = p.M;
     auto tiles = [&](int64_t q, int64_t d) { return ((nq + q - 1) / q) * ((nd + d - 1) / d); };
@@ -625,11 +866,44 @@ hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, cons
     return hipGetLastError();
 }
 
+template <typename T> hipError_t launch_join(const float *partial, int slices, const Out &out, hipStream_t s) {
+    const int64_t n = ((out.np + 3) / 4 * out.no + 255) / 256;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, s, partial, slices, out);
+    return hipGetLastError();
+}
+
+template <typename T> hipError_t launch_mixed_rows(const Dense16 &D, const Mx4Product &p, const MixedPlan &m, const Out &final, bool qfirst, float *partial, hipStream_t s) {
+    RowsOut out{p.C, p.cj, p.ci, p.N, p.M, p.alpha, p.beta, partial};
+    if (partial) out.sq = qfirst ? 1 : p.M, out.sd = qfirst ? p.N : 1;
+    const dim3 grid((unsigned)((p.N + m.bq - 1) / m.bq), (unsigned)m.slices), block(ROWS_WAVES * 64);
+    const bool words = aligned_scales(p.Y), pairs = (uintptr_t)p.Y.scales % 2 == 0 && p.Y.lds % 2 == 0;
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, D, p.Y, pairs, out); };
+    if (p.yt) {
+        if (m.rows == 1) hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 1>), grid, block, 0, s, D, p.Y, words, (int)p.K, out);
+        else hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 2>), grid, block, 0, s, D, p.Y, words, (int)p.K, out);
+    } else if (m.rows == 1) {
+        if (m.bq == 64) go(mixed_rows_kernel<T, 4, 1>);
+        else if (m.bq == 32) go(mixed_rows_kernel<T, 2, 1>);
+        else go(mixed_rows_kernel<T, 1, 1>);
+    } else {
+        if (m.bq == 16) go(mixed_rows_kernel<T, 1, 2>);
+        else if (m.bq == 32) go(mixed_rows_kernel<T, 2, 2>);
+        else if constexpr (Planes<T>::N < 3) go(mixed_rows_kernel<T, 4, 2>);
+    }
+    const hipError_t e = hipGetLastError();
+    return e == hipSuccess && partial ? launch_join<T>(partial, m.slices, final, s) : e;
+}
+
 template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipStream_t s) {
     typedef typename Elem<TYPE>::mem T;
     const MixedPlan m = mixed_plan(q);
     Mx4Product p = q;
-    hipError_t e = align_scales(p.Y, work, s);
+    const bool qfirst = p.cj == 1;   // the 4-bit factor's index is the contiguous one of C
+    const int64_t ld = qfirst ? p.ci : p.cj;
+    const Out out{p.C, ld, qfirst ? p.N : p.M, qfirst ? p.M : p.N, p.alpha, p.beta,
+                  (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
+    hipError_t e = hipSuccess;
+    if (!m.rows) e = align_scales(p.Y, work, s);
     if (e != hipSuccess) return e;
     Dense16 D{(const uint16_t *)p.X.ptr, p.M, p.X.sr, 0, (int)(p.K / 8)};
     if (!m.direct) {
@@ -648,11 +922,8 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
         if (e != hipSuccess) return e;
         D = Dense16{planes, p.M, m.ld, p.M * m.ld, (int)n8};
     }
-    const bool qfirst = p.cj == 1;   // the 4-bit factor's index is the contiguous one of C
-    const int64_t ld = qfirst ? p.ci : p.cj;
-    const Out out{p.C, ld, qfirst ? p.N : p.M, qfirst ? p.M : p.N, p.alpha, p.beta,
-                  (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
     float *partial = m.slices > 1 ? (float *)work : nullptr;
+    if (m.rows) return launch_mixed_rows<T>(D, p, m, out, qfirst, partial, s);
     auto go = [&](auto yt) -> hipError_t {
         constexpr bool YT = decltype(yt)::value;
         if constexpr (Planes<T>::N == 1)
@@ -662,10 +933,7 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     };
     e = p.yt ? go(std::true_type{}) : go(std::false_type{});
     if (e != hipSuccess || !partial) return e;
-    const int64_t n = (out.np + 3) / 4 * out.no;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)((n + 255) / 256 < 65536 ? (n + 255) / 256 : 65536)), dim3(256), 0, s, partial,
-                       m.slices, out);
-    return hipGetLastError();
+    return launch_join<T>(partial, m.slices, out, s);
 }
 
 template <int TYPE> hipError_t product_t(const Mx4Product &p, void *work, hipStream_t s) {

@@ -303,6 +303,20 @@ def test_products_close(cuda, m, n, k, alpha, beta, t, side, opA, opB):
     c.check_close()
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 16390, 70), (9, 8200, 300), (16, 16384, 544), (20, 16390, 96), (32, 8195, 520),
+                                   (5, 700, 5000), (31, 300, 9000)])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("opB", ["T", "N"])
+def test_few_rows_exact(cuda, opB, t, m, n, k):
+    """Few rows against wide and against long 4-bit matrices; |x y| <= 4 * 6 in halves, k <= 9000."""
+    for side, layout in (("right", "R"), ("left", "C")):
+        a, b = (m, n) if side == "right" else (n, m)
+        ops = ("N", opB) if side == "right" else ("N" if opB == "T" else "T", "N")
+        c = Case(cuda, side, a, b, k, t, layout, *ops, m, True, low=126, high=127)
+        c.run()
+        c.check_bitwise()
+
+
 @pytest.mark.parametrize("scale_pad", [0, 1, 3])
 @pytest.mark.parametrize("side,opB", [("right", "T"), ("right", "N"), ("both", "T")])
 def test_scales_of_any_alignment(cuda, side, opB, scale_pad):
