@@ -718,10 +718,10 @@ def spmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
 # 4-bit microscaled matrices (MXFP4; no reference counterpart)
 # --------------------------------------------------------------------------------------------
 _MX4_TAGS = {np.dtype(np.float64): "f64", np.dtype(np.float32): "f32", np.dtype(np.float16): "f16"}
-_MX4_BYTES = [np.dtype(np.uint8)]
+_MX4_BYTES = {np.dtype(np.uint8)}
 if torch is not None:
     _MX4_TAGS.update({torch.float64: "f64", torch.float32: "f32", torch.float16: "f16", torch.bfloat16: "bf16"})
-    _MX4_BYTES.append(torch.uint8)
+    _MX4_BYTES.add(torch.uint8)
 ROUNDINGS = {"nearest": 0, "stochastic": 1}   # RBH_ROUND_*
 _MX4_QUANTIZE = {t: getattr(lib, f"rbh_mx4_quantize_{t}") for t in ("f64", "f32", "f16", "bf16")}
 _MX4_DEQUANTIZE = {t: getattr(lib, f"rbh_mx4_dequantize_{t}") for t in ("f64", "f32", "f16", "bf16")}
@@ -743,35 +743,42 @@ def _mx4_stream(x, stream):
 
 
 def _bytes_2d(x, name, rows, width):
-    """The bytes between rows of a uint8 array of at least rows x width, checked."""
+    """Address of, and bytes between the rows of, a uint8 array of at least rows x width, checked."""
     if x.dtype not in _MX4_BYTES or x.ndim != 2:
         raise TypeError(f"{name} must be a 2-D uint8 array")
-    strides, (have, wide) = x.strides if isinstance(x, np.ndarray) else x.stride(), x.shape
+    (far, near), (have, wide) = x.strides if isinstance(x, np.ndarray) else x.stride(), x.shape
     if rows == 0 or width == 0:
-        return width
-    if have < rows or wide < width or (wide > 1 and strides[1] != 1):
+        return _ptr(x), width
+    if have < rows or wide < width or (wide > 1 and near != 1):
         raise ValueError(f"{name} must hold {rows} rows of {width} consecutive bytes")
-    return strides[0] if rows > 1 else max(strides[0], width)
+    return _ptr(x), far if rows > 1 else max(far, width)
 
 
-@dataclass(frozen=True)
 class MX4Matrix:
     """A 4-bit microscaled matrix (rbh_mx4, include/randblas_hip.h): n_rows x n_cols E2M1 elements, blocks
     of 32 along a row, one E8M0 scale a block. codes: uint8, n_rows x 16 bytes a block, two elements a
     byte, the even column in the low half. scales: uint8, n_rows x one byte a block. Device tensors or
-    host arrays; rows may be further apart than they are long (codes: by multiples of 16)."""
+    host arrays; rows may be further apart than they are long (codes: by multiples of 16). The arrays
+    are fixed when the matrix is made; their contents are read by each call."""
 
-    n_rows: int
-    n_cols: int
-    codes: object
-    scales: object
-    _c: MX4MatrixC = field(default=None, repr=False, compare=False)
+    __slots__ = ("n_rows", "n_cols", "codes", "scales", "_c")
 
-    def __post_init__(self):
-        nb = (self.n_cols + 31) // 32
-        c = MX4MatrixC(self.n_rows, self.n_cols, _ptr(self.codes), _bytes_2d(self.codes, "codes", self.n_rows, 16 * nb),
-                       _ptr(self.scales), _bytes_2d(self.scales, "scales", self.n_rows, nb))
-        object.__setattr__(self, "_c", c)
+    def __init__(self, n_rows: int, n_cols: int, codes, scales):
+        nb = (n_cols + 31) // 32
+        at, ld = _bytes_2d(codes, "codes", n_rows, 16 * nb)
+        sat, sld = _bytes_2d(scales, "scales", n_rows, nb)
+        set_ = object.__setattr__
+        set_(self, "n_rows", n_rows)
+        set_(self, "n_cols", n_cols)
+        set_(self, "codes", codes)
+        set_(self, "scales", scales)
+        set_(self, "_c", MX4MatrixC(n_rows, n_cols, at, ld, sat, sld))
+
+    def __setattr__(self, name, value):
+        raise AttributeError(f"{name} of an MX4Matrix is fixed")
+
+    def __repr__(self):
+        return f"MX4Matrix(n_rows={self.n_rows}, n_cols={self.n_cols})"
 
 
 def mx4_empty(n_rows: int, n_cols: int, device=None) -> MX4Matrix:
@@ -779,8 +786,8 @@ def mx4_empty(n_rows: int, n_cols: int, device=None) -> MX4Matrix:
     start at multiples of 4 bytes."""
     nb = (n_cols + 31) // 32
     device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
-    return MX4Matrix(n_rows, n_cols, torch.empty(n_rows, 16 * nb, dtype=torch.uint8, device=device),
-                     torch.empty(n_rows, (nb + 3) // 4 * 4, dtype=torch.uint8, device=device))
+    return MX4Matrix(n_rows, n_cols, torch.empty((n_rows, 16 * nb), dtype=torch.uint8, device=device),
+                     torch.empty((n_rows, (nb + 3) // 4 * 4), dtype=torch.uint8, device=device))
 
 
 def mx4_quantize(layout, op, n_rows, n_cols, A, lda, Q: MX4Matrix, rounding="nearest",

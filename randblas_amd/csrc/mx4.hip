@@ -223,8 +223,7 @@ template <int TYPE> __device__ __forceinline__ void decode8(uint32_t w, float sc
 
 template <int TYPE>
 __global__ __launch_bounds__(MXT) void dequantize_rows_kernel(Mx4View Q, typename Elem<TYPE>::mem *__restrict__ A,
-                                                               int64_t ld, FastDiv nb, uint32_t units, int64_t row0,
-                                                               bool vec) {
+                                                               int64_t ld, FastDiv nb, uint32_t units, int64_t row0) {
     typedef typename Elem<TYPE>::mem M;
     typedef M m8_t __attribute__((ext_vector_type(8)));
     const uint32_t u = blockIdx.x * (uint32_t)MXT + threadIdx.x;
@@ -237,7 +236,7 @@ __global__ __launch_bounds__(MXT) void dequantize_rows_kernel(Mx4View Q, typenam
     M o[8];
     decode8<TYPE>(w, scale_f32(Q.scales[r * Q.lds + b]), o);
     M *p = A + r * ld + c;
-    if (vec && c + 8 <= Q.cols) {
+    if (c + 8 <= Q.cols) {
         m8_t m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m[i] = o[i];
@@ -247,6 +246,19 @@ __global__ __launch_bounds__(MXT) void dequantize_rows_kernel(Mx4View Q, typenam
         for (int i = 0; i < 8; ++i)
             if (c + i < Q.cols) p[i] = o[i];
     }
+}
+
+// Rows that are not at multiples of 16 bytes: a lane an element, so that a wave's stores are contiguous all the
+// same (8 elements a lane at 8 bytes each took 18.5 us for 2999 x 1013 doubles, this UNALIGNED_US)
+template <int TYPE>
+__global__ __launch_bounds__(MXT) void dequantize_elements_kernel(Mx4View Q, typename Elem<TYPE>::mem *__restrict__ A, int64_t ld) {
+    typedef typename Elem<TYPE>::mem M;
+    for (int64_t r = blockIdx.y; r < Q.rows; r += gridDim.y)
+        for (int64_t c = (int64_t)blockIdx.x * MXT + threadIdx.x; c < Q.cols; c += (int64_t)gridDim.x * MXT) {
+            M o[8];
+            decode8<TYPE>(Q.codes[r * Q.ldq + (c >> 1)], scale_f32(Q.scales[r * Q.lds + (c >> 5)]), o);
+            A[r * ld + c] = c & 1 ? o[1] : o[0];
+        }
 }
 
 template <int TYPE>
@@ -311,11 +323,16 @@ template <int TYPE> hipError_t dequantize_t(const Mx4View &Q, const Mx4Dense &A,
     M *a = (M *)const_cast<void *>(A.ptr);
     const int64_t nb = mx4_blocks(Q.cols);
     if (A.sc == 1) {
-        const bool vec = (uintptr_t)a % 16 == 0 && (A.sr * sizeof(M)) % 16 == 0;
+        if ((uintptr_t)a % 16 != 0 || (A.sr * sizeof(M)) % 16 != 0) {
+            const int64_t x = (Q.cols + MXT - 1) / MXT;
+            hipLaunchKernelGGL((dequantize_elements_kernel<TYPE>), dim3((unsigned)(x < 65536 ? x : 65536), (unsigned)(Q.rows < 65535 ? Q.rows : 65535)),
+                               dim3(MXT), 0, s, Q, a, A.sr);
+            return hipGetLastError();
+        }
         return row_chunks(Q.rows, nb * 4, [&](int64_t r0, int64_t rows) {
             const uint32_t units = (uint32_t)(rows * nb * 4);
             hipLaunchKernelGGL((dequantize_rows_kernel<TYPE>), dim3((units + MXT - 1) / MXT), dim3(MXT), 0, s, Q, a, A.sr,
-                               fast_div((uint32_t)nb), units, r0, vec);
+                               fast_div((uint32_t)nb), units, r0);
             return hipGetLastError();
         });
     }

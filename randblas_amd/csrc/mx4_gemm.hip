@@ -18,6 +18,8 @@ template <> struct Elem<MX4_BF16> { typedef __bf16 mem; };
 typedef int v4i __attribute__((ext_vector_type(4)));
 typedef int v8i __attribute__((ext_vector_type(8)));
 typedef float v4f __attribute__((ext_vector_type(4)));
+typedef uint32_t v4u __attribute__((ext_vector_type(4)));
+typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 // D += A B^T over 128 columns: lane l holds row l & 15 of a factor, the block l >> 4 of its 4 blocks (32
 // codes, 16 bytes) and that block's scale in the low byte of a word; D: column l & 15 (B's row), rows
@@ -80,6 +82,22 @@ __device__ __forceinline__ void load_lds16(Buffer b, void *lds, uint32_t voffset
 __device__ __forceinline__ void load_lds4(Buffer b, void *lds, uint32_t voffset, uint32_t soffset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void *)lds, 4, (int)voffset,
                                              (int)soffset, 0, 0);
+}
+__device__ __forceinline__ v4u load16(Buffer b, uint32_t voffset, uint32_t soffset) {
+    return __builtin_amdgcn_raw_buffer_load_b128(b, (int)voffset, (int)soffset, 0);
+}
+__device__ __forceinline__ v2u load8(Buffer b, uint32_t voffset, uint32_t soffset) {
+    return __builtin_amdgcn_raw_buffer_load_b64(b, (int)voffset, (int)soffset, 0);
+}
+__device__ __forceinline__ uint32_t load4(Buffer b, uint32_t voffset, uint32_t soffset) {
+    return __builtin_amdgcn_raw_buffer_load_b32(b, (int)voffset, (int)soffset, 0);
+}
+// All but this wave's last N loads have arrived. The compiler does not count loads to LDS for the reads of
+// it, so their waits are written out; it leaves no load on the other side of one.
+template <int N> __device__ __forceinline__ void wait_loads() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
 }
 // Every wave's loads to LDS have arrived and every wave has read what they will overwrite. The wait has to
 // be written out: __syncthreads does not wait for loads that go to LDS.
@@ -215,44 +233,6 @@ hipError_t launch_both_tile(const Mx4View &P, const Mx4View &O, const Out &out, 
     return hipGetLastError();
 }
 
-// Scales whose rows do not start at multiples of 4 bytes are copied to rows that do.
-bool aligned_scales(const Mx4View &v) { return (uintptr_t)v.scales % 4 == 0 && v.lds % 4 == 0; }
-size_t scales_work(const Mx4View &v) {
-    return aligned_scales(v) ? 0 : (size_t)((v.rows * ((mx4_blocks(v.cols) + 3) / 4 * 4) + 255) / 256 * 256);
-}
-__global__ __launch_bounds__(256) void copy_scales_kernel(const uint8_t *src, int64_t lds, int64_t rows, int nb, int nb4, uint8_t *dst) {
-    const int b = blockIdx.x * 256 + threadIdx.x;
-    if (b >= nb) return;
-    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) dst[r * nb4 + b] = src[r * lds + b];
-}
-hipError_t align_scales(Mx4View &v, uint8_t *&work, hipStream_t s) {
-    if (aligned_scales(v)) return hipSuccess;
-    const int nb = (int)mx4_blocks(v.cols), nb4 = (nb + 3) / 4 * 4;
-    const dim3 grid((unsigned)((nb + 255) / 256), (unsigned)(v.rows < 65535 ? v.rows : 65535));
-    hipLaunchKernelGGL(copy_scales_kernel, grid, dim3(256), 0, s, v.scales, v.lds, v.rows, nb, nb4, work);
-    const size_t bytes = scales_work(v);
-    v.scales = work;
-    v.lds = nb4;
-    work += bytes;
-    return hipGetLastError();
-}
-
-template <int TYPE> hipError_t both_t(const Mx4Product &q, uint8_t *work, hipStream_t s) {
-    Mx4Product p = q;
-    hipError_t e = align_scales(p.XQ, work, s);
-    if (e == hipSuccess) e = align_scales(p.Y, work, s);
-    if (e != hipSuccess) return e;
-    typedef typename Elem<TYPE>::mem T;
-    // the factor whose rows are the contiguous index of C gives the operand whose 4 entries a lane holds
-    const bool xp = p.ci == 1;
-    const Mx4View &P = xp ? p.XQ : p.Y, &O = xp ? p.Y : p.XQ;
-    const int64_t ld = xp ? p.cj : p.ci;
-    const Out out{p.C, ld, P.rows, O.rows, p.alpha, p.beta, (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
-    auto tiles = [&](int64_t b) { return ((P.rows + b - 1) / b) * ((O.rows + b - 1) / b); };
-    if (tiles(256) >= 256) return launch_both_tile<T, 256, 256, 128, 64>(P, O, out, s);
-    return launch_both_tile<T, 128, 128, 64, 64>(P, O, out, s);
-}
-
 // ---------------------------------------------------------------------------------------------
 // One dense and one 4-bit factor on the bf16 matrix instruction
 // ---------------------------------------------------------------------------------------------
@@ -262,8 +242,6 @@ template <int TYPE> hipError_t both_t(const Mx4Product &q, uint8_t *work, hipStr
 // 5 times the f32 instruction's rate). Sums are f32.
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
-typedef uint32_t v4u __attribute__((ext_vector_type(4)));
-typedef uint32_t v2u __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -554,7 +532,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 // contraction, its 8 waves take the slice's units in turn, and each wave streams its codes from memory
 // straight to registers, so nothing but the codes' bytes bounds it: every load of a unit is issued before the
 // one before it is used, and no barrier stands between them. The waves' sums are added in LDS, in order.
-//   blocks along the contraction: unit of 256 elements; lane (r, g) holds blocks 2 g, 2 g + 1 of row r
+//   blocks along the contraction: unit of 256 elements; lane (r, g) holds blocks 2 g and 2 g + 1 of row r
 //   blocks across it (YT): unit of 32 rows and 256 columns; lane (c, g) holds columns 16 c .. + 15 of rows
 //     8 g .. + 7 (128 bytes of a row, whole lines, are read by 16 lanes together)
 // entry (q, d) of the result at ptr[q * sq + d * sd]; partial sums where `partial` is set
@@ -575,10 +553,12 @@ template <typename T> __device__ __forceinline__ void put1(const RowsOut &o, int
 }
 
 constexpr int ROWS_WAVES = 8;
+// with dense rows in LDS: as many waves as it holds buffers for
+__host__ __device__ constexpr int dense_waves(int planes) { return planes <= 2 ? 8 : 4; }
 
-// adds the 8 waves' N operands and hands each sum to f(operand, lane, value)
-template <int N, typename F> __device__ __forceinline__ void add_waves(const v4f *acc, v4f *lds, int lane, int wave, F &&f) {
-    constexpr int C = N < 8 ? N : 8;
+// adds the W waves' N operands and hands each sum to f(operand, lane, value)
+template <int W, int N, typename F> __device__ __forceinline__ void add_waves(const v4f *acc, v4f *lds, int lane, int wave, F &&f) {
+    constexpr int C = N < W ? N : W;
     static_assert(N % C == 0, "whole rounds");
 #pragma unroll
     for (int r = 0; r < N; r += C) {
@@ -589,150 +569,229 @@ template <int N, typename F> __device__ __forceinline__ void add_waves(const v4f
         if (wave < C) {
             v4f sum = lds[wave * 64 + lane];
 #pragma unroll
-            for (int w = 1; w < ROWS_WAVES; ++w) sum += lds[(w * C + wave) * 64 + lane];
+            for (int w = 1; w < W; ++w) sum += lds[(w * C + wave) * 64 + lane];
             f(r + wave, lane, sum);
         }
     }
 }
 
-template <typename T, int NF, int DF>
-__global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_kernel(Dense16 D, Mx4View Y, bool pairs, RowsOut out) {
-    constexpr int PL = Planes<T>::N;
-    __shared__ v4f sums[ROWS_WAVES * (NF * DF < 8 ? NF * DF : 8) * 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
-    const int64_t q0 = (int64_t)blockIdx.x * (NF * 16);
-    const int nb = (int)mx4_blocks(Y.cols);
-    const int units = (nb + 7) / 8, stride = ROWS_WAVES * gridDim.y;
-    const uint8_t *cp[NF], *sp[NF];
-#pragma unroll
-    for (int f = 0; f < NF; ++f) {
-        const int64_t r = q0 + f * 16 + r16 < Y.rows ? q0 + f * 16 + r16 : Y.rows - 1;
-        cp[f] = Y.codes + r * Y.ldq + 32 * g;
-        sp[f] = Y.scales + r * Y.lds + 2 * g;
-    }
-    struct Codes {
-        v4u c[NF][2];
-        uint32_t s[NF];
-    };
-    auto load = [&](int u, Codes &x) {
-        const int b = u * 8 + 2 * g;
+// 16 NF rows of a 4-bit factor from row0 in one unit of 128 H columns: lane (r, g) holds the H blocks H g ..
+// of row r of each 16 and the word that their scales are in. What lies behind the last block or row reads
+// as zeros.
+template <int NF, int H> struct RowCodes {
+    v4u c[NF][H];
+    uint32_t s[NF];
+};
+template <int NF, int H> struct RowReader {
+    Buffer cb, sb;
+    uint32_t co[NF], so[NF];
+    int nb, g;
+    __device__ __forceinline__ RowReader(const Mx4View &V, int64_t row0, int r16, int group) : nb((int)mx4_blocks(V.cols)), g(group) {
+        const int64_t left = V.rows - row0 < NF * 16 ? V.rows - row0 : NF * 16;
+        cb = buffer(V.codes + row0 * V.ldq, (uint32_t)((left - 1) * V.ldq + nb * 16));
+        sb = buffer(V.scales + row0 * V.lds, (uint32_t)((left - 1) * V.lds + (nb + 3) / 4 * 4));
 #pragma unroll
         for (int f = 0; f < NF; ++f) {
-            x.c[f][0] = b < nb ? *(const v4u *)(cp[f] + (int64_t)u * 128) : v4u{0, 0, 0, 0};
-            x.c[f][1] = b + 1 < nb ? *(const v4u *)(cp[f] + (int64_t)u * 128 + 16) : v4u{0, 0, 0, 0};
-            const uint8_t *s = sp[f] + (int64_t)u * 8;
-            if (pairs && b + 1 < nb) x.s[f] = *(const uint16_t *)s;
-            else x.s[f] = (b < nb ? s[0] : 0u) | (b + 1 < nb ? s[1] : 0u) << 8;
+            co[f] = (uint32_t)((f * 16 + r16) * V.ldq) + 16 * H * g;
+            so[f] = (uint32_t)((f * 16 + r16) * V.lds) + (H * g / 4) * 4;
         }
-    };
+    }
+    __device__ __forceinline__ int block(int u, int h) const { return (u * 4 + g) * H + h; }
+    __device__ __forceinline__ void load(int u, RowCodes<NF, H> &x) const {
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int f = 0; f < NF; ++f) x.c[f][h] = load16(cb, block(u, h) < nb ? co[f] + 16 * h : OUTSIDE, u * 64 * H);
+#pragma unroll
+        for (int f = 0; f < NF; ++f) x.s[f] = load4(sb, block(u, 0) < nb ? so[f] : OUTSIDE, u * 4 * H);
+    }
+    // the scale of this lane's block h of unit u; past the last block 0, whatever is there
+    __device__ __forceinline__ uint32_t scale(int u, int h, uint32_t word) const {
+        return __builtin_amdgcn_ubfe(word, 8 * ((g * H + h) & 3), block(u, h) < nb ? 8 : 0);
+    }
+};
+
+// The dense rows of a unit go through LDS, each wave's own: a matrix operand wants 16 rows at once, 16 bytes
+// of each, which as loads from memory would be 64 lines for one operand; straight to LDS a load takes whole
+// lines, and only the rows that there are. A half unit (every other block, 128 elements, 256 bytes a row)
+// is a buffer; its piece p of row r is kept at place p ^ r.
+// RG: loads of 4 dense rows each.
+template <typename T, int NF, int RG>
+__global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, 2) void mixed_rows_kernel(Dense16 D, Mx4View Y, RowsOut out) {
+    constexpr int PL = Planes<T>::N, DF = RG > 4 ? 2 : 1;
+    constexpr int BUF = PL * DF * 16 * 256;             // bytes of a wave's half unit
+    constexpr int W = dense_waves(PL * DF), C = NF * DF < W ? NF * DF : W;
+    static_assert(2 * W * BUF <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) uint8_t half0[W * BUF < W * C * 1024 ? W * C * 1024 : W * BUF];
+    __shared__ __attribute__((aligned(16))) uint8_t half1[W * BUF];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
+    const int64_t q0 = (int64_t)blockIdx.x * (NF * 16);
+    const RowReader<NF, 2> q(Y, q0, r16, g);
+    const int units = (q.nb + 7) / 8, stride = W * gridDim.y;
     v4f acc[NF * DF];
 #pragma unroll
     for (int i = 0; i < NF * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    // the dense rows of this lane, and how many pieces of 8 elements it may read of them
-    const uint16_t *xp[DF];
-    int have[DF];
+    const int rows = (int)D.rows;
+    Buffer db[PL];
 #pragma unroll
-    for (int d = 0; d < DF; ++d) {
-        have[d] = d * 16 + r16 < D.rows ? D.chunks : 0;
-        xp[d] = D.ptr + (have[d] ? (d * 16 + r16) * D.ld : 0);
-    }
-    auto dense = [&](int piece, v4u (&d)[DF][PL]) {
+    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane, (uint32_t)((rows - 1) * D.ld * 2 + D.chunks * 16));
+    // one load: 4 rows, lane l places l & 15 of row l / 16 of them; rows that are not there are zeros
+    auto load_dense = [&](int hu, uint8_t *lds) {       // half unit hu
 #pragma unroll
-        for (int e = 0; e < DF; ++e)
+        for (int i = 0; i < RG; ++i) {                  // further rows' places hold anything: their results are not stored
+            const int row = i * 4 + g, kept = r16 ^ (row & 15);   // piece of the half: 4 of each 8 of the unit
+            const int piece = (hu >> 1) * 32 + (kept >> 2) * 8 + (hu & 1) * 4 + (kept & 3);
+            const uint32_t where = piece < D.chunks ? (uint32_t)(row * D.ld * 2) + (uint32_t)piece * 16 : OUTSIDE;
 #pragma unroll
-            for (int i = 0; i < PL; ++i)
-                d[e][i] = piece < have[e] ? *(const v4u *)(xp[e] + i * D.plane + piece * 8) : v4u{0, 0, 0, 0};
+            for (int p = 0; p < PL; ++p) load_lds16(db[p], lds + wave * BUF + (p * DF * 16 + i * 4) * 256, where, 0);
+        }
     };
-    auto compute = [&](int u, const Codes &x) {
+    auto compute = [&](int u, int h, const RowCodes<NF, 2> &x, const uint8_t *lds) {
+        float scale[NF];
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
+        for (int f = 0; f < NF; ++f) scale[f] = __builtin_bit_cast(float, q.scale(u, h, x.s[f]) << 23);
+        const uint8_t *row = lds + wave * BUF + r16 * 256;
 #pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                v4u d[DF][PL];
-                dense(u * 32 + g * 8 + h * 4 + t, d);
+        for (int t = 0; t < 4; ++t) {
+            v4u d[DF][PL];
 #pragma unroll
-                for (int f = 0; f < NF; ++f) {
-                    const v4u q = decode_bf16(x.c[f][h][t], __builtin_bit_cast(float, __builtin_amdgcn_ubfe(x.s[f], 8 * h, 8) << 23));
+            for (int e = 0; e < DF; ++e)
 #pragma unroll
-                    for (int e = 0; e < DF; ++e)
+                for (int p = 0; p < PL; ++p) d[e][p] = *(const v4u *)(row + (p * DF + e) * 16 * 256 + ((g * 4 + t) ^ r16) * 16);
 #pragma unroll
-                        for (int i = 0; i < PL; ++i) acc[f * DF + e] = mfma_bf16(q, d[e][i], acc[f * DF + e]);
-                }
+            for (int f = 0; f < NF; ++f) {
+                const v4u w = decode_bf16(x.c[f][h][t], scale[f]);
+#pragma unroll
+                for (int e = 0; e < DF; ++e)
+#pragma unroll
+                    for (int p = 0; p < PL; ++p) acc[f * DF + e] = mfma_bf16(w, d[e][p], acc[f * DF + e]);
             }
         }
     };
-    // a unit past the last is zeros
-    Codes a, b;
-    int u = blockIdx.y * ROWS_WAVES + wave;
-    load(u, a);
-    for (; u < units; u += 2 * stride) {
-        load(u + stride, b);
-        compute(u, a);
-        load(u + 2 * stride, a);
-        compute(u + stride, b);
+    // Loads arrive in their order, and a use waits until no more are on their way than were issued behind
+    // those it needs: LD of dense rows for a half, LC of codes and scales for a unit. The fences keep every
+    // load on its side of a wait. A unit past the last is zeros.
+    constexpr int LD = RG * PL, LC = 3 * NF;
+    RowCodes<NF, 2> a, b;
+    int u = blockIdx.y * W + wave;
+    q.load(u, a);
+    load_dense(2 * u, half0);
+    load_dense(2 * u + 1, half1);
+    auto unit = [&](const RowCodes<NF, 2> &now, RowCodes<NF, 2> &next) {
+        q.load(u + stride, next);
+        wait_loads<LD + LC>();                          // of half 1 and of the next codes
+        compute(u, 0, now, half0);
+        __builtin_amdgcn_sched_barrier(0);
+        load_dense(2 * (u + stride), half0);
+        wait_loads<LC + LD>();                          // of the next codes and of the next half 0
+        compute(u, 1, now, half1);
+        __builtin_amdgcn_sched_barrier(0);
+        load_dense(2 * (u + stride) + 1, half1);
+        u += stride;
+    };
+    while (u < units) {
+        unit(a, b);
+        unit(b, a);
     }
-    add_waves<NF * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
+    arrive();   // nothing is on its way to LDS any more
+    add_waves<W, NF * DF>(acc, (v4f *)half0, lane, wave, [&](int i, int l, v4f v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (i / DF) * 16 + 4 * (l >> 4) + j, (i % DF) * 16 + (l & 15), v[j]);
     });
 }
 
+// The same for two 4-bit factors, 16 NF x 16 DF entries of the result a workgroup: products too small for
+// the tiles, where the time of a call is the way of its loads.
+template <typename T, int NF, int DF>
+__global__ __launch_bounds__(ROWS_WAVES * 64, 2) void both_rows_kernel(Mx4View Q, Mx4View D, RowsOut out) {
+    constexpr int H = NF * DF >= 8 ? 1 : 2;   // what two units in flight leave of the registers
+    __shared__ v4f sums[ROWS_WAVES * (NF * DF < 8 ? NF * DF : 8) * 64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
+    const int64_t q0 = (int64_t)blockIdx.x * (NF * 16), d0 = (int64_t)blockIdx.z * (DF * 16);
+    const RowReader<NF, H> q(Q, q0, r16, g);
+    const RowReader<DF, H> d(D, d0, r16, g);
+    const int units = (q.nb + 4 * H - 1) / (4 * H), stride = ROWS_WAVES * gridDim.y;
+    v4f acc[NF * DF];
+#pragma unroll
+    for (int i = 0; i < NF * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](int u, const RowCodes<NF, H> &x, const RowCodes<DF, H> &y) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            uint32_t sy[DF];
+#pragma unroll
+            for (int e = 0; e < DF; ++e) sy[e] = d.scale(u, h, y.s[e]);
+#pragma unroll
+            for (int f = 0; f < NF; ++f) {
+                const uint32_t sx = q.scale(u, h, x.s[f]);
+#pragma unroll
+                for (int e = 0; e < DF; ++e)
+                    acc[f * DF + e] = mfma_mx4(__builtin_bit_cast(v4i, x.c[f][h]), __builtin_bit_cast(v4i, y.c[e][h]), acc[f * DF + e],
+                                               (int)sx, (int)sy[e]);
+            }
+        }
+    };
+    RowCodes<NF, H> qa, qb;
+    RowCodes<DF, H> da, db;
+    int u = blockIdx.y * ROWS_WAVES + wave;
+    q.load(u, qa);
+    d.load(u, da);
+    for (; u < units; u += 2 * stride) {
+        q.load(u + stride, qb);
+        d.load(u + stride, db);
+        compute(u, qa, da);
+        __builtin_amdgcn_sched_barrier(0);   // not three units at once
+        q.load(u + 2 * stride, qa);
+        d.load(u + 2 * stride, da);
+        compute(u + stride, qb, db);
+    }
+    add_waves<ROWS_WAVES, NF * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (i / DF) * 16 + 4 * (l >> 4) + j, d0 + (i % DF) * 16 + (l & 15), v[j]);
+    });
+}
+
 template <typename T, int DF>
-__global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense16 D, Mx4View Y, bool words, int K, RowsOut out) {
+__global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense16 D, Mx4View Y, int K, RowsOut out) {
     constexpr int PL = Planes<T>::N;
     __shared__ v4f sums[ROWS_WAVES * 8 * 64];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
     const int64_t q0 = (int64_t)blockIdx.x * 256;
-    const int nb = (int)(mx4_blocks(Y.cols) - q0 / 32);   // blocks of a row from this workgroup's first
+    const int nb = (int)(mx4_blocks(Y.cols) - q0 / 32), tile_nb = nb < 8 ? nb : 8;   // blocks of a row from this workgroup's first
     const int units = (K + 31) / 32, stride = ROWS_WAVES * gridDim.y;
     // a wave's scales of a unit, by block and row, as upper halves of floats: 8 blocks x 32 rows (in the place
     // of its sums, which come after the last unit)
     uint16_t *scales = (uint16_t *)&sums[wave * 8 * 64];
-    const uint8_t *cp = Y.codes + q0 / 2 + 8 * r16, *sp = Y.scales + q0 / 32;
-    struct Codes {
-        v2u c[8];
-        uint32_t s;
-    };
-    auto load = [&](int u, Codes &x) {
-        const int64_t k0 = u * 32 + 8 * g;
+    Buffer db[PL];
 #pragma unroll
-        for (int j = 0; j < 8; ++j)
-            x.c[j] = k0 + j < K && (r16 >> 1) < nb ? *(const v2u *)(cp + (k0 + j) * Y.ldq) : v2u{0, 0};
-        // lane: row lane / 2, 4 blocks
-        const int64_t k = u * 32 + (lane >> 1);
-        const int b = (lane & 1) * 4;
-        x.s = 0;
-        if (k < K) {
-            const uint8_t *s = sp + k * Y.lds + b;
-            if (words && b + 4 <= nb) {
-                x.s = *(const uint32_t *)s;
-            } else {
-                for (int i = 0; i < 4; ++i)
-                    if (b + i < nb) x.s |= (uint32_t)s[i] << (8 * i);
-            }
-        }
-    };
-    v4f acc[16 * DF];
-#pragma unroll
-    for (int i = 0; i < 16 * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    // the dense rows of this lane, and how many pieces of 8 elements it may read of them
-    const uint16_t *xp[DF];
-    int have[DF];
-#pragma unroll
-    for (int d = 0; d < DF; ++d) {
-        have[d] = d * 16 + r16 < D.rows ? D.chunks : 0;
-        xp[d] = D.ptr + (have[d] ? (d * 16 + r16) * D.ld : 0);
-    }
+    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane, (uint32_t)((D.rows - 1) * D.ld * 2 + D.chunks * 16));
     auto dense = [&](int piece, v4u (&d)[DF][PL]) {
 #pragma unroll
         for (int e = 0; e < DF; ++e)
 #pragma unroll
             for (int i = 0; i < PL; ++i)
-                d[e][i] = piece < have[e] ? *(const v4u *)(xp[e] + i * D.plane + piece * 8) : v4u{0, 0, 0, 0};
+                d[e][i] = load16(db[i], piece < D.chunks ? (uint32_t)((e * 16 + r16) * D.ld * 2) + (uint32_t)piece * 16 : OUTSIDE, 0);
     };
-    auto compute = [&](int u, const Codes &x) {
+    struct Codes {
+        v2u c[8];
+        uint32_t s;
         v4u d[DF][PL];
-        dense(u * 4 + g, d);
+    };
+    auto load = [&](int u, Codes &x) {
+        const int left = K - u * 32 < 32 ? K - u * 32 : 32;
+        const int64_t k0 = left > 0 ? (int64_t)u * 32 : 0;   // past the last unit the ranges are empty
+        const Buffer cb = buffer(Y.codes + q0 / 2 + k0 * Y.ldq, left > 0 ? (uint32_t)((left - 1) * Y.ldq + tile_nb * 16) : 0u);
+        const Buffer sb = buffer(Y.scales + q0 / 32 + k0 * Y.lds, left > 0 ? (uint32_t)((left - 1) * Y.lds + (tile_nb + 3) / 4 * 4) : 0u);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x.c[j] = load8(cb, (r16 >> 1) < nb ? (uint32_t)((8 * g + j) * Y.ldq) + 8 * r16 : OUTSIDE, 0);
+        // lane: row lane / 2, 4 blocks
+        const int b = (lane & 1) * 4;
+        x.s = load4(sb, b < nb ? (uint32_t)((lane >> 1) * Y.lds) + b : OUTSIDE, 0);
+        dense(u * 4 + g, x.d);
+    };
+    v4f acc[16 * DF];
+#pragma unroll
+    for (int i = 0; i < 16 * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
+    auto compute = [&](const Codes &x) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) scales[((lane & 1) * 4 + i) * 32 + (lane >> 1)] = (uint16_t)(((x.s >> (8 * i)) & 255u) << 7);
         __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -757,7 +816,7 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
 #pragma unroll
                 for (int e = 0; e < DF; ++e)
 #pragma unroll
-                    for (int i = 0; i < PL; ++i) acc[(w * 8 + f) * DF + e] = mfma_bf16(q, d[e][i], acc[(w * 8 + f) * DF + e]);
+                    for (int i = 0; i < PL; ++i) acc[(w * 8 + f) * DF + e] = mfma_bf16(q, x.d[e][i], acc[(w * 8 + f) * DF + e]);
             }
         }
     };
@@ -767,11 +826,13 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
     load(u, a);
     for (; u < units; u += 2 * stride) {
         load(u + stride, b);
-        compute(u, a);
+        compute(a);
+        __builtin_amdgcn_sched_barrier(0);   // not three units at once
         load(u + 2 * stride, a);
-        compute(u + stride, b);
+        compute(b);
+        __builtin_amdgcn_sched_barrier(0);
     }
-    add_waves<16 * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
+    add_waves<ROWS_WAVES, 16 * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (4 * (l >> 4) + j) * 16 + i / DF, (i % DF) * 16 + (l & 15), v[j]);
     });
@@ -781,14 +842,20 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, int slices, Out out) {
     const int64_t n4 = (out.np + 3) / 4, plane = out.np * out.no;
+    const bool vec = out.np % 4 == 0;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n4 * out.no; t += (int64_t)gridDim.x * 256) {
         const int64_t q = t / n4, p = (t - q * n4) * 4;
         const float *x = partial + q * out.np + p;
         v4f sum{0.f, 0.f, 0.f, 0.f};
-        for (int z = 0; z < slices; ++z)
+#pragma unroll 4
+        for (int z = 0; z < slices; ++z) {
+            if (vec) {
+                sum += *(const v4f *)(x + z * plane);
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (p + i < out.np) sum[i] += x[z * plane + i];
+                for (int i = 0; i < 4; ++i) sum[i] += x[z * plane + (p + i < out.np ? i : 0)];
+            }
+        }
         store4<T>(out, p, q, sum);
     }
 }
@@ -804,6 +871,96 @@ template <int TYPE> __global__ __launch_bounds__(256) void scale_kernel(Mx4Produ
     }
 }
 
+// Scales whose rows do not start at multiples of 4 bytes are copied to rows that do.
+bool aligned_scales(const Mx4View &v) { return (uintptr_t)v.scales % 4 == 0 && v.lds % 4 == 0; }
+size_t scales_work(const Mx4View &v) {
+    return aligned_scales(v) ? 0 : (size_t)((v.rows * ((mx4_blocks(v.cols) + 3) / 4 * 4) + 255) / 256 * 256);
+}
+__global__ __launch_bounds__(256) void copy_scales_kernel(const uint8_t *src, int64_t lds, int64_t rows, int nb, int nb4, uint8_t *dst) {
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b >= nb) return;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) dst[r * nb4 + b] = src[r * lds + b];
+}
+hipError_t align_scales(Mx4View &v, uint8_t *&work, hipStream_t s) {
+    if (aligned_scales(v)) return hipSuccess;
+    const int nb = (int)mx4_blocks(v.cols), nb4 = (nb + 3) / 4 * 4;
+    const dim3 grid((unsigned)((nb + 255) / 256), (unsigned)(v.rows < 65535 ? v.rows : 65535));
+    hipLaunchKernelGGL(copy_scales_kernel, grid, dim3(256), 0, s, v.scales, v.lds, v.rows, nb, nb4, work);
+    const size_t bytes = scales_work(v);
+    v.scales = work;
+    v.lds = nb4;
+    work += bytes;
+    return hipGetLastError();
+}
+
+constexpr size_t round256(size_t n) { return (n + 255) / 256 * 256; }
+
+template <typename T> hipError_t launch_join(const float *partial, int slices, const Out &out, hipStream_t s) {
+    const int64_t n = ((out.np + 3) / 4 * out.no + 255) / 256;
+    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, s, partial, slices, out);
+    return hipGetLastError();
+}
+
+// How a product of two 4-bit factors runs: tile 256 or 128, or 0 and the kernel for small ones
+struct BothPlan {
+    int tile, nf, df;
+    int slices;
+    size_t partials, scales;
+};
+BothPlan both_plan(const Mx4Product &p) {
+    BothPlan m{};
+    auto tiles = [&](int64_t b) { return ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
+    m.slices = 1;
+    m.scales = scales_work(p.XQ) + scales_work(p.Y);
+    m.tile = tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 0;
+    if (m.tile) return m;
+    const int64_t small = p.M < p.N ? p.M : p.N, large = p.M < p.N ? p.N : p.M;
+    auto groups = [&] { return ((large + 16 * m.nf - 1) / (16 * m.nf)) * ((small + 16 * m.df - 1) / (16 * m.df)); };
+    m.df = small <= 16 ? 1 : small <= 32 ? 2 : 4;
+    m.nf = 4;
+    while (groups() < 256 && m.nf > 1) {
+        m.nf /= 2;
+        if (m.df > 2) m.df = 2;
+        if (m.df == 2 && m.nf == 1) { m.nf = 2; break; }
+    }
+    const int64_t units = (p.K + 255) / 256;
+    while (groups() * m.slices < 256 && units / (m.slices * 2) >= 2 * ROWS_WAVES) m.slices *= 2;
+    if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
+    return m;
+}
+
+template <int TYPE> hipError_t both_t(const Mx4Product &q, uint8_t *work, hipStream_t s) {
+    typedef typename Elem<TYPE>::mem T;
+    const BothPlan m = both_plan(q);
+    Mx4Product p = q;
+    const bool xp = p.ci == 1;   // X's index is the contiguous one of C
+    const int64_t ld = xp ? p.cj : p.ci;
+    const Out out{p.C, ld, xp ? p.M : p.N, xp ? p.N : p.M, p.alpha, p.beta, (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
+    hipError_t e = align_scales(p.XQ, work, s);
+    if (e == hipSuccess) e = align_scales(p.Y, work, s);
+    if (e != hipSuccess) return e;
+    if (m.tile) {
+        // the factor whose rows are the contiguous index gives the operand whose 4 entries a lane holds
+        const Mx4View &P = xp ? p.XQ : p.Y, &O = xp ? p.Y : p.XQ;
+        return m.tile == 256 ? launch_both_tile<T, 256, 256, 128, 64>(P, O, out, s) : launch_both_tile<T, 128, 128, 64, 64>(P, O, out, s);
+    }
+    const bool xq = p.M >= p.N;   // the larger factor
+    const Mx4View &Q = xq ? p.XQ : p.Y, &D = xq ? p.Y : p.XQ;
+    float *partial = m.slices > 1 ? (float *)work : nullptr;
+    RowsOut o{p.C, xq ? p.ci : p.cj, xq ? p.cj : p.ci, Q.rows, D.rows, p.alpha, p.beta, partial};
+    if (partial) o.sq = xq == xp ? 1 : D.rows, o.sd = xq == xp ? Q.rows : 1;
+    const dim3 grid((unsigned)((Q.rows + 16 * m.nf - 1) / (16 * m.nf)), (unsigned)m.slices, (unsigned)((D.rows + 16 * m.df - 1) / (16 * m.df)));
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, dim3(ROWS_WAVES * 64), 0, s, Q, D, o); };
+    if (m.df == 4) go(both_rows_kernel<T, 4, 4>);
+    else if (m.df == 2 && m.nf == 4) go(both_rows_kernel<T, 4, 2>);
+    else if (m.df == 2) go(both_rows_kernel<T, 2, 2>);
+    else if (m.nf == 4) go(both_rows_kernel<T, 4, 1>);
+    else if (m.nf == 2) go(both_rows_kernel<T, 2, 1>);
+    else go(both_rows_kernel<T, 1, 1>);
+    e = hipGetLastError();
+    return e == hipSuccess && partial ? launch_join<T>(partial, m.slices, out, s) : e;
+}
+
 // How a mixed product runs
 struct MixedPlan {
     int rows;            // dense rows / 16 of the kernel for few rows, 0 for the tiles
@@ -813,7 +970,6 @@ struct MixedPlan {
     int slices, steps_z; // of the contraction, and steps of 64 in each
     size_t planes, partials, scales;   // workspace bytes
 };
-constexpr size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
 MixedPlan mixed_plan(const Mx4Product &p) {
     MixedPlan m{};
@@ -821,22 +977,23 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     // 16-byte pieces of 8 elements, whole ones only, rows within reach of a 32-bit offset
     m.direct = p.type == MX4_BF16 && p.X.sc == 1 && (uintptr_t)p.X.ptr % 16 == 0 && p.X.sr % 8 == 0 && p.K % 8 == 0 &&
                p.X.sr <= (1 << 21);
+    m.scales = scales_work(p.Y);
     m.ld = (p.K + 63) / 64 * 64;
     if (!m.direct) m.planes = round256((size_t)pl * p.M * m.ld * 2);
-    if (p.M <= 32) {
+    if (p.M <= (pl == 3 ? 16 : 32)) {   // 3 planes of 32 rows: more than LDS, or with blocks across the registers, hold
         m.rows = p.M <= 16 ? 1 : 2;
-        const int64_t groups = p.yt ? (p.N + 255) / 256 : (p.N + 63) / 64;
-        const int64_t units = p.yt ? (p.K + 31) / 32 : (p.K + 255) / 256;
-        // 64 columns a workgroup where that makes 256 of them, else fewer (a dense row is read by each)
-        // (64 x 32 in three planes does not fit the registers)
-        m.bq = p.yt ? 256 : p.N >= 64 * 256 && !(pl == 3 && m.rows == 2) ? 64 : p.N >= 32 * 256 ? 32 : 16;
+        // Columns a workgroup: each reads the dense rows whole, so enough that those are fewer bytes than its
+        // codes, and more where that still makes a workgroup for every compute unit. The contraction is cut
+        // until there are 256 workgroups.
+        m.bq = p.yt ? 256 : 16;
+        if (!p.yt)
+            while (m.bq < 64 && (m.bq < 4 * pl * p.M || p.N >= 512 * m.bq)) m.bq *= 2;
+        const int64_t groups = (p.N + m.bq - 1) / m.bq, units = p.yt ? (p.K + 31) / 32 : (p.K + 255) / 256;
         m.slices = 1;
-        if (p.yt)
-            while (groups * m.slices * 2 <= 512 && units / (m.slices * 2) >= 2 * ROWS_WAVES) m.slices *= 2;
+        while (groups * m.slices < 256 && units / (m.slices * 2) >= (p.yt ? 2 * ROWS_WAVES : dense_waves(pl * m.rows))) m.slices *= 2;
         if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
         return m;
     }
-    m.scales = scales_work(p.Y);
     const int64_t nq = p.N, nd = p.M;
     auto tiles = [&](int64_t q, int64_t d) { return ((nq + q - 1) / q) * ((nd + d - 1) / d); };
     m.bq = 256;
@@ -866,29 +1023,26 @@ hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, cons
     return hipGetLastError();
 }
 
-template <typename T> hipError_t launch_join(const float *partial, int slices, const Out &out, hipStream_t s) {
-    const int64_t n = ((out.np + 3) / 4 * out.no + 255) / 256;
-    hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, s, partial, slices, out);
-    return hipGetLastError();
-}
-
 template <typename T> hipError_t launch_mixed_rows(const Dense16 &D, const Mx4Product &p, const MixedPlan &m, const Out &final, bool qfirst, float *partial, hipStream_t s) {
     RowsOut out{p.C, p.cj, p.ci, p.N, p.M, p.alpha, p.beta, partial};
     if (partial) out.sq = qfirst ? 1 : p.M, out.sd = qfirst ? p.N : 1;
-    const dim3 grid((unsigned)((p.N + m.bq - 1) / m.bq), (unsigned)m.slices), block(ROWS_WAVES * 64);
-    const bool words = aligned_scales(p.Y), pairs = (uintptr_t)p.Y.scales % 2 == 0 && p.Y.lds % 2 == 0;
-    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, D, p.Y, pairs, out); };
+    const dim3 grid((unsigned)((p.N + m.bq - 1) / m.bq), (unsigned)m.slices), block((p.yt ? ROWS_WAVES : dense_waves(Planes<T>::N * m.rows)) * 64);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, D, p.Y, out); };
     if (p.yt) {
-        if (m.rows == 1) hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 1>), grid, block, 0, s, D, p.Y, words, (int)p.K, out);
-        else hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 2>), grid, block, 0, s, D, p.Y, words, (int)p.K, out);
-    } else if (m.rows == 1) {
+        if (m.rows == 1) hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 1>), grid, block, 0, s, D, p.Y, (int)p.K, out);
+        else if constexpr (Planes<T>::N < 3) hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 2>), grid, block, 0, s, D, p.Y, (int)p.K, out);
+    } else if (p.M <= 4) {
         if (m.bq == 64) go(mixed_rows_kernel<T, 4, 1>);
         else if (m.bq == 32) go(mixed_rows_kernel<T, 2, 1>);
         else go(mixed_rows_kernel<T, 1, 1>);
-    } else {
-        if (m.bq == 16) go(mixed_rows_kernel<T, 1, 2>);
-        else if (m.bq == 32) go(mixed_rows_kernel<T, 2, 2>);
-        else if constexpr (Planes<T>::N < 3) go(mixed_rows_kernel<T, 4, 2>);
+    } else if (m.rows == 1) {
+        if (m.bq == 64) go(mixed_rows_kernel<T, 4, 4>);
+        else if (m.bq == 32) go(mixed_rows_kernel<T, 2, 4>);
+        else go(mixed_rows_kernel<T, 1, 4>);
+    } else if constexpr (Planes<T>::N < 3) {
+        if (m.bq == 16) go(mixed_rows_kernel<T, 1, 8>);
+        else if (m.bq == 32) go(mixed_rows_kernel<T, 2, 8>);
+        else go(mixed_rows_kernel<T, 4, 8>);
     }
     const hipError_t e = hipGetLastError();
     return e == hipSuccess && partial ? launch_join<T>(partial, m.slices, final, s) : e;
@@ -902,8 +1056,7 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     const int64_t ld = qfirst ? p.ci : p.cj;
     const Out out{p.C, ld, qfirst ? p.N : p.M, qfirst ? p.M : p.N, p.alpha, p.beta,
                   (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
-    hipError_t e = hipSuccess;
-    if (!m.rows) e = align_scales(p.Y, work, s);
+    hipError_t e = align_scales(p.Y, work, s);
     if (e != hipSuccess) return e;
     Dense16 D{(const uint16_t *)p.X.ptr, p.M, p.X.sr, 0, (int)(p.K / 8)};
     if (!m.direct) {
@@ -950,7 +1103,10 @@ template <int TYPE> hipError_t product_t(const Mx4Product &p, void *work, hipStr
 
 size_t mx4_product_work(const Mx4Product &p) {
     if (p.K <= 0 || p.alpha == 0.f) return 0;
-    if (p.both) return scales_work(p.XQ) + scales_work(p.Y);
+    if (p.both) {
+        const BothPlan b = both_plan(p);
+        return b.scales + b.partials;
+    }
     const MixedPlan m = mixed_plan(p);
     return m.scales + m.planes + m.partials;
 }
