@@ -1882,8 +1882,9 @@ bool mx4_ok(const rbh_mx4 *Q) {
     return Q != nullptr && Q->n_rows >= 0 && Q->n_cols >= 0 &&
            (Q->n_rows == 0 || Q->n_cols == 0 || (Q->codes != nullptr && Q->scales != nullptr));
 }
-// the window of rows x cols of Q at (ro, co), staged
-int mx4_window(Stager &st, const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t rows, int64_t cols, bool out, Mx4View &v) {
+// the window of rows x cols of Q at (ro, co); what is not on a device (DeviceOf::look) is staged
+int mx4_window(Stager &st, bool codes_here, bool scales_here, const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t rows,
+               int64_t cols, bool out, Mx4View &v) {
     v = Mx4View{};
     v.rows = rows;
     v.cols = cols;
@@ -1892,10 +1893,14 @@ int mx4_window(Stager &st, const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t row
     if (rows == 0 || cols == 0) return RBH_OK;
     const int64_t nb = mx4_blocks(cols);
     uint8_t *q = Q->codes + ro * Q->ld_codes + co / 2, *sc = Q->scales + ro * Q->ld_scales + co / MX4_BLOCK;
-    RBH_HIP(st.map_window(q, (size_t)extent('R', rows, nb * 16, Q->ld_codes), !out, out, (size_t)(nb * 16), (size_t)rows,
-                          (size_t)Q->ld_codes, (void **)&v.codes));
-    RBH_HIP(st.map_window(sc, (size_t)extent('R', rows, nb, Q->ld_scales), !out, out, (size_t)nb, (size_t)rows,
-                          (size_t)Q->ld_scales, (void **)&v.scales));
+    v.codes = q;
+    v.scales = sc;
+    if (!codes_here)
+        RBH_HIP(st.map_window(q, (size_t)extent('R', rows, nb * 16, Q->ld_codes), !out, out, (size_t)(nb * 16), (size_t)rows,
+                              (size_t)Q->ld_codes, (void **)&v.codes));
+    if (!scales_here)
+        RBH_HIP(st.map_window(sc, (size_t)extent('R', rows, nb, Q->ld_scales), !out, out, (size_t)nb, (size_t)rows,
+                              (size_t)Q->ld_scales, (void **)&v.scales));
     return RBH_OK;
 }
 
@@ -1928,17 +1933,15 @@ int mx4_quantize(int type, char layout, char op, int64_t n_rows, int64_t n_cols,
     const bool empty = n_rows == 0 || n_cols == 0;
     RBH_REQUIRE(empty || A != nullptr);
     DeviceOf dev;
-    dev.look(A);
-    dev.look(Q->codes);
-    dev.look(Q->scales);
+    const bool a_here = dev.look(A), codes_here = dev.look(Q->codes), scales_here = dev.look(Q->scales);
     RBH_REQUIRE_AS(!dev.differ, "all arrays on one device", __func__);
     RBH_HIP(dev.enter());
     hipStream_t s = (hipStream_t)stream;
     Stager st(s);
-    void *dA;
-    RBH_HIP(st.map(A, (size_t)mx4_size(type) * (size_t)extent(layout, rows_A, cols_A, lda), true, false, &dA));
+    void *dA = const_cast<void *>(A);
+    if (!a_here) RBH_HIP(st.map(A, (size_t)mx4_size(type) * (size_t)extent(layout, rows_A, cols_A, lda), true, false, &dA));
     Mx4View v;
-    const int rc = mx4_window(st, Q, 0, 0, n_rows, n_cols, true, v);
+    const int rc = mx4_window(st, codes_here, scales_here, Q, 0, 0, n_rows, n_cols, true, v);
     if (rc) return rc;
     const bool along = (layout == 'R') == (op == 'N');   // a row of op(A) is contiguous
     const Mx4Dense a{dA, along ? lda : 1, along ? 1 : lda, type};
@@ -1970,17 +1973,15 @@ int mx4_dequantize(int type, char layout, char op, int64_t n_rows, int64_t n_col
     const bool empty = n_rows == 0 || n_cols == 0;
     RBH_REQUIRE(empty || A != nullptr);
     DeviceOf dev;
-    dev.look(A);
-    dev.look(Q->codes);
-    dev.look(Q->scales);
+    const bool a_here = dev.look(A), codes_here = dev.look(Q->codes), scales_here = dev.look(Q->scales);
     RBH_REQUIRE_AS(!dev.differ, "all arrays on one device", __func__);
     RBH_HIP(dev.enter());
     hipStream_t s = (hipStream_t)stream;
     Stager st(s);
-    void *dA;
-    RBH_HIP(st.map_out(A, (size_t)mx4_size(type), layout, rows_A, cols_A, lda, false, &dA));
+    void *dA = A;
+    if (!a_here) RBH_HIP(st.map_out(A, (size_t)mx4_size(type), layout, rows_A, cols_A, lda, false, &dA));
     Mx4View v;
-    const int rc = mx4_window(st, Q, ro, co, n_rows, n_cols, false, v);
+    const int rc = mx4_window(st, codes_here, scales_here, Q, ro, co, n_rows, n_cols, false, v);
     if (rc) return rc;
     const bool along = (layout == 'R') == (op == 'N');
     const Mx4Dense a{dA, along ? lda : 1, along ? 1 : lda, type};
@@ -2013,11 +2014,11 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
     if (work) RBH_REQUIRE(work->bytes >= 0);
 
     DeviceOf dev;
-    dev.look(C);
-    if (side != 'B') dev.look(D);
-    if (side != 'R') dev.look(QA->codes), dev.look(QA->scales);
-    if (side != 'L') dev.look(QB->codes), dev.look(QB->scales);
-    if (work) dev.look(work->ptr);
+    const bool c_here = dev.look(C), d_here = dev.look(D);
+    bool qa_here[2] = {}, qb_here[2] = {};
+    if (side != 'R') qa_here[0] = dev.look(QA->codes), qa_here[1] = dev.look(QA->scales);
+    if (side != 'L') qb_here[0] = dev.look(QB->codes), qb_here[1] = dev.look(QB->scales);
+    const bool work_here = work && dev.look(work->ptr);
     RBH_REQUIRE_AS(!dev.differ, "all arrays on one device", __func__);
     RBH_HIP(dev.enter());
     const bool query = work && !work->ptr;
@@ -2031,20 +2032,20 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
     p.both = side == 'B';
     void *dC = C, *dD = const_cast<void *>(D);
     if (!query) {
-        RBH_HIP(st.map_out(C, (size_t)mx4_size(type), layout, m, n, ldc, beta != 0.f, &dC));
-        if (side != 'B' && reads) {
+        if (!c_here) RBH_HIP(st.map_out(C, (size_t)mx4_size(type), layout, m, n, ldc, beta != 0.f, &dC));
+        if (side != 'B' && reads && !d_here) {
             const int64_t r = side == 'R' ? rows_A : rows_B, c = side == 'R' ? cols_A : cols_B;
             RBH_HIP(st.map(D, (size_t)mx4_size(type) * (size_t)extent(layout, r, c, ldd), true, false, &dD));
         }
     }
     p.C = dC;
-    auto view = [&](const rbh_mx4 *Q, int64_t ro, int64_t co, int64_t rows, int64_t cols, Mx4View &v) -> int {
+    auto view = [&](const rbh_mx4 *Q, const bool *here, int64_t ro, int64_t co, int64_t rows, int64_t cols, Mx4View &v) -> int {
         if (query || !reads) {
             v = Mx4View{Q->codes + ro * Q->ld_codes + co / 2, Q->scales + ro * Q->ld_scales + co / MX4_BLOCK, Q->ld_codes,
                         Q->ld_scales, rows, cols};
             return RBH_OK;
         }
-        return mx4_window(st, Q, ro, co, rows, cols, false, v);
+        return mx4_window(st, here[0], here[1], Q, ro, co, rows, cols, false, v);
     };
     const int64_t cr = layout == 'C' ? 1 : ldc, cc = layout == 'C' ? ldc : 1;   // strides of C along rows, columns
     int rc;
@@ -2053,18 +2054,18 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
         const bool along = (layout == 'R') == (opB == 'T');   // op(B)^T has contiguous rows
         p.X = Mx4Dense{dD, along ? ldd : 1, along ? 1 : ldd, type};
         p.yt = opA == 'T';
-        rc = view(QA, ro_a, co_a, rows_A, cols_A, p.Y);
+        rc = view(QA, qa_here, ro_a, co_a, rows_A, cols_A, p.Y);
     } else {
         p.M = m; p.N = n; p.ci = cr; p.cj = cc;
         if (side == 'R') {
             const bool along = (layout == 'R') == (opA == 'N');
             p.X = Mx4Dense{dD, along ? ldd : 1, along ? 1 : ldd, type};
         } else {
-            rc = view(QA, ro_a, co_a, rows_A, cols_A, p.XQ);
+            rc = view(QA, qa_here, ro_a, co_a, rows_A, cols_A, p.XQ);
             if (rc) return rc;
         }
         p.yt = opB == 'N';
-        rc = view(QB, ro_b, co_b, rows_B, cols_B, p.Y);
+        rc = view(QB, qb_here, ro_b, co_b, rows_B, cols_B, p.Y);
     }
     if (rc) return rc;
     const size_t need = empty ? 0 : mx4_product_work(p);
@@ -2076,7 +2077,7 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
     if (need) {
         if (work) {
             RBH_REQUIRE(work->bytes >= (int64_t)need && (uintptr_t)work->ptr % 256 == 0);
-            RBH_REQUIRE(is_device_ptr(work->ptr));
+            RBH_REQUIRE(work_here);
             ws.p = work->ptr;
         } else {
             // a graph would keep the arena's block, which later calls and other graphs use as well

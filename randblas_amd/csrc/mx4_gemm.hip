@@ -1,5 +1,6 @@
 // mx4_gemm.hip -- products with 4-bit microscaled matrices (gfx950).
 #include <type_traits>
+#include <utility>
 
 #include "common.hpp"
 #include "mx4.hpp"
@@ -29,6 +30,21 @@ __device__ __forceinline__ v4f mfma_mx4(v4i a, v4i b, v4f c, int sa, int sb) {
     const v8i wb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
     return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(wa, wb, c, 4, 4, 0, sa, 0, sb);
 }
+
+// the same in 32 x 32: lane l holds row l & 31 and the block l >> 5 of 2; D: column l & 31, rows 8 i + 4 (l >> 5)
+// .. + 3 in entries 4 i .. + 3. Fed from registers by 2 waves a SIMD the 16 x 16 instruction reaches 5.46
+// PFLOP/s on random codes, this one 6.51 (power is the bound: on zeros 9.63)
+typedef float v16f __attribute__((ext_vector_type(16)));
+template <int OA, int OB> __device__ __forceinline__ v16f mfma_mx4_32(v4i a, v4i b, v16f c, int sa, int sb) {
+    const v8i wa = __builtin_shufflevector(a, a, 0, 1, 2, 3, -1, -1, -1, -1);
+    const v8i wb = __builtin_shufflevector(b, b, 0, 1, 2, 3, -1, -1, -1, -1);
+    return __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(wa, wb, c, 4, 4, OA, sa, OB, sb);
+}
+
+template <typename F, int... I> __device__ __forceinline__ void static_for_(F &&f, std::integer_sequence<int, I...>) {
+    (f(std::integral_constant<int, I>{}), ...);
+}
+template <int N, typename F> __device__ __forceinline__ void static_for(F &&f) { static_for_(f, std::make_integer_sequence<int, N>{}); }
 
 // out[o * ld + p] = alpha * sum + beta * out[o * ld + p]
 struct Out {
@@ -118,23 +134,111 @@ __device__ __forceinline__ void tile_of(uint32_t bid, uint32_t tp, uint32_t to, 
     ip = in / h;
 }
 
+// Scales as the tile kernel reads them: for 8 blocks of columns and 128 rows 1024 bytes, the scale of block k and
+// row 32 f + r at byte 128 k + 4 r + f. A word then serves a lane's 4 operands, and a step's scales of a tile
+// are contiguous; from their own rows, 8 bytes each, they cost more than all codes (8192^3 without the
+// products: 162 us for the codes alone, 290 us with scales by rows). Zeros stand for what is not there.
+constexpr int PACK_BLOCKS = 64;   // of columns a workgroup
+struct PackJob {
+    const uint8_t *src;
+    int64_t lds, rows;
+    uint32_t *dst;
+};
+int64_t pack_groups(const Mx4View &v) { return (v.rows + 127) / 128; }
+size_t packed_scales(const Mx4View &v) { return (size_t)(pack_groups(v) * ((mx4_blocks(v.cols) + 7) / 8) * 1024); }
+
+__global__ __launch_bounds__(256) void pack_scales_kernel(PackJob a, PackJob b, unsigned groups_a, int nb, int steps) {
+    constexpr int PITCH = 132;   // bytes a block, so that those of a row are on different banks
+    __shared__ __attribute__((aligned(16))) uint8_t packed[PACK_BLOCKS * PITCH];
+    const PackJob &j = blockIdx.y < groups_a ? a : b;
+    const int64_t group = blockIdx.y < groups_a ? blockIdx.y : blockIdx.y - groups_a, groups = (j.rows + 127) / 128;
+    const int b0 = blockIdx.x * PACK_BLOCKS;
+    const int w = threadIdx.x & 15, k0 = b0 + 4 * w;   // 16 threads a row, 4 scales each
+    const bool words = (uintptr_t)j.src % 4 == 0 && j.lds % 4 == 0;
+    const int64_t row0 = group * 128;
+    uint32_t v[8];
+    if (words) {   // all loads at once
+        const int64_t left = j.rows - row0 < 128 ? j.rows - row0 : 128;
+        const Buffer sb = buffer(j.src + row0 * j.lds, (uint32_t)((left - 1) * j.lds + (nb + 3) / 4 * 4));
+        const uint32_t keep = nb - k0 >= 4 ? ~0u : nb > k0 ? (1u << (8 * (nb - k0))) - 1 : 0u;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = load4(sb, k0 < nb ? (uint32_t)((i * 16 + (threadIdx.x >> 4)) * j.lds) + k0 : OUTSIDE, 0) & keep;
+    } else {
+        for (int i = 0; i < 8; ++i) {
+            const int64_t row = row0 + i * 16 + (threadIdx.x >> 4);
+            v[i] = 0;
+            for (int q = 0; q < 4; ++q)
+                if (row < j.rows && k0 + q < nb) v[i] |= (uint32_t)j.src[row * j.lds + k0 + q] << (8 * q);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int r = i * 16 + (threadIdx.x >> 4);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) packed[(4 * w + q) * PITCH + (r & 31) * 4 + (r >> 5)] = (uint8_t)(v[i] >> (8 * q));
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PACK_BLOCKS * 32 / 256; ++i) {
+        const int word = i * 256 + threadIdx.x, step = b0 / 8 + word / 256;   // 256 words a step
+        if (step < steps) j.dst[((int64_t)step * groups + group) * 256 + (word & 255)] =
+            ((const uint32_t *)packed)[word / 32 * (PITCH / 4) + word % 32];
+    }
+}
+
+// this slice's partial sums as a result: [slice][no][np]
+__device__ __forceinline__ Out partial_of(const Out &o, float *partial) {
+    return Out{partial + (int64_t)blockIdx.y * o.np * o.no, o.np, o.np, o.no, 1.f, 0.f, o.np % 4 == 0};
+}
+
+// A wave's WP x RO part of a result, RO rows of p after each other in LDS, to memory in whole lines: operands
+// hold 4 consecutive entries of many rows, and stores of those are 16 bytes to a line. `pitch` words a row.
+template <typename T, int WP, int RO>
+__device__ __forceinline__ void store_rows(const Out &o, const float *from, int pitch, int64_t p0, int64_t q0, int lane) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    if (o.vec) {
+        constexpr int L = WP / 4, R = 64 / L;   // lanes a row, rows at once
+        static_assert(64 % L == 0 && RO % R == 0, "whole rows");
+#pragma unroll 4
+        for (int r = 0; r < RO; r += R) {
+            const int row = r + lane / L, p = lane % L * 4;
+            store4<T>(o, p0 + p, q0 + row, *(const v4f *)(from + row * pitch + p));
+        }
+    } else {
+        for (int r = 0; r < RO; ++r) {
+            if (q0 + r >= o.no) break;
+            T *c = (T *)o.ptr + (q0 + r) * o.ld + p0;
+#pragma unroll
+            for (int p = lane; p < WP; p += 64)
+                if (p0 + p < o.np) {
+                    const float v = o.alpha * from[r * pitch + p];
+                    c[p] = (T)(o.beta != 0.f ? v + o.beta * (float)c[p] : v);
+                }
+        }
+    }
+}
+
 // BP x BO entries of the result a workgroup, WP x WO a wave; 256 columns (8 blocks) of both factors a step,
-// loaded straight to LDS, double-buffered. A row of a step is 128 bytes of codes; its 16-byte blocks are
-// kept at place block ^ (row / 2 & 7), which spreads the 16 rows that a matrix operand reads at once over
-// all banks (the lane that fills a place loads the block that belongs there). A row's 8 scale bytes lie
-// behind the codes.
+// loaded straight to LDS, double-buffered. A row of a step is 128 bytes of codes, a whole line; its 16-byte
+// blocks are kept at place block ^ (row / 2 & 7), which spreads the 16 rows that an access takes at once over
+// all banks (the lane that fills a place loads the block that belongs there). The packed scales lie behind
+// the codes.
 template <typename T, int BP, int BO, int WP, int WO>
-__global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kernel(Mx4View P, Mx4View O, int nb, Out out) {
+__global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kernel(Mx4View P, Mx4View O, const uint8_t *ps, const uint8_t *os,
+                                                                                  int nb, int steps_z, Out out, float *partial) {
     constexpr int NW = (BP / WP) * (BO / WO), NT = NW * 64;
-    constexpr int FP = WP / 16, FO = WO / 16;
+    constexpr int FP = WP / 32, FO = WO / 32;
     constexpr int ROWS = BP + BO;                       // rows staged, P's first
     constexpr int LP = BP * 8 / NT, LO = BO * 8 / NT;   // 16-byte loads a thread
     static_assert(BP * 8 % NT == 0 && BO * 8 % NT == 0 && NT / 8 % 16 == 0, "whole loads, one block for all rows of a thread");
-    constexpr int SL = ROWS * 2 / NT;                   // 4-byte loads of scales a thread
-    static_assert(ROWS * 2 % NT == 0 && BP % 32 == 0, "whole loads of one factor");
-    __shared__ __attribute__((aligned(16))) uint8_t lds0[ROWS * 136], lds1[ROWS * 136];
+    constexpr int SL = ROWS / 128;                      // waves that load scales, 128 rows each
+    static_assert(BP % 128 == 0 && BO % 128 == 0 && SL <= NW && 128 % WO == 0 && 128 % WP == 0, "scales by 128 rows");
+    constexpr int STAGE = ROWS * 136, PITCH = WP + 4;
+    constexpr int LDS = 2 * STAGE > NW * 32 * PITCH * 4 ? 2 * STAGE : NW * 32 * PITCH * 4;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int r16 = lane & 15, g = lane >> 4;
+    const int r32 = lane & 31, g = lane >> 5;
     uint32_t ip, io;
     tile_of(blockIdx.x, (uint32_t)((P.rows + BP - 1) / BP), (uint32_t)((O.rows + BO - 1) / BO), ip, io);
     const int64_t p0 = (int64_t)ip * BP, o0 = (int64_t)io * BO;
@@ -143,93 +247,112 @@ __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kerne
     const int np = (int)(P.rows - p0 < BP ? P.rows - p0 : BP), no = (int)(O.rows - o0 < BO ? O.rows - o0 : BO);
     const Buffer pb = buffer(P.codes + p0 * P.ldq, (uint32_t)((np - 1) * P.ldq + nb * 16));
     const Buffer ob = buffer(O.codes + o0 * O.ldq, (uint32_t)((no - 1) * O.ldq + nb * 16));
-    const Buffer ps = buffer(P.scales + p0 * P.lds, (uint32_t)((np - 1) * P.lds + (nb + 3) / 4 * 4));
-    const Buffer os = buffer(O.scales + o0 * O.lds, (uint32_t)((no - 1) * O.lds + (nb + 3) / 4 * 4));
-    const int block = (tid & 7) ^ ((tid >> 4) & 7);
+    const int block = (tid & 7) ^ ((tid >> 4) & 7), steps = (nb + 7) / 8;
+    const int t0 = blockIdx.y * steps_z, t1 = t0 + steps_z < steps ? t0 + steps_z : steps;   // this slice's
     const uint32_t vp = (uint32_t)((tid >> 3) * P.ldq) + block * 16, vo = (uint32_t)((tid >> 3) * O.ldq) + block * 16;
     const uint32_t rp = (uint32_t)P.ldq * (NT / 8), ro = (uint32_t)O.ldq * (NT / 8);
-    // blocks b0 .. b0 + 7 of every row; those past the last are zero
-    auto load = [&](int b0, uint8_t *lds) {
-        const bool in = b0 + block < nb;
-#pragma unroll
-        for (int i = 0; i < LP; ++i) load_lds16(pb, lds + (i * NT + wave * 64) * 16, in ? vp + i * rp : OUTSIDE, b0 * 16);
-#pragma unroll
-        for (int i = 0; i < LO; ++i)
-            load_lds16(ob, lds + BP * 128 + (i * NT + wave * 64) * 16, in ? vo + i * ro : OUTSIDE, b0 * 16);
-#pragma unroll
-        for (int i = 0; i < SL; ++i) {   // a wave's 32 rows are of one factor
-            const int w = i * NW + wave, row = w * 32 + (lane >> 1), half = lane & 1;
-            uint8_t *to = lds + ROWS * 128 + w * 256;
-            const bool in = b0 + 4 * half < nb;
-            if (w * 32 < BP) load_lds4(ps, to, in ? (uint32_t)(row * P.lds) + 4 * half : OUTSIDE, b0);
-            else load_lds4(os, to, in ? (uint32_t)((row - BP) * O.lds) + 4 * half : OUTSIDE, b0);
+    // scales of this wave's 128 rows (of the first SL waves)
+    const bool sp = wave * 128 < BP;
+    const int64_t sg = ((sp ? P.rows : O.rows) + 127) / 128, s0 = sp ? p0 / 128 + wave : o0 / 128 + wave - BP / 128;
+    const bool have = wave < SL && s0 < sg;
+    const uint8_t *sbase = (sp ? ps : os) + (have ? s0 : 0) * 1024;
+    // blocks 8 t .. 8 t + 7 of every row; those past the last are zero. Half h of the loads
+    auto load = [&](int t, uint8_t *to, int h) {
+        const bool in = t * 8 + block < nb;
+        if (h == 0 && wave < SL) {
+            const bool all = have && t < steps;
+            load_lds16(buffer(sbase + (all ? t : 0) * sg * 1024, all ? 1024u : 0u), to + ROWS * 128 + wave * 1024, lane * 16, 0);
         }
+#pragma unroll
+        for (int i = h * LP / 2; i < (h + 1) * LP / 2; ++i) load_lds16(pb, to + (i * NT + wave * 64) * 16, in ? vp + i * rp : OUTSIDE, t * 128);
+#pragma unroll
+        for (int i = h * LO / 2; i < (h + 1) * LO / 2; ++i) load_lds16(ob, to + BP * 128 + (i * NT + wave * 64) * 16, in ? vo + i * ro : OUTSIDE, t * 128);
     };
 
-    v4f acc[FP][FO];
+    v16f acc[FP][FO];
 #pragma unroll
     for (int a = 0; a < FP; ++a)
 #pragma unroll
-        for (int b = 0; b < FO; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+        for (int b = 0; b < FO; ++b) acc[a][b] = v16f{};
 
-    // LDS places of this lane: one address a factor and half step, everything else an immediate
-    int at[2];
+    // LDS places of this lane: one address a factor and quarter step, everything else an immediate
+    int at[4];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) at[h] = ((h * 4 + g) ^ ((r16 >> 1) & 7)) * 16 + r16 * 128;
-    const int pa = wp * WP * 128, pb_ = (BP + wo * WO) * 128;
-    const int psc = ROWS * 128 + (wp * WP + r16) * 8, osc = ROWS * 128 + (BP + wo * WO + r16) * 8;
-    auto compute = [&](int b0, const uint8_t *lds) {
-        const uint8_t *ssa = lds + psc, *ssb = lds + osc;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const uint8_t *ca = lds + (pa + at[h]), *cb = lds + (pb_ + at[h]);
-            v4i a[FP], b[FO];
-            uint32_t sa[FP], sb[FO];
-            const uint32_t width = b0 + h * 4 + g < nb ? 8 : 0;   // scales past the last block, whatever is there, as 0
-#pragma unroll
-            for (int f = 0; f < FO; ++f) {
-                b[f] = *(const v4i *)(cb + f * 16 * 128);
-                sb[f] = __builtin_amdgcn_ubfe(*(const uint32_t *)(ssb + f * 16 * 8 + h * 4), 8 * g, width);
-            }
-#pragma unroll
-            for (int f = 0; f < FP; ++f) {
-                a[f] = *(const v4i *)(ca + f * 16 * 128);
-                sa[f] = __builtin_amdgcn_ubfe(*(const uint32_t *)(ssa + f * 16 * 8 + h * 4), 8 * g, width);
-            }
-#pragma unroll
-            for (int fa = 0; fa < FP; ++fa)
-#pragma unroll
-                for (int fb = 0; fb < FO; ++fb) acc[fa][fb] = mfma_mx4(a[fa], b[fb], acc[fa][fb], (int)sa[fa], (int)sb[fb]);
-        }
+    for (int h = 0; h < 4; ++h) at[h] = ((h * 2 + g) ^ ((r32 >> 1) & 7)) * 16 + r32 * 128;
+    const int pa = wp * WP * 128, oa = (BP + wo * WO) * 128;
+    const int psc = ROWS * 128 + (wp * WP) / 128 * 1024 + g * 128 + r32 * 4, pbit = wp * WP % 128 / 32 * 8;
+    const int osc = ROWS * 128 + (BP + wo * WO) / 128 * 1024 + g * 128 + r32 * 4, obit = wo * WO % 128 / 32 * 8;
+    struct Operands {
+        v4i a[FP], b[FO];
+        uint32_t sa, sb;
     };
-    // two steps a round, so that each works on its own array and its loads are seen to go to the other
-    load(0, lds0);
-    arrive();
-    int b0 = 0;
-    for (; b0 + 8 < nb; b0 += 16) {
-        load(b0 + 8, lds1);
-        __builtin_amdgcn_sched_barrier(0);   // the loads leave before the products, not behind them
-        compute(b0, lds0);
-        arrive();
-        load(b0 + 16, lds0);   // past the last block: nothing but zeros, unread or added
-        __builtin_amdgcn_sched_barrier(0);
-        compute(b0 + 8, lds1);
-        arrive();
-    }
-    if (b0 < nb) compute(b0, lds0);
+    auto read = [&](const uint8_t *from, int h, Operands &x) {
+        const uint8_t *ca = from + (pa + at[h]), *cb = from + (oa + at[h]);
+        x.sa = *(const uint32_t *)(from + psc + h * 256) >> pbit;
+        x.sb = *(const uint32_t *)(from + osc + h * 256) >> obit;
 #pragma unroll
-    for (int b = 0; b < FO; ++b)
+        for (int f = 0; f < FO; ++f) x.b[f] = *(const v4i *)(cb + f * 32 * 128);
+#pragma unroll
+        for (int f = 0; f < FP; ++f) x.a[f] = *(const v4i *)(ca + f * 32 * 128);
+    };
+    auto multiply = [&](const Operands &x) {
+        static_for<FP>([&](auto fa) {
+            static_for<FO>([&](auto fb) {
+                constexpr int A = decltype(fa)::value, B = decltype(fb)::value;
+                acc[A][B] = mfma_mx4_32<A, B>(x.a[A], x.b[B], acc[A][B], (int)x.sa, (int)x.sb);
+            });
+        });
+    };
+    load(t0, lds, 0);
+    load(t0, lds, 1);
+    arrive();
+    int now = 0;
+    for (int t = t0; t < t1; ++t) {
+        // A quarter's products run beside the reads for the next one. The next step's loads go before the first
+        // two: all at the start would keep the waves from their products until the last is issued, spread
+        // over all four the last ones come late (8192^3: 301 and 298 us, this 278)
+        Operands x[2];
+        read(lds + now, 0, x[0]);
+#pragma unroll
+        for (int h = 0; h < 4; ++h) {
+            if (h < 2) load(t + 1, lds + STAGE - now, h);   // past the last step nothing but zeros
+            if (h < 3) read(lds + now, h + 1, x[(h + 1) & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+            multiply(x[h & 1]);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        arrive();
+        now = STAGE - now;
+    }
+    float *rows = (float *)lds + wave * 32 * PITCH;   // this wave's
+#pragma unroll
+    for (int b = 0; b < FO; ++b) {
 #pragma unroll
         for (int a = 0; a < FP; ++a)
-            store4<T>(out, p0 + wp * WP + a * 16 + 4 * g, o0 + wo * WO + b * 16 + r16, acc[a][b]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(v4f *)(rows + r32 * PITCH + a * 32 + 8 * i + 4 * g) =
+                    v4f{acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
+        __builtin_amdgcn_wave_barrier();
+        if (partial) store_rows<float, WP, 32>(partial_of(out, partial), rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, lane);
+        else store_rows<T, WP, 32>(out, rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, lane);
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 template <typename T, int BP, int BO, int WP, int WO>
-hipError_t launch_both_tile(const Mx4View &P, const Mx4View &O, const Out &out, hipStream_t s) {
-    const int nb = (int)mx4_blocks(P.cols);
+hipError_t launch_both_tile(const Mx4View &P, const Mx4View &O, uint8_t *work, int slices, int steps_z, const Out &out, float *partial, hipStream_t s) {
+    const int nb = (int)mx4_blocks(P.cols), steps = (nb + 7) / 8;
+    uint8_t *ps = work, *os = work + packed_scales(P);
+    const unsigned gp = (unsigned)pack_groups(P), go = (unsigned)pack_groups(O);
+    hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((nb + PACK_BLOCKS - 1) / PACK_BLOCKS), gp + go), dim3(256), 0, s,
+                       PackJob{P.scales, P.lds, P.rows, (uint32_t *)ps}, PackJob{O.scales, O.lds, O.rows, (uint32_t *)os}, gp, nb, steps);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
     const int64_t tiles = ((P.rows + BP - 1) / BP) * ((O.rows + BO - 1) / BO);
     constexpr int NT = (BP / WP) * (BO / WO) * 64;
-    hipLaunchKernelGGL((both_tile_kernel<T, BP, BO, WP, WO>), dim3((unsigned)tiles), dim3(NT), 0, s, P, O, nb, out);
+    hipLaunchKernelGGL((both_tile_kernel<T, BP, BO, WP, WO>), dim3((unsigned)tiles, (unsigned)slices), dim3(NT), 0, s, P, O, ps, os, nb, steps_z,
+                       out, partial);
     return hipGetLastError();
 }
 
@@ -320,8 +443,20 @@ struct Dense16 {
     int chunks;
 };
 
+// The pipeline of the tile kernels: a ring of NS stages in LDS, loaded NS - 1 steps ahead. A step waits for its
+// own wave's loads of the stage, then at the barrier for the other waves', which also says that all are done
+// with the stage that the next loads overwrite. `per_step` loads a wave are issued a step, so those of the
+// stage have arrived when no more than (NS - 2) per_step are on their way; past the last step loads go on
+// (of nothing), to keep that count.
+template <int NS, int PER_STEP> __device__ __forceinline__ void stage_ready() {
+    wait_loads<(NS - 2) * PER_STEP>();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
 // BQ rows (YT: columns) of the 4-bit factor x BD rows of the dense one a workgroup, WQ x WD a wave; 64
-// elements of the contraction a step, loaded straight to LDS, double-buffered.
+// elements of the contraction a step.
 //
 // A step's two matrix instructions take their 32 elements from all over the 64: lane group g holds
 // elements 16 g + 8 t .. + 7 of both factors for instruction t, so a lane's 16 codes lie in one word pair
@@ -331,8 +466,8 @@ struct Dense16 {
 //   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes a word (8 columns 8 c .. +
 //     7) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 8
 //     operands are then columns 8 c + f, and the operand f of the wave is columns f, f + 8, .. -- an order of
-//     the result's rows or columns that the stores undo. Scales are kept as the upper halves of floats.
-template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, bool QFIRST>
+//     the result's rows or columns that the stores undo. Scales: word w of the rows after each other.
+template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, int NS, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
     constexpr int NW = (BQ / WQ) * (BD / WD), NT = NW * 64;
@@ -344,10 +479,10 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     constexpr int DENSE = PL * BD * 128;
     constexpr int PITCH = YT ? (BQ == 256 ? 1056 : 1088) : 1024;   // 64 lanes' codes; lane groups on different banks
     constexpr int CODES = NW * PITCH;
-    constexpr int SCALES = YT ? BQ / 32 * 128 : BQ * 4;
-    constexpr int STAGE = DENSE + CODES + SCALES;
-    static_assert(2 * STAGE <= 160 * 1024, "LDS");
-    __shared__ __attribute__((aligned(16))) uint8_t lds0[STAGE], lds1[STAGE];
+    constexpr int SW = YT ? BQ / 128 : BQ / 64;               // waves that load scales, 64 words each
+    constexpr int STAGE = DENSE + CODES + SW * 256;
+    static_assert(NS * STAGE <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[NS * STAGE];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const int64_t nq = YT ? Y.cols : Y.rows;
@@ -380,8 +515,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
         vq = (uint32_t)((wave * 32 + (lane >> 1)) * Y.ldq) + qpart * 16;
         vs = (uint32_t)((wave * 64 + lane) * Y.lds);
     }
-    uint32_t sreg = 0;   // YT: 4 scales of a row on their way to LDS
-    auto load = [&](int step, uint8_t *lds) {
+    auto load = [&](int step, uint8_t *to) {
         if constexpr (YT) {
             const int64_t k0 = (int64_t)step * 64;
             const int64_t left = K - k0 < 64 ? K - k0 : 64;
@@ -390,40 +524,19 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             // past the last step the range is empty, and reads zeros
             const Buffer cb = buffer(Y.codes + q0 / 2 + (have ? k0 : 0) * Y.ldq, have * ((rows - 1) * (uint32_t)Y.ldq + nb * 16));
             const Buffer kb = buffer(Y.scales + q0 / 32 + (have ? k0 : 0) * Y.lds, have * ((rows - 1) * (uint32_t)Y.lds + (nb + 3) / 4 * 4));
-            constexpr int WR = BQ / 128;                  // words of scales a row
-            if (tid < 64 * WR) {
-                const int w = tid % WR;
-                sreg = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, w * 4 < nb ? (int)((tid / WR) * Y.lds + w * 4) : (int)OUTSIDE, 0, 0);
-            }
-            load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
+            load_lds16(cb, to + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
+            if (wave < SW) load_lds4(kb, to + DENSE + CODES + wave * 256, wave * 4 < nb ? (uint32_t)(lane * Y.lds) + wave * 4 : OUTSIDE, 0);
         } else {
-            load_lds16(qb, lds + DENSE + wave * PITCH, step * 2 + qpart < nb ? vq : OUTSIDE, step * 32);
-            if (wave < BQ / 64) load_lds4(sb, lds + DENSE + CODES + wave * 256, step * 2 < nb ? vs : OUTSIDE, step * 2 / 4 * 4);
+            load_lds16(qb, to + DENSE + wave * PITCH, step * 2 + qpart < nb ? vq : OUTSIDE, step * 32);
+            if (wave < SW) load_lds4(sb, to + DENSE + CODES + wave * 256, step * 2 < nb ? vs : OUTSIDE, step * 2 / 4 * 4);
         }
         const bool in = step * 8 + piece < D.chunks;
 #pragma unroll
         for (int p = 0; p < PL; ++p)
 #pragma unroll
             for (int i = 0; i < LD; ++i)
-                load_lds16(db[p], lds + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
+                load_lds16(db[p], to + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
     };
-    auto put_scales = [&](uint8_t *lds) {
-        if constexpr (YT) {
-            constexpr int WR = BQ / 128;
-            if (tid < 64 * WR) {
-                uint16_t *s = (uint16_t *)(lds + DENSE + CODES) + (tid % WR) * 4 * 64 + tid / WR;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i * 64] = (uint16_t)(((sreg >> (8 * i)) & 255u) << 7);
-            }
-        }
-    };
-    // the loads have arrived (for YT the scales of the next step too), every wave is done with this step
-    auto next = [&](uint8_t *lds) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        put_scales(lds);
-        __syncthreads();
-    };
-
     v4f acc[FQ][FD];
 #pragma unroll
     for (int a = 0; a < FQ; ++a)
@@ -459,13 +572,13 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             if constexpr (YT) {
                 constexpr int ROW = BQ / 2;               // bytes of codes a row; rows 16 g + 8 t .. + 7 are in one piece
                 const uint8_t *cq = lds + (DENSE + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 64 + r16 * 4);
-                const uint8_t *sq = lds + (DENSE + CODES + (wq * 4 + (r16 >> 2)) * 128 + g * 32 + t * 16);
-                const v4u sc = *(const v4u *)sq;
+                const uint8_t *sq = lds + (DENSE + CODES + wq * 256 + (g * 16 + t * 8) * 4);   // words of the 8 rows
+                const v4u sc[2] = {*(const v4u *)sq, *(const v4u *)(sq + 16)};
                 v4u row[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const uint32_t half = (j & 1) ? sc[j >> 1] & 0xFFFF0000u : sc[j >> 1] << 16;
-                    row[j] = decode_bf16(*(const uint32_t *)(cq + j * ROW), __builtin_bit_cast(float, half));
+                    const uint32_t e = __builtin_amdgcn_ubfe(sc[j >> 2][j & 3], 8 * (r16 >> 2), 8) << 23;
+                    row[j] = decode_bf16(*(const uint32_t *)(cq + j * ROW), __builtin_bit_cast(float, e));
                 }
 #pragma unroll
                 for (int f = 0; f < FQ; ++f)
@@ -485,20 +598,20 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
                         acc[fq][fd] = QFIRST ? mfma_bf16(q[fq], d[p][fd], acc[fq][fd]) : mfma_bf16(d[p][fd], q[fq], acc[fq][fd]);
         }
     };
-    load(s0, lds0);
-    next(lds0);
-    int st = s0;
-    for (; st + 1 < s1; st += 2) {
-        load(st + 1, lds1);
+#pragma unroll
+    for (int i = 0; i < NS - 1; ++i) load(s0 + i, lds + i * STAGE);
+    int now = 0, next = (NS - 1) * STAGE;
+    constexpr int PER = LD * PL + 1;
+    for (int st = s0; st < s1; ++st) {
+        if (wave < SW) stage_ready<NS, PER + 1>();
+        else stage_ready<NS, PER>();
+        load(st + NS - 1, lds + next);
         __builtin_amdgcn_sched_barrier(0);
-        compute(st, lds0);
-        next(lds1);
-        load(st + 2, lds0);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(st + 1, lds1);
-        next(lds0);
+        compute(st, lds + now);
+        next = now;
+        now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
     }
-    if (st < s1) compute(st, lds0);
+    arrive();   // nothing is on its way to LDS any more
 
     // entry i of a lane's 4: QFIRST: 4-bit index 4 g + i, dense r16; otherwise the other way round
     const Out to = partial ? Out{partial + (int64_t)blockIdx.y * out.np * out.no, out.np, out.np, out.no, 1.f, 0.f, out.np % 4 == 0} : out;
@@ -904,27 +1017,41 @@ template <typename T> hipError_t launch_join(const float *partial, int slices, c
 // How a product of two 4-bit factors runs: tile 256 or 128, or 0 and the kernel for small ones
 struct BothPlan {
     int tile, nf, df;
-    int slices;
+    int slices, steps_z;   // of the contraction; steps of the tile kernel in each
     size_t partials, scales;
 };
 BothPlan both_plan(const Mx4Product &p) {
     BothPlan m{};
     auto tiles = [&](int64_t b) { return ((p.M + b - 1) / b) * ((p.N + b - 1) / b); };
     m.slices = 1;
-    m.scales = scales_work(p.XQ) + scales_work(p.Y);
-    m.tile = tiles(256) >= 256 ? 256 : tiles(128) >= 256 ? 128 : 0;
-    if (m.tile) return m;
     const int64_t small = p.M < p.N ? p.M : p.N, large = p.M < p.N ? p.N : p.M;
     auto groups = [&] { return ((large + 16 * m.nf - 1) / (16 * m.nf)) * ((small + 16 * m.df - 1) / (16 * m.df)); };
     m.df = small <= 16 ? 1 : small <= 32 ? 2 : 4;
     m.nf = 4;
-    while (groups() < 256 && m.nf > 1) {
-        m.nf /= 2;
-        if (m.df > 2) m.df = 2;
-        if (m.df == 2 && m.nf == 1) { m.nf = 2; break; }
+    // One workgroup a compute unit for the kernel for small products, whose workgroups read both factors
+    // from the L2 (2048 x 2048 x 2048, 1024 workgroups: 44 us, tiles of 128: 19 us; 256 x 4096 x 2048, 256 of
+    // them: 15 and 18 us). Of the tiles the larger ones where there is one for every compute unit (4096 x 4096
+    // x 8192: 72 and 86 us; 2048 x 4096 x 8192: 58 and 47 us).
+    if (tiles(256) >= 256) m.tile = 256;
+    else if (small > 32 && groups() > 256) m.tile = 128;
+    if (m.tile) {
+        const int64_t steps = (p.K + 255) / 256, t = tiles(m.tile);
+        int64_t z = 1;
+        while (t * z * 2 <= 512 && steps / (z * 2) >= 8) z *= 2;
+        m.steps_z = (int)((steps + z - 1) / z);
+        m.slices = (int)((steps + m.steps_z - 1) / m.steps_z);
+        m.scales = packed_scales(p.XQ) + packed_scales(p.Y);
+    } else {
+        while (groups() < 256 && m.nf > 1) {
+            m.nf /= 2;
+            if (m.df > 2) m.df = 2;
+            if (m.df == 2 && m.nf == 1) { m.nf = 2; break; }
+        }
+        const int64_t units = (p.K + 255) / 256;
+        while (groups() * m.slices < 256 && units / (m.slices * 2) >= 2 * ROWS_WAVES) m.slices *= 2;
+        m.scales = scales_work(p.XQ) + scales_work(p.Y);
     }
-    const int64_t units = (p.K + 255) / 256;
-    while (groups() * m.slices < 256 && units / (m.slices * 2) >= 2 * ROWS_WAVES) m.slices *= 2;
+    m.scales = round256(m.scales);
     if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
     return m;
 }
@@ -936,14 +1063,17 @@ template <int TYPE> hipError_t both_t(const Mx4Product &q, uint8_t *work, hipStr
     const bool xp = p.ci == 1;   // X's index is the contiguous one of C
     const int64_t ld = xp ? p.cj : p.ci;
     const Out out{p.C, ld, xp ? p.M : p.N, xp ? p.N : p.M, p.alpha, p.beta, (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
-    hipError_t e = align_scales(p.XQ, work, s);
-    if (e == hipSuccess) e = align_scales(p.Y, work, s);
-    if (e != hipSuccess) return e;
     if (m.tile) {
         // the factor whose rows are the contiguous index gives the operand whose 4 entries a lane holds
         const Mx4View &P = xp ? p.XQ : p.Y, &O = xp ? p.Y : p.XQ;
-        return m.tile == 256 ? launch_both_tile<T, 256, 256, 128, 64>(P, O, out, s) : launch_both_tile<T, 128, 128, 64, 64>(P, O, out, s);
+        float *partial = m.slices > 1 ? (float *)(work + m.scales) : nullptr;
+        const hipError_t e = m.tile == 256 ? launch_both_tile<T, 256, 256, 128, 64>(P, O, work, m.slices, m.steps_z, out, partial, s)
+                                           : launch_both_tile<T, 128, 128, 64, 64>(P, O, work, m.slices, m.steps_z, out, partial, s);
+        return e == hipSuccess && partial ? launch_join<T>(partial, m.slices, out, s) : e;
     }
+    hipError_t e = align_scales(p.XQ, work, s);
+    if (e == hipSuccess) e = align_scales(p.Y, work, s);
+    if (e != hipSuccess) return e;
     const bool xq = p.M >= p.N;   // the larger factor
     const Mx4View &Q = xq ? p.XQ : p.Y, &D = xq ? p.Y : p.XQ;
     float *partial = m.slices > 1 ? (float *)work : nullptr;
@@ -1009,7 +1139,7 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     return m;
 }
 
-template <typename T, bool YT, int BQ, int BD, int WQ, int WD>
+template <typename T, bool YT, int BQ, int BD, int WQ, int WD, int NS>
 hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, const MixedPlan &m, const Out &out, float *partial,
                              bool qfirst, hipStream_t s) {
     constexpr int PL = Planes<T>::N;
@@ -1017,9 +1147,9 @@ hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, cons
     const dim3 grid((unsigned)(((nq + BQ - 1) / BQ) * ((D.rows + BD - 1) / BD)), (unsigned)m.slices);
     constexpr int NT = (BQ / WQ) * (BD / WD) * 64;
     if (qfirst)
-        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, true>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, NS, true>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
     else
-        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, false>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, NS, false>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
     return hipGetLastError();
 }
 
@@ -1080,9 +1210,10 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     auto go = [&](auto yt) -> hipError_t {
         constexpr bool YT = decltype(yt)::value;
         if constexpr (Planes<T>::N == 1)
-            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, YT ? 128 : 64, YT ? 64 : 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        return launch_mixed_tile<T, YT, 128, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, YT ? 128 : 64, YT ? 64 : 128, 3>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        constexpr int NS = Planes<T>::N == 3 ? 2 : Planes<T>::N == 2 ? 3 : 4;   // what LDS holds
+        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, YT ? 128 : 64, YT ? 32 : 64, NS>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        return launch_mixed_tile<T, YT, 128, 128, YT ? 128 : 64, YT ? 32 : 64, NS>(D, p.Y, p.K, m, out, partial, qfirst, s);
     };
     e = p.yt ? go(std::true_type{}) : go(std::false_type{});
     if (e != hipSuccess || !partial) return e;
