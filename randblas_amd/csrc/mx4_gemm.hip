@@ -76,12 +76,6 @@ template <typename T> __device__ __forceinline__ void store4(const Out &o, int64
     }
 }
 
-// partial sums (f32) where there are any, the result otherwise
-template <typename T> __device__ __forceinline__ void put4(const Out &o, const float *partial, int64_t p, int64_t q, v4f v) {
-    if (partial) store4<float>(o, p, q, v);
-    else store4<T>(o, p, q, v);
-}
-
 // A range of memory for loads straight to LDS (16 bytes a lane, lane after lane from `lds`, which is the
 // same for the wave). An offset at or past the range's end reads zeros; `soffset` is added to the address
 // and does not count for that.
@@ -193,21 +187,21 @@ __device__ __forceinline__ Out partial_of(const Out &o, float *partial) {
 
 // A wave's WP x RO part of a result, RO rows of p after each other in LDS, to memory in whole lines: operands
 // hold 4 consecutive entries of many rows, and stores of those are 16 bytes to a line. `pitch` words a row.
-template <typename T, int WP, int RO>
-__device__ __forceinline__ void store_rows(const Out &o, const float *from, int pitch, int64_t p0, int64_t q0, int lane) {
-    typedef T t4 __attribute__((ext_vector_type(4)));
+template <typename T, int WP, int RO, typename Row>
+__device__ __forceinline__ void store_rows(const Out &o, const float *from, int pitch, int64_t p0, int64_t q0, Row row_of, int lane) {
     if (o.vec) {
-        constexpr int L = WP / 4, R = 64 / L;   // lanes a row, rows at once
-        static_assert(64 % L == 0 && RO % R == 0, "whole rows");
+        constexpr int L = WP / 4 < 64 ? WP / 4 : 64, R = 64 / L;   // lanes a row, rows at once
+        static_assert(WP % 4 == 0 && 64 % L == 0 && RO % R == 0 && WP <= 256, "whole rows");
 #pragma unroll 4
         for (int r = 0; r < RO; r += R) {
             const int row = r + lane / L, p = lane % L * 4;
-            store4<T>(o, p0 + p, q0 + row, *(const v4f *)(from + row * pitch + p));
+            store4<T>(o, p0 + p, q0 + row_of(row), *(const v4f *)(from + row * pitch + p));
         }
     } else {
         for (int r = 0; r < RO; ++r) {
-            if (q0 + r >= o.no) break;
-            T *c = (T *)o.ptr + (q0 + r) * o.ld + p0;
+            const int64_t q = q0 + row_of(r);
+            if (q >= o.no) break;
+            T *c = (T *)o.ptr + q * o.ld + p0;
 #pragma unroll
             for (int p = lane; p < WP; p += 64)
                 if (p0 + p < o.np) {
@@ -325,6 +319,7 @@ __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kerne
         now = STAGE - now;
     }
     float *rows = (float *)lds + wave * 32 * PITCH;   // this wave's
+    auto same = [](int r) { return r; };
 #pragma unroll
     for (int b = 0; b < FO; ++b) {
 #pragma unroll
@@ -334,8 +329,8 @@ __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kerne
                 *(v4f *)(rows + r32 * PITCH + a * 32 + 8 * i + 4 * g) =
                     v4f{acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
         __builtin_amdgcn_wave_barrier();
-        if (partial) store_rows<float, WP, 32>(partial_of(out, partial), rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, lane);
-        else store_rows<T, WP, 32>(out, rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, lane);
+        if (partial) store_rows<float, WP, 32>(partial_of(out, partial), rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, same, lane);
+        else store_rows<T, WP, 32>(out, rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, same, lane);
         __builtin_amdgcn_wave_barrier();
     }
 }
@@ -443,20 +438,8 @@ struct Dense16 {
     int chunks;
 };
 
-// The pipeline of the tile kernels: a ring of NS stages in LDS, loaded NS - 1 steps ahead. A step waits for its
-// own wave's loads of the stage, then at the barrier for the other waves', which also says that all are done
-// with the stage that the next loads overwrite. `per_step` loads a wave are issued a step, so those of the
-// stage have arrived when no more than (NS - 2) per_step are on their way; past the last step loads go on
-// (of nothing), to keep that count.
-template <int NS, int PER_STEP> __device__ __forceinline__ void stage_ready() {
-    wait_loads<(NS - 2) * PER_STEP>();
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_sched_barrier(0);
-}
-
 // BQ rows (YT: columns) of the 4-bit factor x BD rows of the dense one a workgroup, WQ x WD a wave; 64
-// elements of the contraction a step.
+// elements of the contraction a step, loaded straight to LDS, double-buffered.
 //
 // A step's two matrix instructions take their 32 elements from all over the 64: lane group g holds
 // elements 16 g + 8 t .. + 7 of both factors for instruction t, so a lane's 16 codes lie in one word pair
@@ -466,8 +449,8 @@ template <int NS, int PER_STEP> __device__ __forceinline__ void stage_ready() {
 //   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes a word (8 columns 8 c .. +
 //     7) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 8
 //     operands are then columns 8 c + f, and the operand f of the wave is columns f, f + 8, .. -- an order of
-//     the result's rows or columns that the stores undo. Scales: word w of the rows after each other.
-template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, int NS, bool QFIRST>
+//     the result's rows or columns that the stores undo. Scales are kept as the upper halves of floats.
+template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
     constexpr int NW = (BQ / WQ) * (BD / WD), NT = NW * 64;
@@ -479,10 +462,13 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     constexpr int DENSE = PL * BD * 128;
     constexpr int PITCH = YT ? (BQ == 256 ? 1056 : 1088) : 1024;   // 64 lanes' codes; lane groups on different banks
     constexpr int CODES = NW * PITCH;
-    constexpr int SW = YT ? BQ / 128 : BQ / 64;               // waves that load scales, 64 words each
-    constexpr int STAGE = DENSE + CODES + SW * 256;
-    static_assert(NS * STAGE <= 160 * 1024, "LDS");
-    __shared__ __attribute__((aligned(16))) uint8_t lds[NS * STAGE];
+    constexpr int SCALES = YT ? BQ / 32 * 128 : BQ * 4;
+    constexpr int STAGE = DENSE + CODES + SCALES;
+    constexpr int W1 = QFIRST ? WQ : WD, PITCH1 = W1 + 4;
+    constexpr int LDS = 2 * STAGE > NW * 16 * PITCH1 * 4 ? 2 * STAGE : NW * 16 * PITCH1 * 4;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    uint8_t *const lds0 = lds, *const lds1 = lds + STAGE;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const int64_t nq = YT ? Y.cols : Y.rows;
@@ -515,7 +501,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
         vq = (uint32_t)((wave * 32 + (lane >> 1)) * Y.ldq) + qpart * 16;
         vs = (uint32_t)((wave * 64 + lane) * Y.lds);
     }
-    auto load = [&](int step, uint8_t *to) {
+    uint32_t sreg = 0;   // YT: 4 scales of a row on their way to LDS
+    auto load = [&](int step, uint8_t *lds) {
         if constexpr (YT) {
             const int64_t k0 = (int64_t)step * 64;
             const int64_t left = K - k0 < 64 ? K - k0 : 64;
@@ -524,19 +511,40 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             // past the last step the range is empty, and reads zeros
             const Buffer cb = buffer(Y.codes + q0 / 2 + (have ? k0 : 0) * Y.ldq, have * ((rows - 1) * (uint32_t)Y.ldq + nb * 16));
             const Buffer kb = buffer(Y.scales + q0 / 32 + (have ? k0 : 0) * Y.lds, have * ((rows - 1) * (uint32_t)Y.lds + (nb + 3) / 4 * 4));
-            load_lds16(cb, to + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
-            if (wave < SW) load_lds4(kb, to + DENSE + CODES + wave * 256, wave * 4 < nb ? (uint32_t)(lane * Y.lds) + wave * 4 : OUTSIDE, 0);
+            constexpr int WR = BQ / 128;                  // words of scales a row
+            if (tid < 64 * WR) {
+                const int w = tid % WR;
+                sreg = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, w * 4 < nb ? (int)((tid / WR) * Y.lds + w * 4) : (int)OUTSIDE, 0, 0);
+            }
+            load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
         } else {
-            load_lds16(qb, to + DENSE + wave * PITCH, step * 2 + qpart < nb ? vq : OUTSIDE, step * 32);
-            if (wave < SW) load_lds4(sb, to + DENSE + CODES + wave * 256, step * 2 < nb ? vs : OUTSIDE, step * 2 / 4 * 4);
+            load_lds16(qb, lds + DENSE + wave * PITCH, step * 2 + qpart < nb ? vq : OUTSIDE, step * 32);
+            if (wave < BQ / 64) load_lds4(sb, lds + DENSE + CODES + wave * 256, step * 2 < nb ? vs : OUTSIDE, step * 2 / 4 * 4);
         }
         const bool in = step * 8 + piece < D.chunks;
 #pragma unroll
         for (int p = 0; p < PL; ++p)
 #pragma unroll
             for (int i = 0; i < LD; ++i)
-                load_lds16(db[p], to + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
+                load_lds16(db[p], lds + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
     };
+    auto put_scales = [&](uint8_t *lds) {
+        if constexpr (YT) {
+            constexpr int WR = BQ / 128;
+            if (tid < 64 * WR) {
+                uint16_t *s = (uint16_t *)(lds + DENSE + CODES) + (tid % WR) * 4 * 64 + tid / WR;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[i * 64] = (uint16_t)(((sreg >> (8 * i)) & 255u) << 7);
+            }
+        }
+    };
+    // the loads have arrived (for YT the scales of the next step too), every wave is done with this step
+    auto next = [&](uint8_t *lds) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        put_scales(lds);
+        __syncthreads();
+    };
+
     v4f acc[FQ][FD];
 #pragma unroll
     for (int a = 0; a < FQ; ++a)
@@ -572,13 +580,13 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             if constexpr (YT) {
                 constexpr int ROW = BQ / 2;               // bytes of codes a row; rows 16 g + 8 t .. + 7 are in one piece
                 const uint8_t *cq = lds + (DENSE + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 64 + r16 * 4);
-                const uint8_t *sq = lds + (DENSE + CODES + wq * 256 + (g * 16 + t * 8) * 4);   // words of the 8 rows
-                const v4u sc[2] = {*(const v4u *)sq, *(const v4u *)(sq + 16)};
+                const uint8_t *sq = lds + (DENSE + CODES + (wq * 4 + (r16 >> 2)) * 128 + g * 32 + t * 16);
+                const v4u sc = *(const v4u *)sq;
                 v4u row[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const uint32_t e = __builtin_amdgcn_ubfe(sc[j >> 2][j & 3], 8 * (r16 >> 2), 8) << 23;
-                    row[j] = decode_bf16(*(const uint32_t *)(cq + j * ROW), __builtin_bit_cast(float, e));
+                    const uint32_t half = (j & 1) ? sc[j >> 1] & 0xFFFF0000u : sc[j >> 1] << 16;
+                    row[j] = decode_bf16(*(const uint32_t *)(cq + j * ROW), __builtin_bit_cast(float, half));
                 }
 #pragma unroll
                 for (int f = 0; f < FQ; ++f)
@@ -598,46 +606,57 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
                         acc[fq][fd] = QFIRST ? mfma_bf16(q[fq], d[p][fd], acc[fq][fd]) : mfma_bf16(d[p][fd], q[fq], acc[fq][fd]);
         }
     };
-#pragma unroll
-    for (int i = 0; i < NS - 1; ++i) load(s0 + i, lds + i * STAGE);
-    int now = 0, next = (NS - 1) * STAGE;
-    constexpr int PER = LD * PL + 1;
-    for (int st = s0; st < s1; ++st) {
-        if (wave < SW) stage_ready<NS, PER + 1>();
-        else stage_ready<NS, PER>();
-        load(st + NS - 1, lds + next);
+    load(s0, lds0);
+    next(lds0);
+    int st = s0;
+    for (; st + 1 < s1; st += 2) {
+        load(st + 1, lds1);
         __builtin_amdgcn_sched_barrier(0);
-        compute(st, lds + now);
-        next = now;
-        now = now + STAGE == NS * STAGE ? 0 : now + STAGE;
+        compute(st, lds0);
+        next(lds1);
+        load(st + 2, lds0);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(st + 1, lds1);
+        next(lds0);
     }
-    arrive();   // nothing is on its way to LDS any more
+    if (st < s1) compute(st, lds0);
 
-    // entry i of a lane's 4: QFIRST: 4-bit index 4 g + i, dense r16; otherwise the other way round
-    const Out to = partial ? Out{partial + (int64_t)blockIdx.y * out.np * out.no, out.np, out.np, out.no, 1.f, 0.f, out.np % 4 == 0} : out;
+    __syncthreads();
+    // to memory by way of LDS, 16 rows of the second index at a time. Entry i of a lane's 4 is row 4 g + i of
+    // the first operand; YT: the 4-bit index of row r of operand f is 8 r + f
+    const int64_t n1 = QFIRST ? q0 + wq * WQ : d0 + wd * WD;
+    float *rows = (float *)lds + wave * 16 * PITCH1;   // this wave's
+    auto out_rows = [&](int64_t n2, auto row) {
+        __builtin_amdgcn_wave_barrier();
+        if (partial) store_rows<float, W1, 16>(partial_of(out, partial), rows, PITCH1, n1, n2, row, lane);
+        else store_rows<T, W1, 16>(out, rows, PITCH1, n1, n2, row, lane);
+        __builtin_amdgcn_wave_barrier();
+    };
+    if constexpr (QFIRST) {
 #pragma unroll
-    for (int fd = 0; fd < FD; ++fd)
+        for (int fd = 0; fd < FD; ++fd) {
+            float *to = rows + r16 * PITCH1;
+            if constexpr (!YT) {
+#pragma unroll
+                for (int fq = 0; fq < FQ; ++fq) *(v4f *)(to + fq * 16 + 4 * g) = acc[fq][fd];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h)
+                        *(v4f *)(to + (4 * g + i) * 8 + 4 * h) =
+                            v4f{acc[4 * h][fd][i], acc[4 * h + 1][fd][i], acc[4 * h + 2][fd][i], acc[4 * h + 3][fd][i]};
+            }
+            out_rows(d0 + wd * WD + fd * 16, [](int r) { return r; });
+        }
+    } else {
 #pragma unroll
         for (int fq = 0; fq < FQ; ++fq) {
-            const int64_t dd = d0 + wd * WD + fd * 16;
-            if constexpr (!YT) {
-                const int64_t qq = q0 + wq * WQ + fq * 16;
-                if constexpr (QFIRST) put4<T>(to, partial, qq + 4 * g, dd + r16, acc[fq][fd]);
-                else put4<T>(to, partial, dd + 4 * g, qq + r16, acc[fq][fd]);
-            } else if constexpr (!QFIRST) {
-                put4<T>(to, partial, dd + 4 * g, q0 + wq * WQ + r16 * 8 + fq, acc[fq][fd]);
-            }
+#pragma unroll
+            for (int fd = 0; fd < FD; ++fd) *(v4f *)(rows + r16 * PITCH1 + fd * 16 + 4 * g) = acc[fq][fd];
+            if constexpr (YT) out_rows(q0 + wq * WQ + fq, [](int r) { return 8 * r; });
+            else out_rows(q0 + wq * WQ + fq * 16, [](int r) { return r; });
         }
-    if constexpr (YT && QFIRST) {   // columns 8 (4 g + i) + fq: 8 operands make 8 consecutive ones
-#pragma unroll
-        for (int fd = 0; fd < FD; ++fd)
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const v4f v{acc[4 * h][fd][i], acc[4 * h + 1][fd][i], acc[4 * h + 2][fd][i], acc[4 * h + 3][fd][i]};
-                    put4<T>(to, partial, q0 + wq * WQ + (4 * g + i) * 8 + 4 * h, d0 + wd * WD + fd * 16 + r16, v);
-                }
     }
 }
 
@@ -1139,7 +1158,7 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     return m;
 }
 
-template <typename T, bool YT, int BQ, int BD, int WQ, int WD, int NS>
+template <typename T, bool YT, int BQ, int BD, int WQ, int WD>
 hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, const MixedPlan &m, const Out &out, float *partial,
                              bool qfirst, hipStream_t s) {
     constexpr int PL = Planes<T>::N;
@@ -1147,9 +1166,9 @@ hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, cons
     const dim3 grid((unsigned)(((nq + BQ - 1) / BQ) * ((D.rows + BD - 1) / BD)), (unsigned)m.slices);
     constexpr int NT = (BQ / WQ) * (BD / WD) * 64;
     if (qfirst)
-        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, NS, true>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, true>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
     else
-        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, NS, false>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, false>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
     return hipGetLastError();
 }
 
@@ -1210,10 +1229,9 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     auto go = [&](auto yt) -> hipError_t {
         constexpr bool YT = decltype(yt)::value;
         if constexpr (Planes<T>::N == 1)
-            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, YT ? 128 : 64, YT ? 64 : 128, 3>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        constexpr int NS = Planes<T>::N == 3 ? 2 : Planes<T>::N == 2 ? 3 : 4;   // what LDS holds
-        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, YT ? 128 : 64, YT ? 32 : 64, NS>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        return launch_mixed_tile<T, YT, 128, 128, YT ? 128 : 64, YT ? 32 : 64, NS>(D, p.Y, p.K, m, out, partial, qfirst, s);
+            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, YT ? 128 : 64, YT ? 64 : 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        return launch_mixed_tile<T, YT, 128, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
     };
     e = p.yt ? go(std::true_type{}) : go(std::false_type{});
     if (e != hipSuccess || !partial) return e;
