@@ -445,7 +445,9 @@ struct Dense16 {
 // elements 16 g + 8 t .. + 7 of both factors for instruction t, so a lane's 16 codes lie in one word pair
 // and under one scale.
 //   dense: rows of 128 bytes, 16-byte pieces at place piece ^ (row / 2 & 7), a plane after the other
-//   codes, blocks along the contraction: rows of 32 bytes, halves exchanged in 8 of 16 rows; scales: words
+//   codes, blocks along the contraction: SS steps at once, 256 elements, so that rows are whole lines of 128 bytes
+//     (128 where LDS is short), the next ones a part of the rows a step; 16-byte blocks kept like the dense
+//     pieces, the rows' scales behind them
 //   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes a word (8 columns 8 c .. +
 //     7) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 8
 //     operands are then columns 8 c + f, and the operand f of the wave is columns f, f + 8, .. -- an order of
@@ -461,14 +463,16 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     static_assert(!YT || WQ == 128, "8 columns a lane");
     constexpr int DENSE = PL * BD * 128;
     constexpr int PITCH = YT ? (BQ == 256 ? 1056 : 1088) : 1024;   // 64 lanes' codes; lane groups on different banks
-    constexpr int CODES = NW * PITCH;
-    constexpr int SCALES = YT ? BQ / 32 * 128 : BQ * 4;
+    constexpr int CODES = YT ? NW * PITCH : 0;
+    constexpr int SCALES = YT ? BQ / 32 * 128 : 0;
     constexpr int STAGE = DENSE + CODES + SCALES;
+    // blocks along: codes and scales of SS steps at a time
+    constexpr int SS = 2 * (STAGE + BQ * 136) > 160 * 1024 ? 2 : 4, NP = 2 * SS, SUPER = YT ? 0 : BQ * 34 * SS;
     constexpr int W1 = QFIRST ? WQ : WD, PITCH1 = W1 + 4;
-    constexpr int LDS = 2 * STAGE > NW * 16 * PITCH1 * 4 ? 2 * STAGE : NW * 16 * PITCH1 * 4;
+    constexpr int RING = 2 * (STAGE + SUPER), LDS = RING > NW * 16 * PITCH1 * 4 ? RING : NW * 16 * PITCH1 * 4;
     static_assert(LDS <= 160 * 1024, "LDS");
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
-    uint8_t *const lds0 = lds, *const lds1 = lds + STAGE;
+    uint8_t *const lds0 = lds, *const lds1 = lds + STAGE, *const supers = lds + 2 * STAGE;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
     const int64_t nq = YT ? Y.cols : Y.rows;
@@ -497,10 +501,18 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     } else {
         qb = buffer(Y.codes + q0 * Y.ldq, (uint32_t)((mq - 1) * Y.ldq + nb * 16));
         sb = buffer(Y.scales + q0 * Y.lds, (uint32_t)((mq - 1) * Y.lds + (nb + 3) / 4 * 4));
-        qpart = (lane & 1) ^ ((lane >> 4) & 1);           // rows 8-15 of 16: halves exchanged
-        vq = (uint32_t)((wave * 32 + (lane >> 1)) * Y.ldq) + qpart * 16;
-        vs = (uint32_t)((wave * 64 + lane) * Y.lds);
+        qpart = (tid % NP) ^ ((tid >> 4) % NP);
+        vq = (uint32_t)((tid / NP) * Y.ldq) + qpart * 16;
+        vs = (uint32_t)((tid / (SS / 2)) * Y.lds) + tid % (SS / 2) * 4;
     }
+    // blocks along: part c (of the rows) of codes and scales u
+    auto load_super = [&](int u, int c) {
+        uint8_t *to = supers + (u & 1) * SUPER;
+        load_lds16(qb, to + (c * NT + wave * 64) * 16, u * NP + qpart < nb ? vq + (uint32_t)(c * (BQ / SS) * Y.ldq) : OUTSIDE, u * NP * 16);
+        if (wave < BQ / 128)
+            load_lds4(sb, to + BQ * 32 * SS + (c * (BQ / 2) + wave * 64) * 4,
+                      u * NP + tid % (SS / 2) * 4 < nb ? vs + (uint32_t)(c * (BQ / SS) * Y.lds) : OUTSIDE, u * NP);
+    };
     uint32_t sreg = 0;   // YT: 4 scales of a row on their way to LDS
     auto load = [&](int step, uint8_t *lds) {
         if constexpr (YT) {
@@ -517,9 +529,6 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
                 sreg = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, w * 4 < nb ? (int)((tid / WR) * Y.lds + w * 4) : (int)OUTSIDE, 0, 0);
             }
             load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
-        } else {
-            load_lds16(qb, lds + DENSE + wave * PITCH, step * 2 + qpart < nb ? vq : OUTSIDE, step * 32);
-            if (wave < BQ / 64) load_lds4(sb, lds + DENSE + CODES + wave * 256, step * 2 < nb ? vs : OUTSIDE, step * 2 / 4 * 4);
         }
         const bool in = step * 8 + piece < D.chunks;
 #pragma unroll
@@ -558,14 +567,16 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
         v2u raw[YT ? 1 : FQ];
         float scale[YT ? 1 : FQ];
         if constexpr (!YT) {
-            const uint8_t *cq = lds + (DENSE + (wq * WQ + r16) * 32 + ((g * 8) ^ ((r16 >> 3) * 16)));
-            const uint8_t *sq = lds + (DENSE + CODES + (wq * WQ + r16) * 4);
-            const int bit = (step & 1) * 16 + (g >> 1) * 8;
+            const int c = step % SS;
+            const uint8_t *super = supers + (step / SS & 1) * SUPER;
+            const uint8_t *cq = super + ((wq * WQ + r16) * 32 * SS + (((c * 2 + (g >> 1)) ^ ((r16 * NP >> 4) % NP)) * 16) + (g & 1) * 8);
+            const uint8_t *sq = super + (BQ * 32 * SS + (wq * WQ + r16) * 2 * SS + (c >> 1) * 4);
+            const int bit = (c & 1) * 16 + (g >> 1) * 8;
             const uint32_t width = step * 2 + (g >> 1) < nb ? 8 : 0;   // past the last block, whatever is there, as 0
 #pragma unroll
             for (int f = 0; f < FQ; ++f) {
-                raw[f] = *(const v2u *)(cq + f * 16 * 32);
-                scale[f] = __builtin_bit_cast(float, __builtin_amdgcn_ubfe(*(const uint32_t *)(sq + f * 16 * 4), bit, width) << 23);
+                raw[f] = *(const v2u *)(cq + f * 16 * 32 * SS);
+                scale[f] = __builtin_bit_cast(float, __builtin_amdgcn_ubfe(*(const uint32_t *)(sq + f * 16 * 2 * SS), bit, width) << 23);
             }
         }
 #pragma unroll
@@ -606,14 +617,19 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
                         acc[fq][fd] = QFIRST ? mfma_bf16(q[fq], d[p][fd], acc[fq][fd]) : mfma_bf16(d[p][fd], q[fq], acc[fq][fd]);
         }
     };
+    if constexpr (!YT)   // slices start at multiples of 4 steps
+#pragma unroll
+        for (int c = 0; c < SS; ++c) load_super(s0 / SS, c);
     load(s0, lds0);
     next(lds0);
     int st = s0;
     for (; st + 1 < s1; st += 2) {
+        if constexpr (!YT) load_super(st / SS + 1, st % SS);
         load(st + 1, lds1);
         __builtin_amdgcn_sched_barrier(0);
         compute(st, lds0);
         next(lds1);
+        if constexpr (!YT) load_super((st + 1) / SS + 1, (st + 1) % SS);
         load(st + 2, lds0);
         __builtin_amdgcn_sched_barrier(0);
         compute(st + 1, lds1);
@@ -1152,7 +1168,7 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     const int64_t steps = (p.K + 63) / 64, t = tiles(m.bq, m.bd);
     int64_t z = 1;
     while (t * z * 2 <= 256 && steps / (z * 2) >= 8) z *= 2;
-    m.steps_z = (int)((steps + z - 1) / z);
+    m.steps_z = (int)((steps + z - 1) / z + 3) / 4 * 4;   // codes come by 4 steps
     m.slices = (int)((steps + m.steps_z - 1) / m.steps_z);
     if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
     return m;
