@@ -12,9 +12,13 @@
 // Both kernels move each byte once and are bound by HBM. Two forms, by which direction is contiguous:
 //   rows: blocks lie along memory. Four lanes share a block (8 elements each, 16-64 bytes of load and
 //         4 bytes of codes a lane, both contiguous over the wave); the block's maximum crosses the four
-//         lanes in two quad permutes.
+//         lanes in two quad permutes. Accesses are as wide where a row starts at an odd multiple of an element
+//         (4096 x 5731 bf16 back to elements: single elements stored, four a lane, 35 us, this 24 us).
 //   cols: blocks lie across memory. A lane owns a row's block: 32 loads, each contiguous over the 64
 //         lanes, the maximum in registers, 16 bytes of codes a lane.
+// Quantising and dequantising, two launches: 8192 x 16384 f32 248 us (4.6 TB/s; a copy runs at 4.9), 8192 x 8192
+// bf16 61 us, stochastic 93 us (bound by the generator's integer multiplications), 1024 x 16384 f32 across
+// memory 29 us.
 #include "common.hpp"
 #include "mx4.hpp"
 
@@ -106,7 +110,8 @@ __device__ __forceinline__ uint32_t encode8(const V *x, int e, const Mx4Random &
         for (int h = 0; h < 2; ++h) {
             uint32_t ctr[4];
             rb::ctr_add(rnd.ctr, (uint64_t)r * rnd.quads + (uint64_t)(c >> 2) + (uint64_t)h, ctr);
-            const rb::u32x4 w = rb::cbrng(rnd.rng, ctr, rnd.key);
+            const rb::u32x4 w = rnd.rng == rb::RNG_PHILOX ? rb::philox4x32_uk(ctr[0], ctr[1], ctr[2], ctr[3], rnd.key[0], rnd.key[1])
+                                                          : rb::cbrng(rnd.rng, ctr, rnd.key);
 #pragma unroll
             for (int i = 0; i < 4; ++i) v[4 * h + i] = stochastic(x[4 * h + i] * inv, w.v[i]);
         }
@@ -135,7 +140,7 @@ __device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv &f) {
 template <int TYPE, bool SR>
 __global__ __launch_bounds__(MXT) void quantize_rows_kernel(const typename Elem<TYPE>::mem *__restrict__ A, int64_t ld,
                                                              Mx4View Q, FastDiv nb, uint32_t units, int64_t row0,
-                                                             bool vec, Mx4Random rnd) {
+                                                             Mx4Random rnd) {
     typedef typename Elem<TYPE>::mem M;
     typedef typename Elem<TYPE>::val V;
     typedef M m8_t __attribute__((ext_vector_type(8)));
@@ -146,9 +151,9 @@ __global__ __launch_bounds__(MXT) void quantize_rows_kernel(const typename Elem<
     const int64_t r = row0 + rr, c = (int64_t)b * MX4_BLOCK + 8 * q;
     const M *p = A + r * ld + c;
     V x[8];
-    if (vec && c + 8 <= Q.cols) {
+    if (c + 8 <= Q.cols) {
         m8_t m;
-        __builtin_memcpy(&m, __builtin_assume_aligned(p, 16), sizeof m);
+        __builtin_memcpy(&m, p, sizeof m);   // at any multiple of an element one or a few wide loads
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (V)m[i];
     } else {
@@ -240,25 +245,12 @@ __global__ __launch_bounds__(MXT) void dequantize_rows_kernel(Mx4View Q, typenam
         m8_t m;
 #pragma unroll
         for (int i = 0; i < 8; ++i) m[i] = o[i];
-        __builtin_memcpy(__builtin_assume_aligned(p, 16), &m, sizeof m);
+        __builtin_memcpy(p, &m, sizeof m);   // wide at any multiple of an element, as the loads above
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
             if (c + i < Q.cols) p[i] = o[i];
     }
-}
-
-// Rows that are not at multiples of 16 bytes: a lane an element, so that a wave's stores are contiguous all the
-// same (8 elements a lane at 8 bytes each took 18.5 us for 2999 x 1013 doubles, this UNALIGNED_US)
-template <int TYPE>
-__global__ __launch_bounds__(MXT) void dequantize_elements_kernel(Mx4View Q, typename Elem<TYPE>::mem *__restrict__ A, int64_t ld) {
-    typedef typename Elem<TYPE>::mem M;
-    for (int64_t r = blockIdx.y; r < Q.rows; r += gridDim.y)
-        for (int64_t c = (int64_t)blockIdx.x * MXT + threadIdx.x; c < Q.cols; c += (int64_t)gridDim.x * MXT) {
-            M o[8];
-            decode8<TYPE>(Q.codes[r * Q.ldq + (c >> 1)], scale_f32(Q.scales[r * Q.lds + (c >> 5)]), o);
-            A[r * ld + c] = c & 1 ? o[1] : o[0];
-        }
 }
 
 template <int TYPE>
@@ -304,11 +296,10 @@ hipError_t quantize_t(const Mx4Dense &A, const Mx4View &Q, const Mx4Random &rnd,
     const M *a = (const M *)A.ptr;
     const int64_t nb = mx4_blocks(Q.cols);
     if (A.sc == 1) {
-        const bool vec = (uintptr_t)a % 16 == 0 && (A.sr * sizeof(M)) % 16 == 0;
         return row_chunks(Q.rows, nb * 4, [&](int64_t r0, int64_t rows) {
             const uint32_t units = (uint32_t)(rows * nb * 4);
             hipLaunchKernelGGL((quantize_rows_kernel<TYPE, SR>), dim3((units + MXT - 1) / MXT), dim3(MXT), 0, s, a,
-                               A.sr, Q, fast_div((uint32_t)nb), units, r0, vec, rnd);
+                               A.sr, Q, fast_div((uint32_t)nb), units, r0, rnd);
             return hipGetLastError();
         });
     }
@@ -323,12 +314,6 @@ template <int TYPE> hipError_t dequantize_t(const Mx4View &Q, const Mx4Dense &A,
     M *a = (M *)const_cast<void *>(A.ptr);
     const int64_t nb = mx4_blocks(Q.cols);
     if (A.sc == 1) {
-        if ((uintptr_t)a % 16 != 0 || (A.sr * sizeof(M)) % 16 != 0) {
-            const int64_t x = (Q.cols + MXT - 1) / MXT;
-            hipLaunchKernelGGL((dequantize_elements_kernel<TYPE>), dim3((unsigned)(x < 65536 ? x : 65536), (unsigned)(Q.rows < 65535 ? Q.rows : 65535)),
-                               dim3(MXT), 0, s, Q, a, A.sr);
-            return hipGetLastError();
-        }
         return row_chunks(Q.rows, nb * 4, [&](int64_t r0, int64_t rows) {
             const uint32_t units = (uint32_t)(rows * nb * 4);
             hipLaunchKernelGGL((dequantize_rows_kernel<TYPE>), dim3((units + MXT - 1) / MXT), dim3(MXT), 0, s, Q, a, A.sr,

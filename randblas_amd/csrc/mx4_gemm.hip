@@ -779,10 +779,10 @@ __global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, 
     v4f acc[NF * DF];
 #pragma unroll
     for (int i = 0; i < NF * DF; ++i) acc[i] = v4f{0.f, 0.f, 0.f, 0.f};
-    const int rows = (int)D.rows;
+    const int64_t d0 = (int64_t)blockIdx.z * (16 * DF), rows = D.rows - d0 < 16 * DF ? D.rows - d0 : 16 * DF;
     Buffer db[PL];
 #pragma unroll
-    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane, (uint32_t)((rows - 1) * D.ld * 2 + D.chunks * 16));
+    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane + d0 * D.ld, (uint32_t)((rows - 1) * D.ld * 2 + D.chunks * 16));
     // one load: 4 rows, lane l places l & 15 of row l / 16 of them; rows that are not there are zeros
     auto load_dense = [&](int hu, uint8_t *lds) {       // half unit hu
 #pragma unroll
@@ -844,7 +844,7 @@ __global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, 
     arrive();   // nothing is on its way to LDS any more
     add_waves<W, NF * DF>(acc, (v4f *)half0, lane, wave, [&](int i, int l, v4f v) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (i / DF) * 16 + 4 * (l >> 4) + j, (i % DF) * 16 + (l & 15), v[j]);
+        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (i / DF) * 16 + 4 * (l >> 4) + j, d0 + (i % DF) * 16 + (l & 15), v[j]);
     });
 }
 
@@ -909,9 +909,10 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
     // a wave's scales of a unit, by block and row, as upper halves of floats: 8 blocks x 32 rows (in the place
     // of its sums, which come after the last unit)
     uint16_t *scales = (uint16_t *)&sums[wave * 8 * 64];
+    const int64_t d0 = (int64_t)blockIdx.z * (16 * DF), rows = D.rows - d0 < 16 * DF ? D.rows - d0 : 16 * DF;
     Buffer db[PL];
 #pragma unroll
-    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane, (uint32_t)((D.rows - 1) * D.ld * 2 + D.chunks * 16));
+    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane + d0 * D.ld, (uint32_t)((rows - 1) * D.ld * 2 + D.chunks * 16));
     auto dense = [&](int piece, v4u (&d)[DF][PL]) {
 #pragma unroll
         for (int e = 0; e < DF; ++e)
@@ -982,7 +983,7 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
     }
     add_waves<ROWS_WAVES, 16 * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (4 * (l >> 4) + j) * 16 + i / DF, (i % DF) * 16 + (l & 15), v[j]);
+        for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (4 * (l >> 4) + j) * 16 + i / DF, d0 + (i % DF) * 16 + (l & 15), v[j]);
     });
 }
 
@@ -1145,15 +1146,21 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     m.scales = scales_work(p.Y);
     m.ld = (p.K + 63) / 64 * 64;
     if (!m.direct) m.planes = round256((size_t)pl * p.M * m.ld * 2);
-    if (p.M <= (pl == 3 ? 16 : 32)) {   // 3 planes of 32 rows: more than LDS, or with blocks across the registers, hold
-        m.rows = p.M <= 16 ? 1 : 2;
-        // Columns a workgroup: each reads the dense rows whole, so enough that those are fewer bytes than its
-        // codes, and more where that still makes a workgroup for every compute unit. The contraction is cut
-        // until there are 256 workgroups.
-        m.bq = p.yt ? 256 : 16;
+    // The kernel for few rows, 16 or 32 of them (3 planes of 32: more than LDS, or with blocks across the
+    // registers, hold) and 16 to 64 columns (256) a workgroup. Columns: each workgroup reads its dense rows whole, so
+    // enough that those are fewer bytes than its codes, and more where that still makes a workgroup for every
+    // compute unit. The contraction is cut until there are 256 workgroups. More rows too where that makes
+    // no more than a workgroup for each compute unit (64 x 8192 x 4096 bf16 16.5 us, in tiles 20.6; 88 x 59 x 812
+    // f32 14.5 and 27.8), except for one or two planes with blocks across (64 x 4096 x 4096 25.0 and 19.9).
+    const int df = p.M <= 16 || pl == 3 ? 1 : 2;
+    const int64_t dgroups = (p.M + 16 * df - 1) / (16 * df);
+    const int64_t widest = p.yt ? 256 : 64;
+    if (p.M <= 16 * df || ((!p.yt || pl == 3) && (p.N + widest - 1) / widest * dgroups <= 256)) {
+        m.rows = df;
+        m.bq = (int)widest;
         if (!p.yt)
-            while (m.bq < 64 && (m.bq < 4 * pl * p.M || p.N >= 512 * m.bq)) m.bq *= 2;
-        const int64_t groups = (p.N + m.bq - 1) / m.bq, units = p.yt ? (p.K + 31) / 32 : (p.K + 255) / 256;
+            for (m.bq = 16; m.bq < 64 && (m.bq < 4 * pl * (p.M < 16 * df ? p.M : 16 * df) || p.N * dgroups >= 512 * m.bq);) m.bq *= 2;
+        const int64_t groups = (p.N + m.bq - 1) / m.bq * dgroups, units = p.yt ? (p.K + 31) / 32 : (p.K + 255) / 256;
         m.slices = 1;
         while (groups * m.slices < 256 && units / (m.slices * 2) >= (p.yt ? 2 * ROWS_WAVES : dense_waves(pl * m.rows))) m.slices *= 2;
         if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
@@ -1166,8 +1173,9 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     if (pl == 1 && tiles(256, 256) >= 256) m.bd = 256;
     else if (tiles(256, 128) < 256) m.bq = 128;
     const int64_t steps = (p.K + 63) / 64, t = tiles(m.bq, m.bd);
+    // one plane: two tiles of 128 x 128 fit a compute unit (533 x 4231 x 5056: cut to 512 workgroups 51.5 us, to 256 59.0)
     int64_t z = 1;
-    while (t * z * 2 <= 256 && steps / (z * 2) >= 8) z *= 2;
+    while (t * z * 2 <= (pl == 1 && m.bq == 128 ? 512 : 256) && steps / (z * 2) >= 8) z *= 2;
     m.steps_z = (int)((steps + z - 1) / z + 3) / 4 * 4;   // codes come by 4 steps
     m.slices = (int)((steps + m.steps_z - 1) / m.steps_z);
     if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);
@@ -1191,7 +1199,7 @@ hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, cons
 template <typename T> hipError_t launch_mixed_rows(const Dense16 &D, const Mx4Product &p, const MixedPlan &m, const Out &final, bool qfirst, float *partial, hipStream_t s) {
     RowsOut out{p.C, p.cj, p.ci, p.N, p.M, p.alpha, p.beta, partial};
     if (partial) out.sq = qfirst ? 1 : p.M, out.sd = qfirst ? p.N : 1;
-    const dim3 grid((unsigned)((p.N + m.bq - 1) / m.bq), (unsigned)m.slices), block((p.yt ? ROWS_WAVES : dense_waves(Planes<T>::N * m.rows)) * 64);
+    const dim3 grid((unsigned)((p.N + m.bq - 1) / m.bq), (unsigned)m.slices, (unsigned)((p.M + 16 * m.rows - 1) / (16 * m.rows))), block((p.yt ? ROWS_WAVES : dense_waves(Planes<T>::N * m.rows)) * 64);
     auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, D, p.Y, out); };
     if (p.yt) {
         if (m.rows == 1) hipLaunchKernelGGL((mixed_rows_yt_kernel<T, 1>), grid, block, 0, s, D, p.Y, (int)p.K, out);
