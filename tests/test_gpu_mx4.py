@@ -154,6 +154,24 @@ def test_dequantize(cuda, rows, cols, ro, co, pad, t, layout, op):
     assert torch.all(padding == 7.0)
 
 
+@pytest.mark.parametrize("offset,pad", [(1, 0), (3, 5), (8, 8)])
+@pytest.mark.parametrize("layout", ["R", "C"])
+@pytest.mark.parametrize("t", ["f64", "f32", "f16", "bf16"])
+def test_dequantize_unaligned(cuda, t, layout, offset, pad):
+    """A result at any multiple of an element; what lies around it is left as it was."""
+    rows, cols = 37, 93
+    codes, scales = R.random_mx4(np.random.default_rng(offset), rows, cols)
+    Q = rb.MX4Matrix(rows, cols, torch.from_numpy(codes).to(cuda), torch.from_numpy(scales).to(cuda))
+    inner, outer = (cols, rows) if layout == "R" else (rows, cols)
+    buf = torch.full((offset + outer * (inner + pad) + 16,), 7.0, dtype=TORCH[t], device=cuda)
+    rb.mx4_dequantize(layout, "N", rows, cols, Q, buf[offset:], inner + pad)
+    got = buf.cpu()
+    body = got[offset: offset + outer * (inner + pad)].view(outer, inner + pad)
+    exp = torch.from_numpy(R.values(codes, scales, cols)).to(TORCH[t])
+    assert torch.equal(body[:, :inner], exp if layout == "R" else exp.t())
+    assert torch.all(body[:, inner:] == 7.0) and torch.all(got[:offset] == 7.0) and torch.all(got[-16:] == 7.0)
+
+
 def test_dequantize_extreme_scales(cuda):
     """2^-127 (a subnormal) to 2^127: 64-bit values are exact, 32-bit ones overflow to infinity."""
     codes = np.tile(np.arange(0, 256, 16, dtype=np.uint8), (3, 1))
@@ -315,6 +333,38 @@ def test_few_rows_exact(cuda, opB, t, m, n, k):
         c = Case(cuda, side, a, b, k, t, layout, *ops, m, True, low=126, high=127)
         c.run()
         c.check_bitwise()
+
+
+@pytest.mark.parametrize("side,t,opB,layout,m,n,k,pad", [
+    ("right", "bf16", "T", "R", 4100, 4099, 200, 1),    # 256 x 256, rows of C at odd multiples of an element
+    ("right", "bf16", "N", "C", 4100, 4100, 264, 0),
+    ("left", "bf16", "T", "C", 4099, 4100, 264, 3),
+    ("left", "bf16", "N", "R", 4100, 4100, 200, 4),
+    ("right", "bf16", "T", "C", 2100, 4100, 300, 1),    # 256 x 128
+    ("right", "f32", "N", "R", 2100, 4098, 136, 2),
+    ("left", "f16", "T", "R", 4098, 2100, 300, 0),
+    ("left", "f32", "N", "C", 4100, 2100, 328, 0),
+    ("right", "bf16", "T", "R", 700, 1030, 2500, 3),    # 128 x 128, the contraction cut
+    ("right", "f16", "N", "C", 700, 1001, 2500, 0),
+    ("left", "f32", "T", "C", 1030, 700, 2500, 1),
+    ("right", "bf16", "N", "R", 130, 260, 9000, 0),
+    ("right", "bf16", "T", "R", 50, 4100, 300, 1),      # several groups of few rows
+    ("right", "f16", "T", "C", 75, 900, 5000, 0),
+    ("left", "f32", "T", "R", 64, 100, 3000, 1),
+    ("right", "f32", "N", "R", 100, 600, 3000, 2),
+    ("both", "f32", "T", "R", 4100, 4099, 300, 1),      # 256 x 256
+    ("both", "bf16", "T", "C", 4099, 4100, 520, 0),
+    ("both", "f16", "T", "R", 1050, 1060, 4500, 2),     # 128 x 128, the contraction cut
+    ("both", "f32", "T", "C", 2090, 700, 8200, 1),
+    ("both", "bf16", "T", "R", 260, 130, 9000, 0),      # small, the contraction cut
+])
+def test_every_kernel_exact(cuda, side, t, opB, layout, m, n, k, pad):
+    """Each tile, orientation and split with edges in every direction. Scales 2^-1 and 2^0: a dense factor's
+    products are at most 24 in quarters, two 4-bit factors' at most 36 in 1/16: sums of 9000 are exact."""
+    ops = ("N", "T") if side == "both" else ("N", opB) if side == "right" else (opB, "N")
+    c = Case(cuda, side, m, n, k, t, layout, *ops, m + n, True, alpha=0.5, beta=2.0, pad=pad, ro=1, co=32, low=126, high=127)
+    c.run()
+    c.check_bitwise()
 
 
 @pytest.mark.parametrize("scale_pad", [0, 1, 3])
