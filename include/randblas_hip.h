@@ -410,8 +410,8 @@ int rbh_sksy_tri_ex_f32(char layout, char side, char uplo, char A_fmt, int64_t d
  * rows are never read for a result nor written. codes and ld_codes are multiples of 16, scales may have
  * any alignment. (Where scales and ld_scales are multiples of 4, products read whole words of 4 scales,
  * otherwise they copy them first.) ld_codes
- * and ld_scales are at most 2^22. Device or host memory, as for every matrix; all device arrays
- * of a call are on one device. */
+ * and ld_scales are at most 2^22, n_rows at most 2^28. Device or host memory, as for every matrix; all
+ * device arrays of a call are on one device. */
 typedef struct rbh_mx4 {
     int64_t n_rows, n_cols;
     uint8_t *codes;
@@ -462,10 +462,11 @@ int rbh_mx4_dequantize_bf16(char layout, char op, int64_t n_rows, int64_t n_cols
 
 /* C (m x n) = alpha op(A) op(B) + beta C, sums in 32 bits. right: B is submat(B) of a 4-bit matrix at
  * (ro_b, co_b), as the sparse factor of rbh_spmm_right_*; left: A is; both: both are, and their blocks
- * have to lie along the contraction (opA = 'N', opB = 'T'). Column offsets are multiples of 32. The
- * dense factor and C have one type, k is at most 2^21; the dense factor enters the sums with all its bits. The gradient of
- * a product's dense factor is the product of C's gradient with op flipped on the 4-bit one. C overlaps
- * no other array. */
+ * have to lie along the contraction (opA = 'N', opB = 'T'). Column offsets are multiples of 32; a window
+ * that ends inside a block of a wider matrix is copied first where its further codes would count. The
+ * dense factor and C have one type, m and n are at most 2^28, k at most 2^21; the dense factor enters the
+ * sums with all its bits, 4-bit values of 2^128 or more as infinities. The gradient of a product's dense
+ * factor is the product of C's gradient with op flipped on the 4-bit one. C overlaps no other array. */
 int rbh_mxmm_right_f32(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const float *A,
                        int64_t lda, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta, float *C, int64_t ldc,
                        rbh_work *work, void *stream);

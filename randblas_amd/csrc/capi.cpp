@@ -1890,6 +1890,7 @@ int mx4_window(Stager &st, bool codes_here, bool scales_here, const rbh_mx4 *Q, 
     v.cols = cols;
     v.ldq = Q->ld_codes;
     v.lds = Q->ld_scales;
+    v.cut = cols % MX4_BLOCK != 0 && co + cols < Q->n_cols;
     if (rows == 0 || cols == 0) return RBH_OK;
     const int64_t nb = mx4_blocks(cols);
     uint8_t *q = Q->codes + ro * Q->ld_codes + co / 2, *sc = Q->scales + ro * Q->ld_scales + co / MX4_BLOCK;
@@ -1908,8 +1909,9 @@ int mx4_window(Stager &st, bool codes_here, bool scales_here, const rbh_mx4 *Q, 
 #define RBH_REQUIRE_MX4(Q, rows, cols, ro, co)                          \
     RBH_REQUIRE(mx4_ok(Q));                                             \
     RBH_REQUIRE((ro) >= 0 && (co) >= 0 && (co) % 32 == 0);              \
-    RBH_REQUIRE((Q)->n_rows >= (rows) + (ro));                          \
-    RBH_REQUIRE((Q)->n_cols >= (cols) + (co));                          \
+    RBH_REQUIRE((Q)->n_rows <= (1 << 28));                              \
+    RBH_REQUIRE((Q)->n_rows >= (rows) && (Q)->n_rows - (rows) >= (ro)); \
+    RBH_REQUIRE((Q)->n_cols >= (cols) && (Q)->n_cols - (cols) >= (co)); \
     RBH_REQUIRE((Q)->ld_codes % 16 == 0 && (Q)->ld_codes <= (1 << 22)); \
     RBH_REQUIRE((Q)->ld_scales <= (1 << 22));                           \
     RBH_REQUIRE((Q)->ld_codes >= 16 * mx4_blocks((Q)->n_cols));         \
@@ -1998,7 +2000,7 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
     RBH_REQUIRE(layout == 'C' || layout == 'R');
     RBH_REQUIRE(opA == 'N' || opA == 'T');
     RBH_REQUIRE(opB == 'N' || opB == 'T');
-    RBH_REQUIRE(m >= 0 && n >= 0 && k >= 0 && k <= (1 << 21));
+    RBH_REQUIRE(m >= 0 && n >= 0 && k >= 0 && m <= (1 << 28) && n <= (1 << 28) && k <= (1 << 21));
     const int64_t rows_A = opA == 'N' ? m : k, cols_A = opA == 'N' ? k : m;
     const int64_t rows_B = opB == 'N' ? k : n, cols_B = opB == 'N' ? n : k;
     RBH_REQUIRE(ldc >= (layout == 'C' ? m : n));
@@ -2042,7 +2044,7 @@ int mxmm(int type, char side, char layout, char opA, char opB, int64_t m, int64_
     auto view = [&](const rbh_mx4 *Q, const bool *here, int64_t ro, int64_t co, int64_t rows, int64_t cols, Mx4View &v) -> int {
         if (query || !reads) {
             v = Mx4View{Q->codes + ro * Q->ld_codes + co / 2, Q->scales + ro * Q->ld_scales + co / MX4_BLOCK, Q->ld_codes,
-                        Q->ld_scales, rows, cols};
+                        Q->ld_scales, rows, cols, cols % MX4_BLOCK != 0 && co + cols < Q->n_cols};
             return RBH_OK;
         }
         return mx4_window(st, here[0], here[1], Q, ro, co, rows, cols, false, v);

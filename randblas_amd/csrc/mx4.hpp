@@ -16,11 +16,13 @@ inline int mx4_size(int type) { return type == MX4_F64 ? 8 : type == MX4_F32 ? 4
 constexpr int MX4_BLOCK = 32;
 __host__ __device__ inline int64_t mx4_blocks(int64_t cols) { return (cols + MX4_BLOCK - 1) / MX4_BLOCK; }
 
-// rows x cols window of a 4-bit matrix that starts at a block; ldq / lds: bytes between rows
+// rows x cols window of a 4-bit matrix that starts at a block; ldq / lds: bytes between rows; cut: it ends
+// inside a block whose further codes belong to the matrix
 struct Mx4View {
     uint8_t *codes, *scales;
     int64_t ldq, lds;
     int64_t rows, cols;
+    bool cut;
 };
 
 // A dense matrix seen as element (r, c) = ptr[r * sr + c * sc]; sr or sc is 1

@@ -144,9 +144,9 @@ size_t packed_scales(const Mx4View &v) { return (size_t)(pack_groups(v) * ((mx4_
 __global__ __launch_bounds__(256) void pack_scales_kernel(PackJob a, PackJob b, unsigned groups_a, int nb, int steps) {
     constexpr int PITCH = 132;   // bytes a block, so that those of a row are on different banks
     __shared__ __attribute__((aligned(16))) uint8_t packed[PACK_BLOCKS * PITCH];
-    const PackJob &j = blockIdx.y < groups_a ? a : b;
-    const int64_t group = blockIdx.y < groups_a ? blockIdx.y : blockIdx.y - groups_a, groups = (j.rows + 127) / 128;
-    const int b0 = blockIdx.x * PACK_BLOCKS;
+    const PackJob &j = blockIdx.x < groups_a ? a : b;
+    const int64_t group = blockIdx.x < groups_a ? blockIdx.x : blockIdx.x - groups_a, groups = (j.rows + 127) / 128;
+    const int b0 = blockIdx.y * PACK_BLOCKS;
     const int w = threadIdx.x & 15, k0 = b0 + 4 * w;   // 16 threads a row, 4 scales each
     const bool words = (uintptr_t)j.src % 4 == 0 && j.lds % 4 == 0;
     const int64_t row0 = group * 128;
@@ -340,7 +340,7 @@ hipError_t launch_both_tile(const Mx4View &P, const Mx4View &O, uint8_t *work, i
     const int nb = (int)mx4_blocks(P.cols), steps = (nb + 7) / 8;
     uint8_t *ps = work, *os = work + packed_scales(P);
     const unsigned gp = (unsigned)pack_groups(P), go = (unsigned)pack_groups(O);
-    hipLaunchKernelGGL(pack_scales_kernel, dim3((unsigned)((nb + PACK_BLOCKS - 1) / PACK_BLOCKS), gp + go), dim3(256), 0, s,
+    hipLaunchKernelGGL(pack_scales_kernel, dim3(gp + go, (unsigned)((nb + PACK_BLOCKS - 1) / PACK_BLOCKS)), dim3(256), 0, s,
                        PackJob{P.scales, P.lds, P.rows, (uint32_t *)ps}, PackJob{O.scales, O.lds, O.rows, (uint32_t *)os}, gp, nb, steps);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(256) void planes_kernel(const T *__restrict__ x, in
         r = blockIdx.y;
         c8 = (int64_t)blockIdx.x * 256 + threadIdx.x;
     }
-    for (; COLS ? r < rows && c8 < n8 : r < rows && c8 < n8;) {
+    while (r < rows && c8 < n8) {
         uint32_t b[8][PL];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
@@ -1044,6 +1044,49 @@ hipError_t align_scales(Mx4View &v, uint8_t *&work, hipStream_t s) {
 
 constexpr size_t round256(size_t n) { return (n + 255) / 256 * 256; }
 
+// A window that ends inside a block of a wider matrix holds that block's further codes, which the products
+// would take with the other factor's: they are zeros in a copy.
+__global__ __launch_bounds__(256) void trim_codes_kernel(const uint8_t *src, int64_t ldq, int64_t rows, int nb, int tail, uint8_t *dst) {
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    if (b >= nb) return;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        v4u c = *(const v4u *)(src + r * ldq + b * 16);
+        if (b == nb - 1)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int have = tail - 8 * i;   // columns of this word
+                c[i] = have >= 8 ? c[i] : have > 0 ? c[i] & ((1u << (4 * have)) - 1) : 0u;
+            }
+        *(v4u *)(dst + ((int64_t)r * nb + b) * 16) = c;
+    }
+}
+size_t trim_work(const Mx4View &v) { return v.cut ? round256((size_t)v.rows * mx4_blocks(v.cols) * 16) : 0; }
+hipError_t trim_codes(Mx4View &v, uint8_t *&work, hipStream_t s) {
+    if (!v.cut) return hipSuccess;
+    const int nb = (int)mx4_blocks(v.cols);
+    const dim3 grid((unsigned)((nb + 255) / 256), (unsigned)(v.rows < 65535 ? v.rows : 65535));
+    hipLaunchKernelGGL(trim_codes_kernel, grid, dim3(256), 0, s, v.codes, v.ldq, v.rows, nb, (int)(v.cols - (nb - 1) * 32), work);
+    const size_t bytes = trim_work(v);
+    v.codes = work;
+    v.ldq = nb * 16;
+    v.cut = false;
+    work += bytes;
+    return hipGetLastError();
+}
+
+// One factor that ends in zeros is enough for two 4-bit ones, the smaller one. A dense factor ends in zeros too, but
+// 0 times a 4-bit value of 2^128 or more would be a NaN. Across the contraction nothing has to be cut.
+Mx4Product cut_once(const Mx4Product &q) {
+    Mx4Product p = q;
+    if (p.yt) p.Y.cut = false;
+    if (p.both) {
+        const bool cut = p.XQ.cut && p.Y.cut;
+        p.XQ.cut = cut && p.M < p.N;
+        p.Y.cut = cut && p.M >= p.N;
+    }
+    return p;
+}
+
 template <typename T> hipError_t launch_join(const float *partial, int slices, const Out &out, hipStream_t s) {
     const int64_t n = ((out.np + 3) / 4 * out.no + 255) / 256;
     hipLaunchKernelGGL((join_kernel<T>), dim3((unsigned)(n < 65536 ? n : 65536)), dim3(256), 0, s, partial, slices, out);
@@ -1269,19 +1312,26 @@ template <int TYPE> hipError_t product_t(const Mx4Product &p, void *work, hipStr
                            dim3(256), 0, s, p, inner, outer, p.ci == 1 ? p.cj : p.ci);
         return hipGetLastError();
     }
-    return p.both ? both_t<TYPE>(p, (uint8_t *)work, s) : mixed_t<TYPE>(p, (uint8_t *)work, s);
+    Mx4Product c = cut_once(p);
+    uint8_t *w = (uint8_t *)work;
+    hipError_t e = trim_codes(c.XQ, w, s);
+    if (e == hipSuccess) e = trim_codes(c.Y, w, s);
+    if (e != hipSuccess) return e;
+    return c.both ? both_t<TYPE>(c, w, s) : mixed_t<TYPE>(c, w, s);
 }
 
 }  // namespace
 
-size_t mx4_product_work(const Mx4Product &p) {
-    if (p.K <= 0 || p.alpha == 0.f) return 0;
+size_t mx4_product_work(const Mx4Product &q) {
+    if (q.K <= 0 || q.alpha == 0.f) return 0;
+    const Mx4Product p = cut_once(q);
+    const size_t cut = trim_work(p.XQ) + trim_work(p.Y);
     if (p.both) {
         const BothPlan b = both_plan(p);
-        return b.scales + b.partials;
+        return cut + b.scales + b.partials;
     }
     const MixedPlan m = mixed_plan(p);
-    return m.scales + m.planes + m.partials;
+    return cut + m.scales + m.planes + m.partials;
 }
 
 hipError_t launch_mx4_product(const Mx4Product &p, void *work, hipStream_t s) {

@@ -423,6 +423,66 @@ def test_nan_scale_reaches_its_outputs_only(cuda, m, side, opB):
     assert np.array_equal(got[~np.isnan(exp)], exp[~np.isnan(exp)].astype(np.float32))
 
 
+@pytest.mark.parametrize("side,opA,opB", [("right", "N", "T"), ("right", "N", "N"), ("left", "N", "T"), ("left", "T", "N"),
+                                          ("both", "N", "T")])
+@pytest.mark.parametrize("m,n,k", [(3, 5, 1), (1, 70, 40), (40, 33, 100), (260, 700, 333), (700, 1030, 300), (20, 20, 9000)])
+def test_window_inside_a_block(cuda, m, n, k, side, opA, opB):
+    """Windows that end inside a block of wider matrices, at rows and columns that end inside them too: the
+    block's further codes are of 2^127 (as a product infinite, times 0 a NaN) and do not count. Scales 2^0."""
+    rng = np.random.default_rng(k)
+    ro, co, more = 2, 64, 45
+
+    def factor(rows, cols, op):
+        r, c = (rows, cols) if op == "N" else (cols, rows)
+        codes, scales = R.random_mx4(rng, r + ro + 3, c + co + more, 127, 127)
+        if c % 32:
+            scales[:, (co + c) // 32] = 255 - 1
+            inside = R.random_mx4(rng, r + ro + 3, c + co, 127, 127)[0] * 0   # in the window's last block zeros
+            a, b = (co + c) // 32 * 16, (co + c) // 2
+            codes[:, a:b] = inside[:, a:b]
+            if c % 2:
+                codes[:, b] &= 0xF0
+            codes[:, b + c % 2: a + 16] = 0x77
+        Q = rb.MX4Matrix(r + ro + 3, c + co + more, torch.from_numpy(codes).to(cuda), torch.from_numpy(scales).to(cuda))
+        v = R.values(codes, scales, c + co + more)[ro: ro + r, co: co + c]
+        return Q, v if op == "N" else v.T
+
+    def dense(rows, cols, op):
+        x = rng.integers(-4, 5, (rows, cols)).astype(np.float64)
+        buf, ld = stored(torch.from_numpy(x).float(), "R", op, 1, cuda)
+        return buf, ld, x
+
+    if side == "right":
+        buf, ld, a = dense(m, k, opA)
+        Q, b = factor(k, n, opB)
+        args = (buf, ld, Q, ro, co)
+    elif side == "left":
+        Q, a = factor(m, k, opA)
+        buf, ld, b = dense(k, n, opB)
+        args = (Q, ro, co, buf, ld)
+    else:
+        QA, a = factor(m, k, opA)
+        QB, b = factor(k, n, opB)
+        args = (QA, ro, co, QB, ro, co)
+    C = torch.full((m * n,), float("nan"), device=cuda)
+    rb.mxmm("R", opA, opB, m, n, k, 1.0, *args, 0.0, C, n)
+    assert np.array_equal(C.cpu().double().numpy().reshape(m, n), a @ b)
+
+
+@pytest.mark.parametrize("m,n", [(3, 5), (64, 300), (700, 1030)])
+def test_both_windows_inside_a_block(cuda, m, n):
+    """Ordinary codes behind both windows, and behind one of them only."""
+    rng = np.random.default_rng(m)
+    for k, past_a, past_b in ((40, 24, 24), (335, 9, 200), (335, 0, 200), (335, 200, 0)):
+        (ca, sa), (cb, sb) = (R.random_mx4(rng, r, k + past, 126, 128) for r, past in ((m, past_a), (n, past_b)))
+        A, B = (rb.MX4Matrix(c.shape[0], k + past, torch.from_numpy(c).to(cuda), torch.from_numpy(s).to(cuda))
+                for c, s, past in ((ca, sa, past_a), (cb, sb, past_b)))
+        C = torch.full((m * n,), float("nan"), device=cuda)
+        rb.mxmm("C", "N", "T", m, n, k, 1.0, A, 0, 0, B, 0, 0, 0.0, C, m)
+        exp = R.values(ca, sa, k + past_a)[:, :k] @ R.values(cb, sb, k + past_b)[:, :k].T
+        assert np.array_equal(C.cpu().double().numpy().reshape(n, m).T, exp)
+
+
 @pytest.mark.parametrize("side", ["right", "left", "both"])
 def test_alpha_zero_and_empty_contraction(cuda, side):
     """alpha = 0 or k = 0: C = beta C, factors unread (NaN in them does not show), beta = 0 writes zeros."""

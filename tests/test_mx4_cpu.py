@@ -112,8 +112,8 @@ def test_dequantize_refusals():
     d = rb.mx4_dequantize
     refused("layout == 'C'", d, "x", "N", 40, 70, handle(40, 70), A, 70)
     refused("lda >=", d, "R", "N", 40, 70, handle(40, 70), A, 69)
-    refused("n_rows >= (n_rows) + (ro)", d, "R", "N", 40, 70, handle(40, 70), A, 70, ro=1)
-    refused("n_cols >= (n_cols) + (co)", d, "R", "N", 40, 70, handle(40, 70), A, 70, co=32)
+    refused("n_rows - (n_rows) >= (ro)", d, "R", "N", 40, 70, handle(40, 70), A, 70, ro=1)
+    refused("n_cols - (n_cols) >= (co)", d, "R", "N", 40, 70, handle(40, 70), A, 70, co=32)
     refused("(co) % 32 == 0", d, "R", "N", 40, 8, handle(40, 70), A, 70, co=16)
     refused("(ro) >= 0", d, "R", "N", 40, 8, handle(40, 70), A, 70, ro=-1)
     refused("A != nullptr", d, "R", "N", 40, 70, handle(40, 70), Null(np.float32), 70)
@@ -129,13 +129,20 @@ def test_product_refusals():
     refused("m >= 0", mm, "R", "N", "T", -5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 9)
     refused("ldc >=", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 8)
     refused("ldd >=", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 63, B, 0, 0, 0.0, C, 9)
-    refused("n_cols >= (cols_B) + (co_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 32, 0.0, C, 9)
-    refused("n_rows >= (rows_B) + (ro_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 1, 0, 0.0, C, 9)
+    refused("n_cols - (cols_B) >= (co_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 32, 0.0, C, 9)
+    refused("n_rows - (rows_B) >= (ro_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 1, 0, 0.0, C, 9)
     refused("(co_b) % 32 == 0", mm, "R", "N", "T", 5, 9, 32, 1.0, A, 64, B, 0, 8, 0.0, C, 9)
-    refused("n_rows >= (rows_A) + (ro_a)", mm, "R", "N", "N", 10, 5, 64, 1.0, B, 0, 0, A, 5, 0.0, np.zeros(50, np.float32), 5)
+    refused("n_rows - (rows_A) >= (ro_a)", mm, "R", "N", "N", 10, 5, 64, 1.0, B, 0, 0, A, 5, 0.0, np.zeros(50, np.float32), 5)
     refused("D != nullptr", mm, "R", "N", "T", 5, 9, 64, 1.0, Null(np.float32), 64, B, 0, 0, 0.0, C, 9)
     refused("opA == 'N' && opB == 'T'", mm, "R", "N", "N", 9, 64, 9, 1.0, handle(9, 9), 0, 0, B, 0, 0, 0.0,
             np.zeros(9 * 64, np.float32), 64)
+    # sizes beyond what offsets of 32 bits and the grids reach; offsets whose sum with a size would wrap
+    big = 2 ** 28 + 1
+    refused("m <= (1 << 28)", mm, "R", "N", "T", big, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, C, 9)
+    refused("n <= (1 << 28)", mm, "R", "N", "T", 5, big, 64, 1.0, A, 64, B, 0, 0, 0.0, C, big)
+    refused("k <= (1 << 21)", mm, "R", "N", "T", 5, 9, 2 ** 21 + 1, 1.0, A, 2 ** 21 + 1, B, 0, 0, 0.0, C, 9)
+    refused("n_rows - (rows_B) >= (ro_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 2 ** 63 - 1, 0, 0.0, C, 9)
+    refused("n_cols - (cols_B) >= (co_b)", mm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 2 ** 63 - 32, 0.0, C, 9)
     with pytest.raises(TypeError):   # no 64-bit products
         mm("R", "N", "T", 5, 9, 64, 1.0, A.astype(np.float64), 64, B, 0, 0, 0.0, C.astype(np.float64), 9)
     with pytest.raises(TypeError):   # one type
