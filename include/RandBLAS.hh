@@ -28,6 +28,7 @@
 #include <cmath>
 #include <cstdint>
 #include <cstring>
+#include <new>
 #include <stdexcept>
 #include <string>
 #include <tuple>
@@ -944,5 +945,142 @@ inline void spmm(blas::Layout layout, blas::Op opA, blas::Op opB, int64_t m, int
                                             (const int64_t *)B.idx_arr(), B.vals, ro_b, co_b, beta, C, ldc, nullptr));
     detail::coo_after_apply(B, opB == blas::Op::NoTrans);   // right_spmm flips opB (:194)
 }
+
+// ---------------------------------------------------------------------------------------------
+// 4-bit microscaled matrices (no reference counterpart): quantisation, its inverse, products
+// ---------------------------------------------------------------------------------------------
+namespace ext {
+// 16-bit elements, as their bits
+struct f16 { uint16_t bits; };
+struct bf16 { uint16_t bits; };
+
+// n_rows x n_cols in MXFP4 (the layout is rbh_mx4's). Owns zeroed host memory, or refers to the caller's
+// arrays, on the host or a device.
+struct MX4Matrix {
+    int64_t n_rows, n_cols;
+    uint8_t *codes;
+    int64_t ld_codes;
+    uint8_t *scales;
+    int64_t ld_scales;
+    bool own_memory;
+
+    MX4Matrix(int64_t n_rows_, int64_t n_cols_)
+        : n_rows(n_rows_), n_cols(n_cols_), codes(nullptr), ld_codes((n_cols_ + 31) / 32 * 16), scales(nullptr),
+          ld_scales((n_cols_ + 31) / 32), own_memory(true) {
+        RBH_CXX_REQUIRE(n_rows_ >= 0 && n_cols_ >= 0);
+        codes = new (std::align_val_t(16)) uint8_t[(size_t)(n_rows * ld_codes)]();
+        try {
+            scales = new uint8_t[(size_t)(n_rows * ld_scales)]();
+        } catch (...) {
+            ::operator delete[](codes, std::align_val_t(16));
+            throw;
+        }
+    }
+    MX4Matrix(int64_t n_rows_, int64_t n_cols_, uint8_t *codes_, int64_t ld_codes_, uint8_t *scales_, int64_t ld_scales_)
+        : n_rows(n_rows_), n_cols(n_cols_), codes(codes_), ld_codes(ld_codes_), scales(scales_), ld_scales(ld_scales_),
+          own_memory(false) {}
+    MX4Matrix(const MX4Matrix &) = delete;
+    MX4Matrix &operator=(const MX4Matrix &) = delete;
+    MX4Matrix(MX4Matrix &&o) noexcept
+        : n_rows(o.n_rows), n_cols(o.n_cols), codes(o.codes), ld_codes(o.ld_codes), scales(o.scales),
+          ld_scales(o.ld_scales), own_memory(o.own_memory) {
+        o.own_memory = false;
+    }
+    MX4Matrix &operator=(MX4Matrix &&) = delete;
+    ~MX4Matrix() {
+        if (!own_memory) return;
+        ::operator delete[](codes, std::align_val_t(16));
+        delete[] scales;
+    }
+    rbh_mx4 c() const { return rbh_mx4{n_rows, n_cols, codes, ld_codes, scales, ld_scales}; }
+};
+}  // namespace ext
+
+namespace detail {
+template <typename T> struct MX4Api;
+#define RBH_CXX_MX4(T, SUF, C_T)                                                   \
+    template <> struct MX4Api<T> {                                                 \
+        typedef C_T c_type;                                                        \
+        static constexpr auto quantize = rbh_mx4_quantize_##SUF;                   \
+        static constexpr auto dequantize = rbh_mx4_dequantize_##SUF;               \
+        RBH_CXX_MX4_PRODUCTS_##SUF                                                 \
+    };
+#define RBH_CXX_MX4_PRODUCTS_f64
+#define RBH_CXX_MX4_PRODUCTS_f32 RBH_CXX_MX4_PRODUCTS(f32)
+#define RBH_CXX_MX4_PRODUCTS_f16 RBH_CXX_MX4_PRODUCTS(f16)
+#define RBH_CXX_MX4_PRODUCTS_bf16 RBH_CXX_MX4_PRODUCTS(bf16)
+#define RBH_CXX_MX4_PRODUCTS(SUF)                          \
+    static constexpr auto right = rbh_mxmm_right_##SUF;    \
+    static constexpr auto left = rbh_mxmm_left_##SUF;      \
+    static constexpr auto both = rbh_mxmm_both_##SUF;
+RBH_CXX_MX4(double, f64, double)
+RBH_CXX_MX4(float, f32, float)
+RBH_CXX_MX4(ext::f16, f16, uint16_t)
+RBH_CXX_MX4(ext::bf16, bf16, uint16_t)
+#undef RBH_CXX_MX4
+#undef RBH_CXX_MX4_PRODUCTS
+#undef RBH_CXX_MX4_PRODUCTS_f64
+#undef RBH_CXX_MX4_PRODUCTS_f32
+#undef RBH_CXX_MX4_PRODUCTS_f16
+#undef RBH_CXX_MX4_PRODUCTS_bf16
+template <typename T> inline typename MX4Api<T>::c_type *mx4_arr(T *p) { return (typename MX4Api<T>::c_type *)p; }
+template <typename T> inline const typename MX4Api<T>::c_type *mx4_arr(const T *p) { return (const typename MX4Api<T>::c_type *)p; }
+}  // namespace detail
+
+namespace ext {
+// Q (n_rows x n_cols) = op(A), to the nearest element
+template <typename T>
+inline void mx4_quantize(blas::Layout layout, blas::Op op, int64_t n_rows, int64_t n_cols, const T *A, int64_t lda,
+                         MX4Matrix &Q) {
+    const rbh_mx4 q = Q.c();
+    detail::check(detail::MX4Api<T>::quantize((char)layout, (char)op, n_rows, n_cols, detail::mx4_arr(A), lda, &q,
+                                              RBH_ROUND_NEAREST, nullptr, nullptr, nullptr));
+}
+// the same without bias, by the words of `seed`; returns the state after them
+template <typename T, typename RNG>
+inline RNGState<RNG> mx4_quantize(blas::Layout layout, blas::Op op, int64_t n_rows, int64_t n_cols, const T *A,
+                                  int64_t lda, MX4Matrix &Q, const RNGState<RNG> &seed) {
+    const rbh_mx4 q = Q.c();
+    const rbh_state s = detail::c_state(seed);
+    rbh_state next{};
+    detail::check(detail::MX4Api<T>::quantize((char)layout, (char)op, n_rows, n_cols, detail::mx4_arr(A), lda, &q,
+                                              RBH_ROUND_STOCHASTIC, &s, &next, nullptr));
+    return detail::from_c<RNG>(next);
+}
+// op(A) = submat(Q), n_rows x n_cols at (ro, co)
+template <typename T>
+inline void mx4_dequantize(blas::Layout layout, blas::Op op, int64_t n_rows, int64_t n_cols, const MX4Matrix &Q,
+                           int64_t ro, int64_t co, T *A, int64_t lda) {
+    const rbh_mx4 q = Q.c();
+    detail::check(detail::MX4Api<T>::dequantize((char)layout, (char)op, n_rows, n_cols, &q, ro, co, detail::mx4_arr(A),
+                                                lda, nullptr));
+}
+
+// C = alpha * op(submat(A)) * op(B) + beta * C, A 4-bit (m x k after op), B dense
+template <typename T>
+inline void mxmm(blas::Layout layout, blas::Op opA, blas::Op opB, int64_t m, int64_t n, int64_t k, float alpha,
+                 const MX4Matrix &A, int64_t ro_a, int64_t co_a, const T *B, int64_t ldb, float beta, T *C, int64_t ldc) {
+    const rbh_mx4 a = A.c();
+    detail::check(detail::MX4Api<T>::left((char)layout, (char)opA, (char)opB, m, n, k, alpha, &a, ro_a, co_a,
+                                          detail::mx4_arr(B), ldb, beta, detail::mx4_arr(C), ldc, nullptr, nullptr));
+}
+// C = alpha * op(A) * op(submat(B)) + beta * C, A dense, B 4-bit (k x n after op)
+template <typename T>
+inline void mxmm(blas::Layout layout, blas::Op opA, blas::Op opB, int64_t m, int64_t n, int64_t k, float alpha,
+                 const T *A, int64_t lda, const MX4Matrix &B, int64_t ro_b, int64_t co_b, float beta, T *C, int64_t ldc) {
+    const rbh_mx4 b = B.c();
+    detail::check(detail::MX4Api<T>::right((char)layout, (char)opA, (char)opB, m, n, k, alpha, detail::mx4_arr(A), lda,
+                                           &b, ro_b, co_b, beta, detail::mx4_arr(C), ldc, nullptr, nullptr));
+}
+// C = alpha * submat(A) * submat(B)^T + beta * C, both 4-bit
+template <typename T>
+inline void mxmm(blas::Layout layout, blas::Op opA, blas::Op opB, int64_t m, int64_t n, int64_t k, float alpha,
+                 const MX4Matrix &A, int64_t ro_a, int64_t co_a, const MX4Matrix &B, int64_t ro_b, int64_t co_b,
+                 float beta, T *C, int64_t ldc) {
+    const rbh_mx4 a = A.c(), b = B.c();
+    detail::check(detail::MX4Api<T>::both((char)layout, (char)opA, (char)opB, m, n, k, alpha, &a, ro_a, co_a, &b, ro_b,
+                                          co_b, beta, detail::mx4_arr(C), ldc, nullptr, nullptr));
+}
+}  // namespace ext
 
 }  // namespace RandBLAS

@@ -7,6 +7,9 @@ products in 32 bits is within (k + 2) 2^-24 of the sum of magnitudes, whatever t
 and the product's own rounding, one each for alpha and for the final addition of beta C), and the result
 is rounded once to its type, half a step (eps / 2).
 """
+import os
+import subprocess
+
 import numpy as np
 import pytest
 import torch
@@ -651,3 +654,13 @@ def test_run_together(cuda):
     # unbiased rounding: an element is off by less than a gap of its block (at most 2 units)
     unit = np.repeat(2.0 ** (scale.astype(np.float64) - 127), 32, 1)
     assert np.all(np.abs(q2 - b2) < 2 * unit)
+
+
+def test_cpp_client(tmp_path):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    exe, libdir = str(tmp_path / "test_mx4"), os.path.join(root, "randblas_amd")
+    subprocess.run(["g++", "-std=c++17", "-O2", "-Wall", "-I", os.path.join(root, "include"), "-I", "/opt/rocm/include",
+                    "-D__HIP_PLATFORM_AMD__", os.path.join(root, "tests", "cpp", "test_mx4.cc"), "-L", libdir, "-lrandblas_hip",
+                    "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{libdir}", "-o", exe], check=True)
+    out = subprocess.run([exe], capture_output=True, text=True, timeout=100)
+    assert out.returncode == 0 and "ALL PASSED" in out.stdout, out.stdout + out.stderr

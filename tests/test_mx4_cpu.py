@@ -2,6 +2,9 @@
 C ABI (all of them come before any GPU work)."""
 import ctypes
 
+import os
+import subprocess
+
 import numpy as np
 import pytest
 
@@ -187,3 +190,14 @@ def test_empty_products(m, n, k):
     C = np.full(64, 7.0, np.float32)
     rb.mxmm("R", "N", "T", m, n, k, 1.0, np.zeros(512, np.float32), max(k, 1), handle(n, k), 0, 0, 0.0, C, max(n, 1))
     assert np.all(C == 7.0)
+
+
+@pytest.mark.parametrize("std", ["c++17", "c++20"])
+def test_cpp_client_compiles_and_links(tmp_path, std):
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    libdir = os.path.join(root, "randblas_amd")
+    r = subprocess.run(["g++", f"-std={std}", "-O1", "-Wall", "-Werror", "-I", os.path.join(root, "include"), "-I", "/opt/rocm/include",
+                        "-D__HIP_PLATFORM_AMD__", os.path.join(root, "tests", "cpp", "test_mx4.cc"), "-L", libdir, "-lrandblas_hip",
+                        "-L/opt/rocm/lib", "-lamdhip64", f"-Wl,-rpath,{libdir}", "-o", str(tmp_path / "t")],
+                       capture_output=True, text=True)
+    assert r.returncode == 0, r.stderr
