@@ -46,35 +46,44 @@ template <typename F, int... I> __device__ __forceinline__ void static_for_(F &&
 }
 template <int N, typename F> __device__ __forceinline__ void static_for(F &&f) { static_for_(f, std::make_integer_sequence<int, N>{}); }
 
-// out[o * ld + p] = alpha * sum + beta * out[o * ld + p]
+// out[o * ld + p] = alpha * sum + beta * out[o * ld + p]. Four consecutive p are one access at any multiple of
+// an element (3635 x 4651 f32 onto itself, single elements: 114 us, this 71).
 struct Out {
     void *ptr;
     int64_t ld;
     int64_t np, no;
     float alpha, beta;
-    bool vec;   // four consecutive p at a multiple of four are one aligned access
 };
-template <typename T> __device__ __forceinline__ void store4(const Out &o, int64_t p, int64_t q, v4f v) {
+template <typename T> struct Four {
     typedef T t4 __attribute__((ext_vector_type(4)));
-    if (q >= o.no || p >= o.np) return;
-    T *c = (T *)o.ptr + q * o.ld + p;
-    if (o.vec && p + 4 <= o.np) {
-        t4 r;
-        if (o.beta != 0.f) {
-            const t4 old = *(const t4 *)c;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = (T)(o.alpha * v[i] + o.beta * (float)old[i]);
+    T *c;
+    int n;   // how many there are
+    t4 old;
+    __device__ __forceinline__ void load(const Out &o, T *at, int count) {
+        c = at;
+        n = count;
+        if (o.beta == 0.f) return;
+        if (n == 4) {
+            __builtin_memcpy(&old, c, sizeof old);
         } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = (T)(o.alpha * v[i]);
+            for (int i = 0; i < 3; ++i)
+                if (i < n) old[i] = c[i];
         }
-        *(t4 *)c = r;
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (p + i < o.np) c[i] = (T)(o.beta != 0.f ? o.alpha * v[i] + o.beta * (float)c[i] : o.alpha * v[i]);
     }
-}
+    __device__ __forceinline__ void store(const Out &o, v4f v) {
+        t4 r;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) r[i] = (T)(o.beta != 0.f ? o.alpha * v[i] + o.beta * (float)old[i] : o.alpha * v[i]);
+        if (n == 4) {
+            __builtin_memcpy(c, &r, sizeof r);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (i < n) c[i] = r[i];
+        }
+    }
+};
 
 // A range of memory for loads straight to LDS (16 bytes a lane, lane after lane from `lds`, which is the
 // same for the wave). An offset at or past the range's end reads zeros; `soffset` is added to the address
@@ -182,33 +191,28 @@ __global__ __launch_bounds__(256) void pack_scales_kernel(PackJob a, PackJob b, 
 
 // this slice's partial sums as a result: [slice][no][np]
 __device__ __forceinline__ Out partial_of(const Out &o, float *partial) {
-    return Out{partial + (int64_t)blockIdx.y * o.np * o.no, o.np, o.np, o.no, 1.f, 0.f, o.np % 4 == 0};
+    return Out{partial + (int64_t)blockIdx.y * o.np * o.no, o.np, o.np, o.no, 1.f, 0.f};
 }
 
 // A wave's WP x RO part of a result, RO rows of p after each other in LDS, to memory in whole lines: operands
-// hold 4 consecutive entries of many rows, and stores of those are 16 bytes to a line. `pitch` words a row.
-template <typename T, int WP, int RO, typename Row>
-__device__ __forceinline__ void store_rows(const Out &o, const float *from, int pitch, int64_t p0, int64_t q0, Row row_of, int lane) {
-    if (o.vec) {
-        constexpr int L = WP / 4 < 64 ? WP / 4 : 64, R = 64 / L;   // lanes a row, rows at once
-        static_assert(WP % 4 == 0 && 64 % L == 0 && RO % R == 0 && WP <= 256, "whole rows");
-#pragma unroll 4
-        for (int r = 0; r < RO; r += R) {
-            const int row = r + lane / L, p = lane % L * 4;
-            store4<T>(o, p0 + p, q0 + row_of(row), *(const v4f *)(from + row * pitch + p));
-        }
-    } else {
-        for (int r = 0; r < RO; ++r) {
-            const int64_t q = q0 + row_of(r);
-            if (q >= o.no) break;
-            T *c = (T *)o.ptr + q * o.ld + p0;
+// hold 4 consecutive entries of many rows, and stores of those are 16 bytes to a line. `pitch` words a row. What
+// is there already is read some rows ahead of the stores.
+template <typename T, int WP, int RO, int STEP>
+__device__ __forceinline__ void store_rows(const Out &o, const float *from, int pitch, int64_t p0, int64_t q0, int lane) {
+    constexpr int L = WP / 4, R = 64 / L, N = RO / R, U = N < 8 ? N : 8;   // lanes a row, rows at once
+    static_assert(WP % 4 == 0 && 64 % L == 0 && RO % R == 0 && N % U == 0, "whole rows");
+    const int p = lane % L * 4, row = lane / L;
+    const int have = (int)(o.no - q0 < RO * STEP ? o.no - q0 : RO * STEP);   // rows of the result from q0
+    const int count = p0 + p >= o.np ? 0 : o.np - p0 - p < 4 ? (int)(o.np - p0 - p) : 4;
+    T *c = (T *)o.ptr + (q0 + row * STEP) * o.ld + p0 + p;
+    from += row * pitch + p;
 #pragma unroll
-            for (int p = lane; p < WP; p += 64)
-                if (p0 + p < o.np) {
-                    const float v = o.alpha * from[r * pitch + p];
-                    c[p] = (T)(o.beta != 0.f ? v + o.beta * (float)c[p] : v);
-                }
-        }
+    for (int r = 0; r < RO; r += U * R) {
+        Four<T> x[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].load(o, c + (r + u * R) * STEP * o.ld, (r + u * R + row) * STEP < have ? count : 0);
+#pragma unroll
+        for (int u = 0; u < U; ++u) x[u].store(o, *(const v4f *)(from + (r + u * R) * pitch));
     }
 }
 
@@ -319,7 +323,6 @@ __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kerne
         now = STAGE - now;
     }
     float *rows = (float *)lds + wave * 32 * PITCH;   // this wave's
-    auto same = [](int r) { return r; };
 #pragma unroll
     for (int b = 0; b < FO; ++b) {
 #pragma unroll
@@ -329,8 +332,8 @@ __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kerne
                 *(v4f *)(rows + r32 * PITCH + a * 32 + 8 * i + 4 * g) =
                     v4f{acc[a][b][4 * i], acc[a][b][4 * i + 1], acc[a][b][4 * i + 2], acc[a][b][4 * i + 3]};
         __builtin_amdgcn_wave_barrier();
-        if (partial) store_rows<float, WP, 32>(partial_of(out, partial), rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, same, lane);
-        else store_rows<T, WP, 32>(out, rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, same, lane);
+        if (partial) store_rows<float, WP, 32, 1>(partial_of(out, partial), rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, lane);
+        else store_rows<T, WP, 32, 1>(out, rows, PITCH, p0 + wp * WP, o0 + wo * WO + b * 32, lane);
         __builtin_amdgcn_wave_barrier();
     }
 }
@@ -371,6 +374,14 @@ __device__ __forceinline__ v4u decode_bf16(uint32_t w, float scale) {
     r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
     r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 2));
     r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 3));
+    return r;
+}
+
+// the same for the 4 of a half word
+__device__ __forceinline__ v2u decode_bf16_4(uint32_t w, float scale) {
+    v2u r;
+    r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 0));
+    r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(w, scale, 1));
     return r;
 }
 
@@ -448,10 +459,11 @@ struct Dense16 {
 //   codes, blocks along the contraction: SS steps at once, 256 elements, so that rows are whole lines of 128 bytes
 //     (128 where LDS is short), the next ones a part of the rows a step; 16-byte blocks kept like the dense
 //     pieces, the rows' scales behind them
-//   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes a word (8 columns 8 c .. +
-//     7) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 8
-//     operands are then columns 8 c + f, and the operand f of the wave is columns f, f + 8, .. -- an order of
-//     the result's rows or columns that the stores undo. Scales are kept as the upper halves of floats.
+//   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes half a word (4 columns 4 c ..
+//     + 3) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 4
+//     operands are then columns 4 c + f, and the operand f of the wave is columns f, f + 4, .. -- an order of
+//     the result's rows or columns that the stores undo. Scales are kept as the upper halves of floats. An element
+//     costs an instruction in every wave that decodes it, which is why waves are no wider than 64.
 template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
@@ -459,11 +471,12 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     constexpr int FQ = WQ / 16, FD = WD / 16;
     constexpr int LD = BD * 8 / NT;
     static_assert(BD * 8 % NT == 0 && NT / 8 % 16 == 0, "whole loads of the dense rows");
-    static_assert(BQ * 2 == NT, "one load of codes a thread");
-    static_assert(!YT || WQ == 128, "8 columns a lane");
+    constexpr int CW = BQ / 32;   // waves that load codes, one load a thread
+    static_assert(CW <= NW, "waves that load codes");
+    static_assert(!YT || WQ == 64, "4 columns a lane");
     constexpr int DENSE = PL * BD * 128;
     constexpr int PITCH = YT ? (BQ == 256 ? 1056 : 1088) : 1024;   // 64 lanes' codes; lane groups on different banks
-    constexpr int CODES = YT ? NW * PITCH : 0;
+    constexpr int CODES = YT ? CW * PITCH : 0;
     constexpr int SCALES = YT ? BQ / 32 * 128 : 0;
     constexpr int STAGE = DENSE + CODES + SCALES;
     // blocks along: codes and scales of SS steps at a time
@@ -508,7 +521,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
     // blocks along: part c (of the rows) of codes and scales u
     auto load_super = [&](int u, int c) {
         uint8_t *to = supers + (u & 1) * SUPER;
-        load_lds16(qb, to + (c * NT + wave * 64) * 16, u * NP + qpart < nb ? vq + (uint32_t)(c * (BQ / SS) * Y.ldq) : OUTSIDE, u * NP * 16);
+        if (wave < CW)
+            load_lds16(qb, to + (c * CW + wave) * 1024, u * NP + qpart < nb ? vq + (uint32_t)(c * (BQ / SS) * Y.ldq) : OUTSIDE, u * NP * 16);
         if (wave < BQ / 128)
             load_lds4(sb, to + BQ * 32 * SS + (c * (BQ / 2) + wave * 64) * 4,
                       u * NP + tid % (SS / 2) * 4 < nb ? vs + (uint32_t)(c * (BQ / SS) * Y.lds) : OUTSIDE, u * NP);
@@ -528,7 +542,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
                 const int w = tid % WR;
                 sreg = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, w * 4 < nb ? (int)((tid / WR) * Y.lds + w * 4) : (int)OUTSIDE, 0, 0);
             }
-            load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
+            if (wave < CW) load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
         }
         const bool in = step * 8 + piece < D.chunks;
 #pragma unroll
@@ -590,14 +604,14 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             v4u q[FQ];
             if constexpr (YT) {
                 constexpr int ROW = BQ / 2;               // bytes of codes a row; rows 16 g + 8 t .. + 7 are in one piece
-                const uint8_t *cq = lds + (DENSE + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 64 + r16 * 4);
-                const uint8_t *sq = lds + (DENSE + CODES + (wq * 4 + (r16 >> 2)) * 128 + g * 32 + t * 16);
+                const uint8_t *cq = lds + (DENSE + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 32 + r16 * 2);
+                const uint8_t *sq = lds + (DENSE + CODES + (wq * 2 + (r16 >> 3)) * 128 + g * 32 + t * 16);
                 const v4u sc = *(const v4u *)sq;
-                v4u row[8];
+                v2u row[8];
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
                     const uint32_t half = (j & 1) ? sc[j >> 1] & 0xFFFF0000u : sc[j >> 1] << 16;
-                    row[j] = decode_bf16(*(const uint32_t *)(cq + j * ROW), __builtin_bit_cast(float, half));
+                    row[j] = decode_bf16_4(*(const uint16_t *)(cq + j * ROW), __builtin_bit_cast(float, half));
                 }
 #pragma unroll
                 for (int f = 0; f < FQ; ++f)
@@ -639,13 +653,14 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 
     __syncthreads();
     // to memory by way of LDS, 16 rows of the second index at a time. Entry i of a lane's 4 is row 4 g + i of
-    // the first operand; YT: the 4-bit index of row r of operand f is 8 r + f
+    // the first operand; YT: the 4-bit index of row r of operand f is 4 r + f
     const int64_t n1 = QFIRST ? q0 + wq * WQ : d0 + wd * WD;
     float *rows = (float *)lds + wave * 16 * PITCH1;   // this wave's
-    auto out_rows = [&](int64_t n2, auto row) {
+    constexpr int STEP = YT && !QFIRST ? 4 : 1;
+    auto out_rows = [&](int64_t n2) {
         __builtin_amdgcn_wave_barrier();
-        if (partial) store_rows<float, W1, 16>(partial_of(out, partial), rows, PITCH1, n1, n2, row, lane);
-        else store_rows<T, W1, 16>(out, rows, PITCH1, n1, n2, row, lane);
+        if (partial) store_rows<float, W1, 16, STEP>(partial_of(out, partial), rows, PITCH1, n1, n2, lane);
+        else store_rows<T, W1, 16, STEP>(out, rows, PITCH1, n1, n2, lane);
         __builtin_amdgcn_wave_barrier();
     };
     if constexpr (QFIRST) {
@@ -658,20 +673,16 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             } else {
 #pragma unroll
                 for (int i = 0; i < 4; ++i)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h)
-                        *(v4f *)(to + (4 * g + i) * 8 + 4 * h) =
-                            v4f{acc[4 * h][fd][i], acc[4 * h + 1][fd][i], acc[4 * h + 2][fd][i], acc[4 * h + 3][fd][i]};
+                    *(v4f *)(to + (4 * g + i) * 4) = v4f{acc[0][fd][i], acc[1][fd][i], acc[2][fd][i], acc[3][fd][i]};
             }
-            out_rows(d0 + wd * WD + fd * 16, [](int r) { return r; });
+            out_rows(d0 + wd * WD + fd * 16);
         }
     } else {
 #pragma unroll
         for (int fq = 0; fq < FQ; ++fq) {
 #pragma unroll
             for (int fd = 0; fd < FD; ++fd) *(v4f *)(rows + r16 * PITCH1 + fd * 16 + 4 * g) = acc[fq][fd];
-            if constexpr (YT) out_rows(q0 + wq * WQ + fq, [](int r) { return 8 * r; });
-            else out_rows(q0 + wq * WQ + fq * 16, [](int r) { return r; });
+            out_rows(q0 + wq * WQ + (YT ? fq : fq * 16));
         }
     }
 }
@@ -991,21 +1002,24 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
 template <typename T>
 __global__ __launch_bounds__(256) void join_kernel(const float *__restrict__ partial, int slices, Out out) {
     const int64_t n4 = (out.np + 3) / 4, plane = out.np * out.no;
-    const bool vec = out.np % 4 == 0;
     for (int64_t t = (int64_t)blockIdx.x * 256 + threadIdx.x; t < n4 * out.no; t += (int64_t)gridDim.x * 256) {
         const int64_t q = t / n4, p = (t - q * n4) * 4;
         const float *x = partial + q * out.np + p;
+        Four<T> c;
+        c.load(out, (T *)out.ptr + q * out.ld + p, out.np - p < 4 ? (int)(out.np - p) : 4);
         v4f sum{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 4
         for (int z = 0; z < slices; ++z) {
-            if (vec) {
-                sum += *(const v4f *)(x + z * plane);
+            v4f v;
+            if (c.n == 4) {
+                __builtin_memcpy(&v, x + z * plane, sizeof v);
             } else {
 #pragma unroll
-                for (int i = 0; i < 4; ++i) sum[i] += x[z * plane + (p + i < out.np ? i : 0)];
+                for (int i = 0; i < 4; ++i) v[i] = x[z * plane + (i < c.n ? i : 0)];
             }
+            sum += v;
         }
-        store4<T>(out, p, q, sum);
+        c.store(out, sum);
     }
 }
 
@@ -1141,7 +1155,7 @@ template <int TYPE> hipError_t both_t(const Mx4Product &q, uint8_t *work, hipStr
     Mx4Product p = q;
     const bool xp = p.ci == 1;   // X's index is the contiguous one of C
     const int64_t ld = xp ? p.cj : p.ci;
-    const Out out{p.C, ld, xp ? p.M : p.N, xp ? p.N : p.M, p.alpha, p.beta, (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
+    const Out out{p.C, ld, xp ? p.M : p.N, xp ? p.N : p.M, p.alpha, p.beta};
     if (m.tile) {
         // the factor whose rows are the contiguous index gives the operand whose 4 entries a lane holds
         const Mx4View &P = xp ? p.XQ : p.Y, &O = xp ? p.Y : p.XQ;
@@ -1270,8 +1284,7 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     Mx4Product p = q;
     const bool qfirst = p.cj == 1;   // the 4-bit factor's index is the contiguous one of C
     const int64_t ld = qfirst ? p.ci : p.cj;
-    const Out out{p.C, ld, qfirst ? p.N : p.M, qfirst ? p.M : p.N, p.alpha, p.beta,
-                  (uintptr_t)p.C % (4 * sizeof(T)) == 0 && ld % 4 == 0};
+    const Out out{p.C, ld, qfirst ? p.N : p.M, qfirst ? p.M : p.N, p.alpha, p.beta};
     hipError_t e = align_scales(p.Y, work, s);
     if (e != hipSuccess) return e;
     Dense16 D{(const uint16_t *)p.X.ptr, p.M, p.X.sr, 0, (int)(p.K / 8)};
@@ -1296,9 +1309,9 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     auto go = [&](auto yt) -> hipError_t {
         constexpr bool YT = decltype(yt)::value;
         if constexpr (Planes<T>::N == 1)
-            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, YT ? 128 : 64, YT ? 64 : 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        return launch_mixed_tile<T, YT, 128, 128, YT ? 128 : 64, YT ? 32 : 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, 64, 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, 64, 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        return launch_mixed_tile<T, YT, 128, 128, 64, Planes<T>::N == 1 ? 64 : 32>(D, p.Y, p.K, m, out, partial, qfirst, s);
     };
     e = p.yt ? go(std::true_type{}) : go(std::false_type{});
     if (e != hipSuccess || !partial) return e;
