@@ -91,7 +91,8 @@ template <typename T> struct Four {
 typedef __amdgpu_buffer_rsrc_t Buffer;
 constexpr uint32_t OUTSIDE = 0x7FFFFFF0u;
 __device__ __forceinline__ Buffer buffer(const void *p, uint32_t bytes) {
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, (int)bytes, 0x00020000);
+    // the same for the wave, which the compiler is told, or it loops over the lanes' descriptors
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<void *>(p), 0, __builtin_amdgcn_readfirstlane((int)bytes), 0x00020000);
 }
 __device__ __forceinline__ void load_lds16(Buffer b, void *lds, uint32_t voffset, uint32_t soffset) {
     __builtin_amdgcn_raw_ptr_buffer_load_lds(b, (__attribute__((address_space(3))) void *)lds, 16, (int)voffset,
@@ -449,76 +450,136 @@ struct Dense16 {
     int chunks;
 };
 
-// BQ rows (YT: columns) of the 4-bit factor x BD rows of the dense one a workgroup, WQ x WD a wave; 64
-// elements of the contraction a step, loaded straight to LDS, double-buffered.
+// A wave's part of the result to memory by way of LDS (16 rows of the second index at a time, `rows` this wave's
+// place), q0 and d0 its first entry. Entry i of a lane's 4 is row 4 g + i of the first operand; with YT the 4-bit
+// index of row r of operand f is 4 r + f.
+template <typename T, bool YT, bool QFIRST, int FQ, int FD>
+__device__ __forceinline__ void store_wave(const v4f (&acc)[FQ][FD], float *rows, const Out &out, float *partial, int64_t q0, int64_t d0, int lane) {
+    constexpr int W1 = (QFIRST ? FQ : FD) * 16, PITCH = W1 + 4, STEP = YT && !QFIRST ? 4 : 1;
+    static_assert(!YT || FQ == 4, "4 columns a lane");
+    const int r16 = lane & 15, g = lane >> 4;
+    const int64_t n1 = QFIRST ? q0 : d0;
+    auto out_rows = [&](int64_t n2) {
+        __builtin_amdgcn_wave_barrier();
+        if (partial) store_rows<float, W1, 16, STEP>(partial_of(out, partial), rows, PITCH, n1, n2, lane);
+        else store_rows<T, W1, 16, STEP>(out, rows, PITCH, n1, n2, lane);
+        __builtin_amdgcn_wave_barrier();
+    };
+    if constexpr (QFIRST) {
+#pragma unroll
+        for (int fd = 0; fd < FD; ++fd) {
+            float *to = rows + r16 * PITCH;
+            if constexpr (YT) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                    *(v4f *)(to + (4 * g + i) * 4) = v4f{acc[0][fd][i], acc[1][fd][i], acc[2][fd][i], acc[3][fd][i]};
+            } else {
+#pragma unroll
+                for (int fq = 0; fq < FQ; ++fq) *(v4f *)(to + fq * 16 + 4 * g) = acc[fq][fd];
+            }
+            out_rows(d0 + fd * 16);
+        }
+    } else {
+#pragma unroll
+        for (int fq = 0; fq < FQ; ++fq) {
+#pragma unroll
+            for (int fd = 0; fd < FD; ++fd) *(v4f *)(rows + r16 * PITCH + fd * 16 + 4 * g) = acc[fq][fd];
+            out_rows(q0 + (YT ? fq : fq * 16));
+        }
+    }
+}
+// LDS that the tile kernels' results pass through
+constexpr int store_bytes(int waves, int wq, int wd, bool qfirst) { return waves * 16 * ((qfirst ? wq : wd) + 4) * 4; }
+
+// acc += q d over 32 elements of the contraction, every plane
+template <bool QFIRST, int FQ, int FD, int PL>
+__device__ __forceinline__ void multiply_bf16(v4f (&acc)[FQ][FD], const v4u (&q)[FQ], const v4u (&d)[PL][FD]) {
+#pragma unroll
+    for (int fq = 0; fq < FQ; ++fq)
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int fd = 0; fd < FD; ++fd)
+                acc[fq][fd] = QFIRST ? mfma_bf16(q[fq], d[p][fd], acc[fq][fd]) : mfma_bf16(d[p][fd], q[fq], acc[fq][fd]);
+}
+
+// The dense factor's side of a tile: BD rows, 64 elements of the contraction a step, straight to LDS as rows of
+// 128 bytes, 16-byte pieces at place piece ^ (row / 2 & 7), a plane after the other.
+template <int PL, int BD, int NT> struct DenseTile {
+    static constexpr int LD = BD * 8 / NT, BYTES = PL * BD * 128, LOADS = PL * LD;
+    static_assert(BD * 8 % NT == 0 && NT / 8 % 16 == 0, "whole loads of the dense rows");
+    Buffer db[PL];
+    uint32_t vd, rd;
+    int piece, chunks, wave;
+    __device__ __forceinline__ DenseTile(const Dense16 &D, int64_t d0, int tid, int w) : chunks(D.chunks), wave(w) {
+        const int nd = (int)(D.rows - d0 < BD ? D.rows - d0 : BD);
+#pragma unroll
+        for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane + d0 * D.ld, (uint32_t)((nd - 1) * D.ld * 2 + D.chunks * 16));
+        piece = (tid & 7) ^ ((tid >> 4) & 7);
+        vd = (uint32_t)((tid >> 3) * D.ld * 2) + piece * 16;
+        rd = (uint32_t)(D.ld * 2) * (NT / 8);
+    }
+    // half h of the loads, or all of them
+    __device__ __forceinline__ void load(int step, uint8_t *to, int h = 2) const {
+        static_assert(LD % 2 == 0, "halves");
+        const bool in = step * 8 + piece < chunks;   // past the last step zeros
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int i = h == 1 ? LD / 2 : 0; i < (h == 0 ? LD / 2 : LD); ++i)
+                load_lds16(db[p], to + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
+    }
+    // operands of instruction t of a step, for 16 FD rows from `row`
+    template <int FD> static __device__ __forceinline__ void read(const uint8_t *from, int row, int t, int lane, v4u (&d)[PL][FD]) {
+        const int r16 = lane & 15, g = lane >> 4;
+        const uint8_t *dp = from + row * 128 + r16 * 128 + ((g * 2 + t) ^ ((r16 >> 1) & 7)) * 16;
+#pragma unroll
+        for (int p = 0; p < PL; ++p)
+#pragma unroll
+            for (int f = 0; f < FD; ++f) d[p][f] = *(const v4u *)(dp + (p * BD + f * 16) * 128);
+    }
+};
+
+// BQ rows of a 4-bit factor whose blocks lie along the contraction x BD rows of the dense one a workgroup, WQ x
+// WD a wave; 64 elements of the contraction a step, loaded straight to LDS, double-buffered.
 //
 // A step's two matrix instructions take their 32 elements from all over the 64: lane group g holds
 // elements 16 g + 8 t .. + 7 of both factors for instruction t, so a lane's 16 codes lie in one word pair
-// and under one scale.
-//   dense: rows of 128 bytes, 16-byte pieces at place piece ^ (row / 2 & 7), a plane after the other
-//   codes, blocks along the contraction: SS steps at once, 256 elements, so that rows are whole lines of 128 bytes
-//     (128 where LDS is short), the next ones a part of the rows a step; 16-byte blocks kept like the dense
-//     pieces, the rows' scales behind them
-//   codes, blocks across it (YT): the step's 64 rows as they are. A lane takes half a word (4 columns 4 c ..
-//     + 3) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words between rows; its 4
-//     operands are then columns 4 c + f, and the operand f of the wave is columns f, f + 4, .. -- an order of
-//     the result's rows or columns that the stores undo. Scales are kept as the upper halves of floats. An element
-//     costs an instruction in every wave that decodes it, which is why waves are no wider than 64.
-template <typename T, int PL, bool YT, int BQ, int BD, int WQ, int WD, bool QFIRST>
+// and under one scale. Codes come SS steps at once, 256 elements, so that rows are whole lines of 128 bytes (128
+// where LDS is short), the next ones a part of the rows a step; 16-byte blocks are kept like the dense pieces,
+// the rows' scales behind them.
+template <typename T, int PL, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
     constexpr int NW = (BQ / WQ) * (BD / WD), NT = NW * 64;
     constexpr int FQ = WQ / 16, FD = WD / 16;
-    constexpr int LD = BD * 8 / NT;
-    static_assert(BD * 8 % NT == 0 && NT / 8 % 16 == 0, "whole loads of the dense rows");
+    typedef DenseTile<PL, BD, NT> Dense;
     constexpr int CW = BQ / 32;   // waves that load codes, one load a thread
     static_assert(CW <= NW, "waves that load codes");
-    static_assert(!YT || WQ == 64, "4 columns a lane");
-    constexpr int DENSE = PL * BD * 128;
-    constexpr int PITCH = YT ? (BQ == 256 ? 1056 : 1088) : 1024;   // 64 lanes' codes; lane groups on different banks
-    constexpr int CODES = YT ? CW * PITCH : 0;
-    constexpr int SCALES = YT ? BQ / 32 * 128 : 0;
-    constexpr int STAGE = DENSE + CODES + SCALES;
-    // blocks along: codes and scales of SS steps at a time
-    constexpr int SS = 2 * (STAGE + BQ * 136) > 160 * 1024 ? 2 : 4, NP = 2 * SS, SUPER = YT ? 0 : BQ * 34 * SS;
-    constexpr int W1 = QFIRST ? WQ : WD, PITCH1 = W1 + 4;
-    constexpr int RING = 2 * (STAGE + SUPER), LDS = RING > NW * 16 * PITCH1 * 4 ? RING : NW * 16 * PITCH1 * 4;
+    constexpr int STAGE = Dense::BYTES;
+    // codes and scales of SS steps at a time
+    constexpr int SS = 2 * (STAGE + BQ * 136) > 160 * 1024 ? 2 : 4, NP = 2 * SS, SUPER = BQ * 34 * SS;
+    constexpr int RING = 2 * (STAGE + SUPER), STORE = store_bytes(NW, WQ, WD, QFIRST), LDS = RING > STORE ? RING : STORE;
     static_assert(LDS <= 160 * 1024, "LDS");
     __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
     uint8_t *const lds0 = lds, *const lds1 = lds + STAGE, *const supers = lds + 2 * STAGE;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int r16 = lane & 15, g = lane >> 4;
-    const int64_t nq = YT ? Y.cols : Y.rows;
     uint32_t iq, id;
-    tile_of(blockIdx.x, (uint32_t)((nq + BQ - 1) / BQ), (uint32_t)((D.rows + BD - 1) / BD), iq, id);
+    tile_of(blockIdx.x, (uint32_t)((Y.rows + BQ - 1) / BQ), (uint32_t)((D.rows + BD - 1) / BD), iq, id);
     const int64_t q0 = (int64_t)iq * BQ, d0 = (int64_t)id * BD;
     const int wq = wave % (BQ / WQ), wd = wave / (BQ / WQ);
-    const int nd = (int)(D.rows - d0 < BD ? D.rows - d0 : BD), mq = (int)(nq - q0 < BQ ? nq - q0 : BQ);
+    const int mq = (int)(Y.rows - q0 < BQ ? Y.rows - q0 : BQ);
     const int steps = (int)((K + 63) / 64), s0 = blockIdx.y * steps_z, s1 = s0 + steps_z < steps ? s0 + steps_z : steps;
 
-    Buffer db[PL];
-#pragma unroll
-    for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane + d0 * D.ld, (uint32_t)((nd - 1) * D.ld * 2 + D.chunks * 16));
-    const int piece = (tid & 7) ^ ((tid >> 4) & 7);
-    const uint32_t vd = (uint32_t)((tid >> 3) * D.ld * 2) + piece * 16, rd = (uint32_t)(D.ld * 2) * (NT / 8);
-    // codes and scales
-    const int nb = (int)mx4_blocks(YT ? mq : Y.cols);   // blocks a row (YT: of this tile)
-    Buffer qb, sb;
-    uint32_t vq, vs;
-    int qpart;
-    if constexpr (YT) {
-        constexpr int PR = BQ / 32;                       // pieces a row
-        qpart = lane % PR;
-        vq = (uint32_t)((wave * (64 / PR) + lane / PR) * Y.ldq) + qpart * 16;
-        vs = 0;
-    } else {
-        qb = buffer(Y.codes + q0 * Y.ldq, (uint32_t)((mq - 1) * Y.ldq + nb * 16));
-        sb = buffer(Y.scales + q0 * Y.lds, (uint32_t)((mq - 1) * Y.lds + (nb + 3) / 4 * 4));
-        qpart = (tid % NP) ^ ((tid >> 4) % NP);
-        vq = (uint32_t)((tid / NP) * Y.ldq) + qpart * 16;
-        vs = (uint32_t)((tid / (SS / 2)) * Y.lds) + tid % (SS / 2) * 4;
-    }
-    // blocks along: part c (of the rows) of codes and scales u
+    const Dense dense(D, d0, tid, wave);
+    const int nb = (int)mx4_blocks(Y.cols);
+    const Buffer qb = buffer(Y.codes + q0 * Y.ldq, (uint32_t)((mq - 1) * Y.ldq + nb * 16));
+    const Buffer sb = buffer(Y.scales + q0 * Y.lds, (uint32_t)((mq - 1) * Y.lds + (nb + 3) / 4 * 4));
+    const int qpart = (tid % NP) ^ ((tid >> 4) % NP);
+    const uint32_t vq = (uint32_t)((tid / NP) * Y.ldq) + qpart * 16;
+    const uint32_t vs = (uint32_t)((tid / (SS / 2)) * Y.lds) + tid % (SS / 2) * 4;
+    // part c (of the rows) of codes and scales u
     auto load_super = [&](int u, int c) {
         uint8_t *to = supers + (u & 1) * SUPER;
         if (wave < CW)
@@ -527,45 +588,127 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
             load_lds4(sb, to + BQ * 32 * SS + (c * (BQ / 2) + wave * 64) * 4,
                       u * NP + tid % (SS / 2) * 4 < nb ? vs + (uint32_t)(c * (BQ / SS) * Y.lds) : OUTSIDE, u * NP);
     };
-    uint32_t sreg = 0;   // YT: 4 scales of a row on their way to LDS
-    auto load = [&](int step, uint8_t *lds) {
-        if constexpr (YT) {
-            const int64_t k0 = (int64_t)step * 64;
-            const int64_t left = K - k0 < 64 ? K - k0 : 64;
-            const uint32_t rows = left > 0 ? (uint32_t)left : 0u;
-            const uint32_t have = rows ? 1u : 0u;
-            // past the last step the range is empty, and reads zeros
-            const Buffer cb = buffer(Y.codes + q0 / 2 + (have ? k0 : 0) * Y.ldq, have * ((rows - 1) * (uint32_t)Y.ldq + nb * 16));
-            const Buffer kb = buffer(Y.scales + q0 / 32 + (have ? k0 : 0) * Y.lds, have * ((rows - 1) * (uint32_t)Y.lds + (nb + 3) / 4 * 4));
-            constexpr int WR = BQ / 128;                  // words of scales a row
-            if (tid < 64 * WR) {
-                const int w = tid % WR;
-                sreg = (uint32_t)__builtin_amdgcn_raw_buffer_load_b32(kb, w * 4 < nb ? (int)((tid / WR) * Y.lds + w * 4) : (int)OUTSIDE, 0, 0);
-            }
-            if (wave < CW) load_lds16(cb, lds + DENSE + wave * PITCH, qpart < nb ? vq : OUTSIDE, 0);
+
+    v4f acc[FQ][FD];
+#pragma unroll
+    for (int a = 0; a < FQ; ++a)
+#pragma unroll
+        for (int b = 0; b < FD; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
+
+    auto compute = [&](int step, const uint8_t *from) {
+        v2u raw[FQ];
+        float scale[FQ];
+        const int c = step % SS;
+        const uint8_t *super = supers + (step / SS & 1) * SUPER;
+        const uint8_t *cq = super + ((wq * WQ + r16) * 32 * SS + (((c * 2 + (g >> 1)) ^ ((r16 * NP >> 4) % NP)) * 16) + (g & 1) * 8);
+        const uint8_t *sq = super + (BQ * 32 * SS + (wq * WQ + r16) * 2 * SS + (c >> 1) * 4);
+        const int bit = (c & 1) * 16 + (g >> 1) * 8;
+        const uint32_t width = step * 2 + (g >> 1) < nb ? 8 : 0;   // past the last block, whatever is there, as 0
+#pragma unroll
+        for (int f = 0; f < FQ; ++f) {
+            raw[f] = *(const v2u *)(cq + f * 16 * 32 * SS);
+            scale[f] = __builtin_bit_cast(float, __builtin_amdgcn_ubfe(*(const uint32_t *)(sq + f * 16 * 2 * SS), bit, width) << 23);
         }
-        const bool in = step * 8 + piece < D.chunks;
 #pragma unroll
-        for (int p = 0; p < PL; ++p)
+        for (int t = 0; t < 2; ++t) {
+            v4u d[PL][FD], q[FQ];
+            Dense::read(from, wd * WD, t, lane, d);
 #pragma unroll
-            for (int i = 0; i < LD; ++i)
-                load_lds16(db[p], lds + (p * BD * 8 + i * NT + wave * 64) * 16, in ? vd + i * rd : OUTSIDE, step * 128);
-    };
-    auto put_scales = [&](uint8_t *lds) {
-        if constexpr (YT) {
-            constexpr int WR = BQ / 128;
-            if (tid < 64 * WR) {
-                uint16_t *s = (uint16_t *)(lds + DENSE + CODES) + (tid % WR) * 4 * 64 + tid / WR;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) s[i * 64] = (uint16_t)(((sreg >> (8 * i)) & 255u) << 7);
-            }
+            for (int f = 0; f < FQ; ++f) q[f] = decode_bf16(raw[f][t], scale[f]);
+            multiply_bf16<QFIRST>(acc, q, d);
         }
     };
-    // the loads have arrived (for YT the scales of the next step too), every wave is done with this step
-    auto next = [&](uint8_t *lds) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        put_scales(lds);
-        __syncthreads();
+#pragma unroll
+    for (int c = 0; c < SS; ++c) load_super(s0 / SS, c);   // slices start at multiples of 4 steps
+    dense.load(s0, lds0);
+    arrive();
+    int st = s0;
+    for (; st + 1 < s1; st += 2) {
+        load_super(st / SS + 1, st % SS);
+        dense.load(st + 1, lds1);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(st, lds0);
+        arrive();
+        load_super((st + 1) / SS + 1, (st + 1) % SS);
+        dense.load(st + 2, lds0);
+        __builtin_amdgcn_sched_barrier(0);
+        compute(st + 1, lds1);
+        arrive();
+    }
+    if (st < s1) compute(st, lds0);
+    __syncthreads();
+    store_wave<T, false, QFIRST>(acc, (float *)lds + wave * (STORE / NW / 4), out, partial, q0 + wq * WQ, d0 + wd * WD, lane);
+}
+
+// The same with blocks across the contraction: BQ columns of the 4-bit factor, 64 of them a wave. A lane takes half
+// a word (4 columns 4 c .. + 3) of 8 rows, decodes it under the 8 rows' scales and exchanges halves of words
+// between rows; its 4 operands are then columns 4 c + f, and the operand f of the wave is columns f, f + 4, .. --
+// an order of the result's rows or columns that the stores undo.
+//
+// An element costs two instructions in every wave that decodes it, about as long as its products take, so the
+// two have to run at the same time: a wave decodes the next instruction's operands among the present one's
+// products, also across steps. For that the codes are one step further ahead than the dense rows, which are two
+// steps ahead (one where LDS is short), and the wait of a step leaves its own loads on their way.
+// Scales go to LDS through registers, a block's after each other; the decoding instruction looks at a float's exponent
+// only, so a shift of the word brings a scale there.
+template <typename T, int PL, int BQ, int BD, int WD, bool QFIRST>
+__global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
+                                                                                      Out out, float *partial) {
+    constexpr int NW = (BQ / 64) * (BD / WD), NT = NW * 64, FQ = 4, FD = WD / 16;
+    typedef DenseTile<PL, BD, NT> Dense;
+    constexpr int PR = BQ / 32, CW = BQ / 32, WR = BQ / 128;   // 16-byte pieces a row; waves that load codes, scales
+    static_assert(CW <= NW, "waves that load codes");
+    constexpr int PITCH = BQ == 256 ? 1056 : 1088, ROW = BQ / 2;   // 64 lanes' codes; lane groups on different banks
+    constexpr int CODES = CW * PITCH + PR * 64;
+    constexpr int STAGE = Dense::BYTES + CODES, DS = 3 * STAGE <= 160 * 1024 ? 3 : 2;   // steps held
+    constexpr int RING = DS * STAGE, STORE = store_bytes(NW, 64, WD, QFIRST), LDS = RING > STORE ? RING : STORE;
+    static_assert(LDS <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) uint8_t lds[LDS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int r16 = lane & 15, g = lane >> 4;
+    uint32_t iq, id;
+    tile_of(blockIdx.x, (uint32_t)((Y.cols + BQ - 1) / BQ), (uint32_t)((D.rows + BD - 1) / BD), iq, id);
+    const int64_t q0 = (int64_t)iq * BQ, d0 = (int64_t)id * BD;
+    const int wq = wave % (BQ / 64), wd = wave / (BQ / 64);
+    const int steps = (int)((K + 63) / 64), s0 = blockIdx.y * steps_z, s1 = s0 + steps_z < steps ? s0 + steps_z : steps;
+
+    const Dense dense(D, d0, tid, wave);
+    const int nb = (int)mx4_blocks(Y.cols - q0 < BQ ? Y.cols - q0 : BQ);   // blocks of a row here
+    const int qpart = lane % PR;
+    const uint32_t vq = qpart < nb ? (uint32_t)((wave * (64 / PR) + lane / PR) * Y.ldq) + qpart * 16 : OUTSIDE;
+    const uint32_t vs = wave * 4 < nb ? (uint32_t)(lane * Y.lds) + wave * 4 : OUTSIDE;
+    uint32_t sreg = 0;   // a row's scales of 4 blocks on their way to LDS
+    auto put_scales = [&](uint8_t *to) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[Dense::BYTES + CW * PITCH + (wave * 4 + i) * 64 + lane] = (uint8_t)(sreg >> (8 * i));
+    };
+    // where the next step to be loaded begins, and how many rows are left there; past the last an empty range
+    // reads zeros
+    const uint32_t ldq = __builtin_amdgcn_readfirstlane((int)Y.ldq), ldk = __builtin_amdgcn_readfirstlane((int)Y.lds);
+    const uint32_t code_bytes = nb * 16, scale_bytes = (nb + 3) / 4 * 4;   // of a row
+    const uint8_t *cp = Y.codes + q0 / 2 + (int64_t)s0 * 64 * Y.ldq, *kp = Y.scales + q0 / 32 + (int64_t)s0 * 64 * Y.lds;
+    int left = (int)K - s0 * 64;
+    auto load_codes = [&](uint8_t *to) {
+        const uint32_t rows = left < 64 ? left : 64;
+        if (wave < WR) sreg = load4(buffer(kp, left > 0 ? (rows - 1) * ldk + scale_bytes : 0u), vs, 0);
+        if (CW == NW || wave < CW)
+            load_lds16(buffer(cp, left > 0 ? (rows - 1) * ldq + code_bytes : 0u), to + Dense::BYTES + wave * PITCH, vq, 0);
+        cp += (uint64_t)ldq * 64;
+        kp += (uint64_t)ldk * 64;
+        left -= 64;
+    };
+    // The next step's loads have arrived, those of DS - 2 steps behind it may be on their way, but for the scales. The
+    // barrier alone: __syncthreads would wait for all of them; what was read from LDS is in use already.
+    auto next = [&](uint8_t *scales_to) {
+        if (wave < WR) {
+            wait_loads<DS == 2 ? 0 : Dense::LOADS + 1>();
+            put_scales(scales_to);
+        } else if (DS == 2) wait_loads<0>();
+        else if (CW == NW || wave < CW) wait_loads<Dense::LOADS + 1>();
+        else wait_loads<Dense::LOADS>();
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_sched_barrier(0);
     };
 
     v4f acc[FQ][FD];
@@ -574,117 +717,82 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 #pragma unroll
         for (int b = 0; b < FD; ++b) acc[a][b] = v4f{0.f, 0.f, 0.f, 0.f};
 
-    int dat[2];
-#pragma unroll
-    for (int t = 0; t < 2; ++t) dat[t] = wd * WD * 128 + r16 * 128 + ((g * 2 + t) ^ ((r16 >> 1) & 7)) * 16;
-    auto compute = [&](int step, const uint8_t *lds) {
-        v2u raw[YT ? 1 : FQ];
-        float scale[YT ? 1 : FQ];
-        if constexpr (!YT) {
-            const int c = step % SS;
-            const uint8_t *super = supers + (step / SS & 1) * SUPER;
-            const uint8_t *cq = super + ((wq * WQ + r16) * 32 * SS + (((c * 2 + (g >> 1)) ^ ((r16 * NP >> 4) % NP)) * 16) + (g & 1) * 8);
-            const uint8_t *sq = super + (BQ * 32 * SS + (wq * WQ + r16) * 2 * SS + (c >> 1) * 4);
-            const int bit = (c & 1) * 16 + (g >> 1) * 8;
-            const uint32_t width = step * 2 + (g >> 1) < nb ? 8 : 0;   // past the last block, whatever is there, as 0
-#pragma unroll
-            for (int f = 0; f < FQ; ++f) {
-                raw[f] = *(const v2u *)(cq + f * 16 * 32 * SS);
-                scale[f] = __builtin_bit_cast(float, __builtin_amdgcn_ubfe(*(const uint32_t *)(sq + f * 16 * 2 * SS), bit, width) << 23);
-            }
-        }
-#pragma unroll
-        for (int t = 0; t < 2; ++t) {
-            v4u d[PL][FD];
-            const uint8_t *dp = lds + dat[t];
-#pragma unroll
-            for (int p = 0; p < PL; ++p)
-#pragma unroll
-                for (int f = 0; f < FD; ++f) d[p][f] = *(const v4u *)(dp + (p * BD + f * 16) * 128);
-            v4u q[FQ];
-            if constexpr (YT) {
-                constexpr int ROW = BQ / 2;               // bytes of codes a row; rows 16 g + 8 t .. + 7 are in one piece
-                const uint8_t *cq = lds + (DENSE + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 32 + r16 * 2);
-                const uint8_t *sq = lds + (DENSE + CODES + (wq * 2 + (r16 >> 3)) * 128 + g * 32 + t * 16);
-                const v4u sc = *(const v4u *)sq;
-                v2u row[8];
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const uint32_t half = (j & 1) ? sc[j >> 1] & 0xFFFF0000u : sc[j >> 1] << 16;
-                    row[j] = decode_bf16_4(*(const uint16_t *)(cq + j * ROW), __builtin_bit_cast(float, half));
-                }
-#pragma unroll
-                for (int f = 0; f < FQ; ++f)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)           // rows 2 j, 2 j + 1 of column f
-                        q[f][j] = __builtin_amdgcn_perm(row[2 * j + 1][f >> 1], row[2 * j][f >> 1], (f & 1) ? 0x07060302u : 0x05040100u);
-            } else {
-#pragma unroll
-                for (int f = 0; f < FQ; ++f) q[f] = decode_bf16(raw[f][t], scale[f]);
-            }
-#pragma unroll
-            for (int fq = 0; fq < FQ; ++fq)
-#pragma unroll
-                for (int p = 0; p < PL; ++p)
-#pragma unroll
-                    for (int fd = 0; fd < FD; ++fd)
-                        acc[fq][fd] = QFIRST ? mfma_bf16(q[fq], d[p][fd], acc[fq][fd]) : mfma_bf16(d[p][fd], q[fq], acc[fq][fd]);
-        }
+    struct Raw {
+        uint32_t c[8];
+        v2u s;
     };
-    if constexpr (!YT)   // slices start at multiples of 4 steps
+    auto read_codes = [&](const uint8_t *from, int t, Raw &x) {
+        const uint8_t *cq = from + (Dense::BYTES + (BQ == 256 ? (g * 2 + t) * PITCH : g * PITCH + t * 8 * ROW) + wq * 32 + r16 * 2);
+        x.s = *(const v2u *)(from + (Dense::BYTES + CW * PITCH + (wq * 2 + (r16 >> 3)) * 64 + 16 * g + 8 * t));
 #pragma unroll
-        for (int c = 0; c < SS; ++c) load_super(s0 / SS, c);
-    load(s0, lds0);
-    next(lds0);
-    int st = s0;
-    for (; st + 1 < s1; st += 2) {
-        if constexpr (!YT) load_super(st / SS + 1, st % SS);
-        load(st + 1, lds1);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(st, lds0);
-        next(lds1);
-        if constexpr (!YT) load_super((st + 1) / SS + 1, (st + 1) % SS);
-        load(st + 2, lds0);
-        __builtin_amdgcn_sched_barrier(0);
-        compute(st + 1, lds1);
-        next(lds0);
-    }
-    if (st < s1) compute(st, lds0);
-
-    __syncthreads();
-    // to memory by way of LDS, 16 rows of the second index at a time. Entry i of a lane's 4 is row 4 g + i of
-    // the first operand; YT: the 4-bit index of row r of operand f is 4 r + f
-    const int64_t n1 = QFIRST ? q0 + wq * WQ : d0 + wd * WD;
-    float *rows = (float *)lds + wave * 16 * PITCH1;   // this wave's
-    constexpr int STEP = YT && !QFIRST ? 4 : 1;
-    auto out_rows = [&](int64_t n2) {
-        __builtin_amdgcn_wave_barrier();
-        if (partial) store_rows<float, W1, 16, STEP>(partial_of(out, partial), rows, PITCH1, n1, n2, lane);
-        else store_rows<T, W1, 16, STEP>(out, rows, PITCH1, n1, n2, lane);
-        __builtin_amdgcn_wave_barrier();
+        for (int j = 0; j < 8; ++j) x.c[j] = *(const uint16_t *)(cq + j * ROW);
     };
-    if constexpr (QFIRST) {
+    // byte i of a word to a float's exponent
+    auto exponent = [](uint32_t w, int i) { return __builtin_bit_cast(float, i < 3 ? w << (23 - 8 * i) : w >> 1); };
+    auto decode = [&](const Raw &x, v4u (&q)[FQ]) {
+        v2u row[8];
 #pragma unroll
-        for (int fd = 0; fd < FD; ++fd) {
-            float *to = rows + r16 * PITCH1;
-            if constexpr (!YT) {
+        for (int j = 0; j < 8; ++j)
+            row[j] = decode_bf16_4(x.c[j], exponent(x.s[j >> 2], j & 3));
 #pragma unroll
-                for (int fq = 0; fq < FQ; ++fq) *(v4f *)(to + fq * 16 + 4 * g) = acc[fq][fd];
-            } else {
+        for (int f = 0; f < FQ; ++f)
 #pragma unroll
-                for (int i = 0; i < 4; ++i)
-                    *(v4f *)(to + (4 * g + i) * 4) = v4f{acc[0][fd][i], acc[1][fd][i], acc[2][fd][i], acc[3][fd][i]};
-            }
-            out_rows(d0 + wd * WD + fd * 16);
+            for (int j = 0; j < 4; ++j)   // rows 2 j, 2 j + 1 of column f
+                q[f][j] = __builtin_amdgcn_perm(row[2 * j + 1][f >> 1], row[2 * j][f >> 1], (f & 1) ? 0x07060302u : 0x05040100u);
+    };
+    struct Operands {
+        v4u q[FQ], d[PL][FD];
+    };
+    // the products of `now`; among them the next operands (of instruction t) are read and decoded, and half of a
+    // step's dense rows is sent for
+    auto half = [&](const Operands &now, Operands &next, const uint8_t *from, int t, int step, uint8_t *to) {
+        Raw x;
+        read_codes(from, t, x);
+        Dense::read(from, wd * WD, t, lane, next.d);
+        dense.load(step, to, t);
+        multiply_bf16<QFIRST>(acc, now.q, now.d);
+        decode(x, next.q);
+        constexpr int M = FQ * FD * PL, V = 40, L = Dense::LOADS / 2;   // matrix instructions, others, loads
+        __builtin_amdgcn_sched_group_barrier(0x100, PL * FD + 9, 0);
+#pragma unroll
+        for (int i = 0; i < M; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+            if (i >= 3) __builtin_amdgcn_sched_group_barrier(0x2, (V + M - 4) / (M - 3), 0);
+            if (i % (M / L) == M / L - 1) __builtin_amdgcn_sched_group_barrier(0x20, 1, 0);
         }
-    } else {
+        __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-        for (int fq = 0; fq < FQ; ++fq) {
+        for (int f = 0; f < FQ; ++f) asm volatile("" : "+v"(next.q[f]));   // here, and not behind the step's barrier
+    };
 #pragma unroll
-            for (int fd = 0; fd < FD; ++fd) *(v4f *)(rows + r16 * PITCH1 + fd * 16 + 4 * g) = acc[fq][fd];
-            out_rows(q0 + wq * WQ + (YT ? fq : fq * 16));
-        }
+    for (int i = 0; i < DS; ++i) {
+        load_codes(lds + i * STAGE);
+        if (wave < WR) put_scales(lds + i * STAGE);
+        if (i < DS - 1) dense.load(s0 + i, lds + i * STAGE);
+        else dense.load(s0 + i, lds + i * STAGE, 0);   // the other half goes with the first products
     }
+    arrive();
+    Operands a, b;
+    {
+        Raw x;
+        read_codes(lds, 0, x);
+        Dense::read(lds, wd * WD, 0, lane, a.d);
+        decode(x, a.q);
+    }
+    // A step's first operands are read during the step before, its second ones during its own first half; then all
+    // waves are done with its place, and the step DS further on goes there.
+    int at = 0, last = (DS - 1) * STAGE;   // places of this step and of the one before
+    for (int st = s0; st < s1; ++st) {
+        half(a, b, lds + at, 1, st + DS - 1, lds + last);
+        next(lds + last);
+        load_codes(lds + at);
+        __builtin_amdgcn_sched_barrier(0);
+        last = at;
+        at = at == (DS - 1) * STAGE ? 0 : at + STAGE;
+        half(b, a, lds + at, 0, st + DS, lds + last);
+    }
+    arrive();   // nothing is on its way to LDS any more
+    store_wave<T, true, QFIRST>(acc, (float *)lds + wave * (STORE / NW / 4), out, partial, q0 + wq * 64, d0 + wd * WD, lane);
 }
 
 // Few dense rows (at most 16 DF): a workgroup takes NQ columns of the result over one slice of the
@@ -865,7 +973,7 @@ template <typename T, int NF, int DF>
 __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void both_rows_kernel(Mx4View Q, Mx4View D, RowsOut out) {
     constexpr int H = NF * DF >= 8 ? 1 : 2;   // what two units in flight leave of the registers
     __shared__ v4f sums[ROWS_WAVES * (NF * DF < 8 ? NF * DF : 8) * 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
     const int64_t q0 = (int64_t)blockIdx.x * (NF * 16), d0 = (int64_t)blockIdx.z * (DF * 16);
     const RowReader<NF, H> q(Q, q0, r16, g);
     const RowReader<DF, H> d(D, d0, r16, g);
@@ -913,7 +1021,7 @@ template <typename T, int DF>
 __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense16 D, Mx4View Y, int K, RowsOut out) {
     constexpr int PL = Planes<T>::N;
     __shared__ v4f sums[ROWS_WAVES * 8 * 64];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r16 = lane & 15, g = lane >> 4;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), r16 = lane & 15, g = lane >> 4;
     const int64_t q0 = (int64_t)blockIdx.x * 256;
     const int nb = (int)(mx4_blocks(Y.cols) - q0 / 32), tile_nb = nb < 8 ? nb : 8;   // blocks of a row from this workgroup's first
     const int units = (K + 31) / 32, stride = ROWS_WAVES * gridDim.y;
@@ -1239,17 +1347,15 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     return m;
 }
 
-template <typename T, bool YT, int BQ, int BD, int WQ, int WD>
+template <typename T, bool YT, int BQ, int BD, int WD>
 hipError_t launch_mixed_tile(const Dense16 &D, const Mx4View &Y, int64_t K, const MixedPlan &m, const Out &out, float *partial,
                              bool qfirst, hipStream_t s) {
-    constexpr int PL = Planes<T>::N;
+    constexpr int PL = Planes<T>::N, WQ = 64;
     const int64_t nq = YT ? Y.cols : Y.rows;
-    const dim3 grid((unsigned)(((nq + BQ - 1) / BQ) * ((D.rows + BD - 1) / BD)), (unsigned)m.slices);
-    constexpr int NT = (BQ / WQ) * (BD / WD) * 64;
-    if (qfirst)
-        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, true>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
-    else
-        hipLaunchKernelGGL((mixed_tile_kernel<T, PL, YT, BQ, BD, WQ, WD, false>), grid, dim3(NT), 0, s, D, Y, K, m.steps_z, out, partial);
+    const dim3 grid((unsigned)(((nq + BQ - 1) / BQ) * ((D.rows + BD - 1) / BD)), (unsigned)m.slices), block((BQ / WQ) * (BD / WD) * 64);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, grid, block, 0, s, D, Y, K, m.steps_z, out, partial); };
+    if constexpr (YT) qfirst ? go(mixed_tile_yt_kernel<T, PL, BQ, BD, WD, true>) : go(mixed_tile_yt_kernel<T, PL, BQ, BD, WD, false>);
+    else qfirst ? go(mixed_tile_kernel<T, PL, BQ, BD, WQ, WD, true>) : go(mixed_tile_kernel<T, PL, BQ, BD, WQ, WD, false>);
     return hipGetLastError();
 }
 
@@ -1309,9 +1415,9 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
     auto go = [&](auto yt) -> hipError_t {
         constexpr bool YT = decltype(yt)::value;
         if constexpr (Planes<T>::N == 1)
-            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, 64, 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, 64, 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
-        return launch_mixed_tile<T, YT, 128, 128, 64, Planes<T>::N == 1 ? 64 : 32>(D, p.Y, p.K, m, out, partial, qfirst, s);
+            if (m.bd == 256) return launch_mixed_tile<T, YT, 256, 256, 128>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        if (m.bq == 256) return launch_mixed_tile<T, YT, 256, 128, 64>(D, p.Y, p.K, m, out, partial, qfirst, s);
+        return launch_mixed_tile<T, YT, 128, 128, Planes<T>::N == 1 ? 64 : 32>(D, p.Y, p.K, m, out, partial, qfirst, s);
     };
     e = p.yt ? go(std::true_type{}) : go(std::false_type{});
     if (e != hipSuccess || !partial) return e;
