@@ -1232,13 +1232,14 @@ BothPlan both_plan(const Mx4Product &p) {
     // One workgroup a compute unit for the kernel for small products, whose workgroups read both factors
     // from the L2 (2048 x 2048 x 2048, 1024 workgroups: 44 us, tiles of 128: 19 us; 256 x 4096 x 2048, 256 of
     // them: 15 and 18 us). Of the tiles the larger ones where there is one for every compute unit (4096 x 4096
-    // x 8192: 72 and 86 us; 2048 x 4096 x 8192: 58 and 47 us).
+    // x 8192: 77 and 86 us; 2048 x 4096 x 8192: 63 and 50 us). The contraction is cut to 256 workgroups (2048 x 2048 x
+    // 8192 f32: 36 us, to 512 41 us; 4096 x 4096 x 4096 uncut 47 us, in two 87 us).
     if (tiles(256) >= 256) m.tile = 256;
     else if (small > 32 && groups() > 256) m.tile = 128;
     if (m.tile) {
         const int64_t steps = (p.K + 255) / 256, t = tiles(m.tile);
         int64_t z = 1;
-        while (t * z * 2 <= 512 && steps / (z * 2) >= 8) z *= 2;
+        while (t * z * 2 <= 256 && steps / (z * 2) >= 8) z *= 2;
         m.steps_z = (int)((steps + z - 1) / z);
         m.slices = (int)((steps + m.steps_z - 1) / m.steps_z);
         m.scales = packed_scales(p.XQ) + packed_scales(p.Y);
