@@ -200,7 +200,7 @@ __device__ __forceinline__ Out partial_of(const Out &o, float *partial) {
 // is there already is read some rows ahead of the stores.
 template <typename T, int WP, int RO, int STEP>
 __device__ __forceinline__ void store_rows(const Out &o, const float *from, int pitch, int64_t p0, int64_t q0, int lane) {
-    constexpr int L = WP / 4, R = 64 / L, N = RO / R, U = N < 8 ? N : 8;   // lanes a row, rows at once
+    constexpr int L = WP / 4, R = 64 / L, N = RO / R, U = N < 16 ? N : 16;   // lanes a row, rows at once
     static_assert(WP % 4 == 0 && 64 % L == 0 && RO % R == 0 && N % U == 0, "whole rows");
     const int p = lane % L * 4, row = lane / L;
     const int have = (int)(o.no - q0 < RO * STEP ? o.no - q0 : RO * STEP);   // rows of the result from q0
@@ -1231,11 +1231,11 @@ BothPlan both_plan(const Mx4Product &p) {
     m.nf = 4;
     // One workgroup a compute unit for the kernel for small products, whose workgroups read both factors
     // from the L2 (2048 x 2048 x 2048, 1024 workgroups: 44 us, tiles of 128: 19 us; 256 x 4096 x 2048, 256 of
-    // them: 15 and 18 us). Of the tiles the larger ones where there is one for every compute unit (4096 x 4096
-    // x 8192: 77 and 86 us; 2048 x 4096 x 8192: 63 and 50 us). The contraction is cut to 256 workgroups (2048 x 2048 x
-    // 8192 f32: 36 us, to 512 41 us; 4096 x 4096 x 4096 uncut 47 us, in two 87 us).
-    if (tiles(256) >= 256) m.tile = 256;
-    else if (small > 32 && groups() > 256) m.tile = 128;
+    // them: 15 and 18 us). Of the tiles the ones whose last round leaves less of the card idle: one of 256 a compute
+    // unit takes 28 for a step where two of 128 take 15 (4096 x 4096 x 4096: 46 and 53 us; 2048 x 4096 x 4096: 47 and
+    // 31; 4096 x 4864 x 4096, a second round for 48 of 304: 70 and 64). The contraction is cut to 256 workgroups
+    // (2048 x 2048 x 8192 f32: 36 us, to 512 41 us; 4096 x 4096 x 4096 uncut 47 us, in two 87 us).
+    if (small > 32 && groups() > 256) m.tile = (tiles(256) + 255) / 256 * 28 < (tiles(128) + 511) / 512 * 15 ? 256 : 128;
     if (m.tile) {
         const int64_t steps = (p.K + 255) / 256, t = tiles(m.tile);
         int64_t z = 1;
