@@ -222,6 +222,8 @@ __device__ __forceinline__ void store_rows(const Out &o, const float *from, int 
 // blocks are kept at place block ^ (row / 2 & 7), which spreads the 16 rows that an access takes at once over
 // all banks (the lane that fills a place loads the block that belongs there). The packed scales lie behind
 // the codes.
+// Bound by the power of the products (fed from registers alone 6.5 PFLOP/s): 8192^3 bf16 271 us with the scales' pass,
+// 4.05 PFLOP/s. Short contractions are bound by the results' way to memory: 4096 x 4096 x 1024 f32 24 us, 2.9 TB/s.
 template <typename T, int BP, int BO, int WP, int WO>
 __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kernel(Mx4View P, Mx4View O, const uint8_t *ps, const uint8_t *os,
                                                                                   int nb, int steps_z, Out out, float *partial) {
@@ -363,7 +365,6 @@ hipError_t launch_both_tile(const Mx4View &P, const Mx4View &O, uint8_t *work, i
 // bits, cut off from the top 8 at a time: each remainder is exact, and 3 bf16 products at 2.5 PFLOP/s are
 // 5 times the f32 instruction's rate). Sums are f32.
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
-typedef __bf16 v2bf __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8bf, a), __builtin_bit_cast(v8bf, b), c, 0, 0, 0);
@@ -409,6 +410,7 @@ __device__ __forceinline__ uint32_t bf16_bits(__bf16 x) { return __builtin_bit_c
 // The planes of a dense factor in a workspace: plane i of element (r, c) at out[(i * rows + r) * ld + c], ld a
 // multiple of 64, zeros behind the last column. One thread makes 8 columns of a row; with COLS the rows
 // are contiguous in memory, and lanes go along them.
+// Bound by HBM: 1001 x 8192 f32 20 us, 4.1 TB/s.
 template <typename T, bool COLS>
 __global__ __launch_bounds__(256) void planes_kernel(const T *__restrict__ x, int64_t stride, int64_t rows, int64_t cols,
                                                      int64_t ld, uint16_t *__restrict__ out) {
@@ -548,6 +550,9 @@ template <int PL, int BD, int NT> struct DenseTile {
 // and under one scale. Codes come SS steps at once, 256 elements, so that rows are whole lines of 128 bytes (128
 // where LDS is short), the next ones a part of the rows a step; 16-byte blocks are kept like the dense pieces,
 // the rows' scales behind them.
+//
+// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 204 us, 1.35 PFLOP/s, the rate of a
+// large bf16 product by the library; 4096 x 1001 x 8192 f32, three planes, 173 us with their pass, 1.16.
 template <typename T, int PL, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
@@ -651,6 +656,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 // steps ahead (one where LDS is short), and the wait of a step leaves its own loads on their way.
 // Scales go to LDS through registers, a block's after each other; the decoding instruction looks at a float's exponent
 // only, so a shift of the word brings a scale there.
+// 2048 x 4096 x 8192 bf16 (256 x 128 tiles) 120 us, 1.14 PFLOP/s, without the operands ahead and with 8 bytes' scales by
+// two reads 146; bound by the decoding beside the products and the reads from LDS.
 template <typename T, int PL, int BQ, int BD, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                       Out out, float *partial) {
@@ -883,8 +890,10 @@ template <int NF, int H> struct RowReader {
 // lines, and only the rows that there are. A half unit (every other block, 128 elements, 256 bytes a row)
 // is a buffer; its piece p of row r is kept at place p ^ r.
 // RG: loads of 4 dense rows each.
+// 1 x 16384 x 4096 bf16 10 us, 3.6 TB/s of codes and scales (a read runs at 3.7); 16 x 4096 x 16384 14.4 us, 2.5 TB/s,
+// 2.5 us of it the addition of the slices.
 template <typename T, int NF, int RG>
-__global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, 2) void mixed_rows_kernel(Dense16 D, Mx4View Y, RowsOut out) {
+__global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) / 4) void mixed_rows_kernel(Dense16 D, Mx4View Y, RowsOut out) {
     constexpr int PL = Planes<T>::N, DF = RG > 4 ? 2 : 1;
     constexpr int BUF = PL * DF * 16 * 256;             // bytes of a wave's half unit
     constexpr int W = dense_waves(PL * DF), C = NF * DF < W ? NF * DF : W;
@@ -969,6 +978,7 @@ __global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, 
 
 // The same for two 4-bit factors, 16 NF x 16 DF entries of the result a workgroup: products too small for
 // the tiles, where the time of a call is the way of its loads.
+// 77 x 1000 x 2080 f16 runs in 6 us, less than a call takes on the host; 256 x 4096 x 2048 bf16 15 us.
 template <typename T, int NF, int DF>
 __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void both_rows_kernel(Mx4View Q, Mx4View D, RowsOut out) {
     constexpr int H = NF * DF >= 8 ? 1 : 2;   // what two units in flight leave of the registers
@@ -1017,6 +1027,8 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void both_rows_kernel(Mx4View Q
     });
 }
 
+// Few dense rows and blocks across the contraction: codes, scales and dense rows from memory to registers, two units on
+// their way. 16 x 8192 x 8192 bf16 20 us, 1.8 TB/s, bound by the decoding (two instructions an element).
 template <typename T, int DF>
 __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense16 D, Mx4View Y, int K, RowsOut out) {
     constexpr int PL = Planes<T>::N;
@@ -1305,7 +1317,7 @@ struct MixedPlan {
 
 MixedPlan mixed_plan(const Mx4Product &p) {
     MixedPlan m{};
-    const int esz = mx4_size(p.type), pl = p.type == MX4_F32 ? 3 : p.type == MX4_F16 ? 2 : 1;
+    const int pl = p.type == MX4_F32 ? 3 : p.type == MX4_F16 ? 2 : 1;
     // 16-byte pieces of 8 elements, whole ones only, rows within reach of a 32-bit offset
     m.direct = p.type == MX4_BF16 && p.X.sc == 1 && (uintptr_t)p.X.ptr % 16 == 0 && p.X.sr % 8 == 0 && p.K % 8 == 0 &&
                p.X.sr <= (1 << 21);
