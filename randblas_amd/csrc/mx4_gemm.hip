@@ -1243,11 +1243,12 @@ BothPlan both_plan(const Mx4Product &p) {
     m.nf = 4;
     // One workgroup a compute unit for the kernel for small products, whose workgroups read both factors
     // from the L2 (2048 x 2048 x 2048, 1024 workgroups: 44 us, tiles of 128: 19 us; 256 x 4096 x 2048, 256 of
-    // them: 15 and 18 us). Of the tiles the ones whose last round leaves less of the card idle: one of 256 a compute
+    // them: 14 and 17 us, at 8192 columns 34 and 23 us). Of the tiles the ones whose last round leaves less of the
+    // card idle: one of 256 a compute
     // unit takes 28 for a step where two of 128 take 15 (4096 x 4096 x 4096: 46 and 53 us; 2048 x 4096 x 4096: 47 and
     // 31; 4096 x 4864 x 4096, a second round for 48 of 304: 70 and 64). The contraction is cut to 256 workgroups
     // (2048 x 2048 x 8192 f32: 36 us, to 512 41 us; 4096 x 4096 x 4096 uncut 47 us, in two 87 us).
-    if (small > 32 && groups() > 256) m.tile = (tiles(256) + 255) / 256 * 28 < (tiles(128) + 511) / 512 * 15 ? 256 : 128;
+    if ((small > 32 && groups() > 256) || (small > 64 && p.K > 4096)) m.tile = (tiles(256) + 255) / 256 * 28 < (tiles(128) + 511) / 512 * 15 ? 256 : 128;
     if (m.tile) {
         const int64_t steps = (p.K + 255) / 256, t = tiles(m.tile);
         int64_t z = 1;
