@@ -506,18 +506,25 @@ __device__ __forceinline__ void multiply_bf16(v4f (&acc)[FQ][FD], const v4u (&q)
 }
 
 // The dense factor's side of a tile: BD rows, 64 elements of the contraction a step, straight to LDS as rows of
-// 128 bytes, 16-byte pieces at place piece ^ (row / 2 & 7), a plane after the other.
-template <int PL, int BD, int NT> struct DenseTile {
+// 128 bytes, a plane after the other. Where 16-byte pieces of a row are kept: the lanes that a read takes at once are rows
+// 0 - 3 and 12 - 15 of one lane group and rows 4 - 11 of the next one, whose pieces differ in bit 1. XOR with row / 2
+// puts the one on the other's banks, XOR with a map of it that sends 12 to 2 does not (bank conflicts 8.6 million and
+// 0.1 million). The latter is faster with blocks along the contraction (4096 x 8192 x 4096, calls in a row: 231 and 240 us)
+// and slower with blocks across (SPREAD off; 2048 x 4096 x 8192: 137 and 132).
+template <int PL, int BD, int NT, bool SPREAD> struct DenseTile {
     static constexpr int LD = BD * 8 / NT, BYTES = PL * BD * 128, LOADS = PL * LD;
     static_assert(BD * 8 % NT == 0 && NT / 8 % 16 == 0, "whole loads of the dense rows");
     Buffer db[PL];
     uint32_t vd, rd;
     int piece, chunks, wave;
+    static __device__ __forceinline__ int place(int piece, int row) {
+        return SPREAD ? piece ^ (row >> 1 & 1) ^ (row & 4) ^ (row & 8 ? 6 : 0) : piece ^ (row >> 1 & 7);
+    }
     __device__ __forceinline__ DenseTile(const Dense16 &D, int64_t d0, int tid, int w) : chunks(D.chunks), wave(w) {
         const int nd = (int)(D.rows - d0 < BD ? D.rows - d0 : BD);
 #pragma unroll
         for (int i = 0; i < PL; ++i) db[i] = buffer(D.ptr + i * D.plane + d0 * D.ld, (uint32_t)((nd - 1) * D.ld * 2 + D.chunks * 16));
-        piece = (tid & 7) ^ ((tid >> 4) & 7);
+        piece = place(tid & 7, tid >> 3);
         vd = (uint32_t)((tid >> 3) * D.ld * 2) + piece * 16;
         rd = (uint32_t)(D.ld * 2) * (NT / 8);
     }
@@ -534,7 +541,7 @@ template <int PL, int BD, int NT> struct DenseTile {
     // operands of instruction t of a step, for 16 FD rows from `row`
     template <int FD> static __device__ __forceinline__ void read(const uint8_t *from, int row, int t, int lane, v4u (&d)[PL][FD]) {
         const int r16 = lane & 15, g = lane >> 4;
-        const uint8_t *dp = from + row * 128 + r16 * 128 + ((g * 2 + t) ^ ((r16 >> 1) & 7)) * 16;
+        const uint8_t *dp = from + row * 128 + r16 * 128 + place(g * 2 + t, r16) * 16;
 #pragma unroll
         for (int p = 0; p < PL; ++p)
 #pragma unroll
@@ -548,8 +555,8 @@ template <int PL, int BD, int NT> struct DenseTile {
 // A step's two matrix instructions take their 32 elements from all over the 64: lane group g holds
 // elements 16 g + 8 t .. + 7 of both factors for instruction t, so a lane's 16 codes lie in one word pair
 // and under one scale. Codes come SS steps at once, 256 elements, so that rows are whole lines of 128 bytes (128
-// where LDS is short), the next ones a part of the rows a step; 16-byte blocks are kept like the dense pieces,
-// the rows' scales behind them.
+// where LDS is short), the next ones a part of the rows a step; 16-byte blocks at place
+// block ^ (row / 2), the rows' scales behind them.
 //
 // 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 204 us, 1.35 PFLOP/s, the rate of a
 // large bf16 product by the library; 4096 x 1001 x 8192 f32, three planes, 173 us with their pass, 1.16.
@@ -558,7 +565,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
                                                                                    Out out, float *partial) {
     constexpr int NW = (BQ / WQ) * (BD / WD), NT = NW * 64;
     constexpr int FQ = WQ / 16, FD = WD / 16;
-    typedef DenseTile<PL, BD, NT> Dense;
+    typedef DenseTile<PL, BD, NT, true> Dense;
     constexpr int CW = BQ / 32;   // waves that load codes, one load a thread
     static_assert(CW <= NW, "waves that load codes");
     constexpr int STAGE = Dense::BYTES;
@@ -662,7 +669,7 @@ template <typename T, int PL, int BQ, int BD, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                       Out out, float *partial) {
     constexpr int NW = (BQ / 64) * (BD / WD), NT = NW * 64, FQ = 4, FD = WD / 16;
-    typedef DenseTile<PL, BD, NT> Dense;
+    typedef DenseTile<PL, BD, NT, false> Dense;
     constexpr int PR = BQ / 32, CW = BQ / 32, WR = BQ / 128;   // 16-byte pieces a row; waves that load codes, scales
     static_assert(CW <= NW, "waves that load codes");
     constexpr int PITCH = BQ == 256 ? 1056 : 1088, ROW = BQ / 2;   // 64 lanes' codes; lane groups on different banks
