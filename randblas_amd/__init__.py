@@ -767,12 +767,11 @@ class MX4Matrix:
         nb = (n_cols + 31) // 32
         at, ld = _bytes_2d(codes, "codes", n_rows, 16 * nb)
         sat, sld = _bytes_2d(scales, "scales", n_rows, nb)
-        set_ = object.__setattr__
-        set_(self, "n_rows", n_rows)
-        set_(self, "n_cols", n_cols)
-        set_(self, "codes", codes)
-        set_(self, "scales", scales)
-        set_(self, "_c", MX4MatrixC(n_rows, n_cols, at, ld, sat, sld))
+        self._hold(n_rows, n_cols, codes, scales, MX4MatrixC(n_rows, n_cols, at, ld, sat, sld))
+
+    def _hold(self, *values):
+        for name, value in zip(self.__slots__, values):
+            object.__setattr__(self, name, value)
 
     def __setattr__(self, name, value):
         raise AttributeError(f"{name} of an MX4Matrix is fixed")
@@ -785,9 +784,12 @@ def mx4_empty(n_rows: int, n_cols: int, device=None) -> MX4Matrix:
     """An uninitialised MX4Matrix of device tensors (device: the current one by default); rows of scales
     start at multiples of 4 bytes."""
     nb = (n_cols + 31) // 32
-    device = device if device is not None else torch.device("cuda", torch.cuda.current_device())
-    return MX4Matrix(n_rows, n_cols, torch.empty((n_rows, 16 * nb), dtype=torch.uint8, device=device),
-                     torch.empty((n_rows, (nb + 3) // 4 * 4), dtype=torch.uint8, device=device))
+    codes = torch.empty((n_rows, 16 * nb), dtype=torch.uint8, device="cuda" if device is None else device)
+    wide = (nb + 3) // 4 * 4
+    scales = codes.new_empty((n_rows, wide))
+    Q = MX4Matrix.__new__(MX4Matrix)   # arrays of its own making need no checks
+    Q._hold(n_rows, n_cols, codes, scales, MX4MatrixC(n_rows, n_cols, codes.data_ptr(), 16 * nb, scales.data_ptr(), wide))
+    return Q
 
 
 def mx4_quantize(layout, op, n_rows, n_cols, A, lda, Q: MX4Matrix, rounding="nearest",

@@ -507,6 +507,84 @@ def test_large_products_agree_with_64_bits(cuda):
         c.check_close()
 
 
+@pytest.mark.parametrize("m", [2, 150])
+@pytest.mark.parametrize("side,opB", [("right", "T"), ("right", "N"), ("both", "T")])
+def test_products_of_extreme_scales(cuda, m, side, opB):
+    """One E2M1 value a column under 2^-127 .. 2^125, times 1: exact, subnormal results included."""
+    k, n = 64, 9 * 16
+    scale = np.repeat(np.array([0, 1, 2, 60, 127, 200, 250, 251, 252]), 16)   # of a column
+    code = np.zeros((n, k), np.uint8)
+    code[:, 33] = np.tile(np.arange(16), 9)
+    if opB == "T":
+        q, s = code, np.full((n, 2), 127)
+        s[:, 1] = scale
+    else:   # a row's blocks hold 32 columns: the even blocks' columns get the lower of two scales
+        q = np.ascontiguousarray(code.T)
+        s = np.full((k, (n + 31) // 32), 127)
+        s[33] = scale[::32][: s.shape[1]]
+    Q = rb.MX4Matrix(*q.shape, torch.from_numpy(R.pack(np.pad(q, ((0, 0), (0, -q.shape[1] % 32))))).to(cuda),
+                     torch.from_numpy(s.astype(np.uint8)).to(cuda))
+    v = R.values(Q.codes.cpu().numpy(), s, q.shape[1])
+    v = v.T if opB == "T" else v
+    C = torch.empty(m * n, dtype=torch.float32, device=cuda)
+    if side == "both":
+        one = rb.MX4Matrix(m, k, torch.full((m, k // 2), 0x22, dtype=torch.uint8, device=cuda),
+                           torch.full((m, 2), 127, dtype=torch.uint8, device=cuda))
+        rb.mxmm("R", "N", "T", m, n, k, 1.0, one, 0, 0, Q, 0, 0, 0.0, C, n)
+    else:
+        x = torch.ones(m * k, dtype=torch.float32, device=cuda)
+        rb.mxmm("R", "N", opB, m, n, k, 1.0, x, k, Q, 0, 0, 0.0, C, n)
+    exp = np.broadcast_to(v.sum(0), (m, n)).astype(np.float32)
+    assert np.array_equal(C.cpu().numpy().reshape(m, n), exp)
+
+
+def test_two_streams_at_once(cuda):
+    """Calls that need workspaces, in flight on two streams together, keep apart."""
+    cases = [Case(cuda, "right", 150, 700, 2100, "f32", "R", "N", "T", 1, True, low=126, high=127),
+             Case(cuda, "right", 300, 500, 3000, "f32", "R", "N", "N", 2, True, low=126, high=127),
+             Case(cuda, "both", 700, 700, 2100, "f32", "R", "N", "T", 3, True, low=126, high=127)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    outs = []
+    for i in range(12):
+        c = cases[i % 3]
+        out = torch.full_like(c.C, float("nan"))
+        outs.append((c, out))
+    torch.cuda.synchronize()
+    for i, (c, out) in enumerate(outs):
+        rb.mxmm(*c.head, *c.factors, 0.0, out, c.ldc, stream=streams[(i // 3) % 2].cuda_stream)
+    torch.cuda.synchronize()
+    for c, out in outs:
+        c.C = out
+        c.check_bitwise()
+
+
+def test_workspace_of_the_callers(cuda):
+    """The C ABI: a query, a block that is large enough, one that is too small, one that is not aligned."""
+    import ctypes
+
+    c = Case(cuda, "right", 150, 300, 1100, "f32", "R", "N", "T", 5, True)
+    buf, lda, Q, ro, co = c.factors
+    fn, w = rb.lib.rbh_mxmm_right_f32, rb.WorkC()
+    call = lambda: fn(b"R", b"N", b"T", 150, 300, 1100, 1.0, buf.data_ptr(), lda, Q._c, ro, co, 0.0, c.C.data_ptr(), c.ldc,
+                      ctypes.byref(w), torch.cuda.current_stream().cuda_stream)
+    assert call() == 0 and w.bytes > 0
+    need = w.bytes
+    block = torch.zeros(need + 512, dtype=torch.uint8, device=cuda)
+    guard = block[need:].clone()
+    w.ptr = block.data_ptr()
+    assert call() == 0
+    c.check_bitwise()
+    assert torch.equal(block[need:], guard)   # nothing behind what was asked for
+    w.bytes = need - 1
+    assert call() != 0 and "work->bytes" in rb.lib.rbh_last_error().decode()
+    w.bytes, w.ptr = need, block.data_ptr() + 16
+    assert call() != 0
+    host = np.zeros(need + 256, np.uint8)
+    w.ptr = host.ctypes.data + (-host.ctypes.data % 256)
+    assert call() != 0 and "work_here" in rb.lib.rbh_last_error().decode()
+
+
 def test_another_stream(cuda):
     c = Case(cuda, "right", 150, 260, 500, "f32", "R", "N", "T", 6, True)
     side = torch.cuda.Stream()
