@@ -16,9 +16,9 @@
 //         (4096 x 5731 bf16 back to elements: single elements stored, four a lane, 35 us, this 24 us).
 //   cols: blocks lie across memory. A lane owns a row's block: 32 loads, each contiguous over the 64
 //         lanes, the maximum in registers, 16 bytes of codes a lane.
-// Quantising and dequantising, two launches: 8192 x 16384 f32 248 us (4.6 TB/s; a copy runs at 4.9), 8192 x 8192
-// bf16 61 us, stochastic 93 us (bound by the generator's integer multiplications), 1024 x 16384 f32 across
-// memory 29 us.
+// Quantising and dequantising, two launches: 8192 x 16384 f32 192 us (5.96 TB/s; a copy through the caches runs at
+// 4.9), 8192 x 8192 bf16 56 us, stochastic 90 us (bound by the generator's integer multiplications), 1024 x 16384 f32
+// across memory 29 us.
 #include "common.hpp"
 #include "mx4.hpp"
 
@@ -137,13 +137,13 @@ __device__ __forceinline__ uint32_t operator/(uint32_t n, const FastDiv &f) {
     return f.d == 1 ? n : (((n - t) >> 1) + t) >> (f.shift - 1);
 }
 
-template <int TYPE, bool SR>
+template <int TYPE, bool SR, bool NT>
 __global__ __launch_bounds__(MXT) void quantize_rows_kernel(const typename Elem<TYPE>::mem *__restrict__ A, int64_t ld,
                                                              Mx4View Q, FastDiv nb, uint32_t units, int64_t row0,
                                                              Mx4Random rnd) {
     typedef typename Elem<TYPE>::mem M;
     typedef typename Elem<TYPE>::val V;
-    typedef M m8_t __attribute__((ext_vector_type(8)));
+    typedef M any8_t __attribute__((ext_vector_type(8), aligned(sizeof(M))));   // one or a few wide loads wherever it is
     const uint32_t u = blockIdx.x * (uint32_t)MXT + threadIdx.x;
     const bool live = u < units;   // whole quads only: 4 units a block
     const uint32_t ub = (live ? u : 0u) >> 2, q = u & 3u;
@@ -152,8 +152,7 @@ __global__ __launch_bounds__(MXT) void quantize_rows_kernel(const typename Elem<
     const M *p = A + r * ld + c;
     V x[8];
     if (c + 8 <= Q.cols) {
-        m8_t m;
-        __builtin_memcpy(&m, p, sizeof m);   // at any multiple of an element one or a few wide loads
+        const any8_t m = NT ? __builtin_nontemporal_load((const any8_t *)p) : *(const any8_t *)p;
 #pragma unroll
         for (int i = 0; i < 8; ++i) x[i] = (V)m[i];
     } else {
@@ -170,7 +169,7 @@ __global__ __launch_bounds__(MXT) void quantize_rows_kernel(const typename Elem<
     if (q == 0) Q.scales[r * Q.lds + b] = (uint8_t)(e + 127);
 }
 
-template <int TYPE, bool SR>
+template <int TYPE, bool SR, bool NT>
 __global__ __launch_bounds__(MXT) void quantize_cols_kernel(const typename Elem<TYPE>::mem *__restrict__ A, int64_t ld,
                                                              Mx4View Q, int64_t nb, Mx4Random rnd) {
     typedef typename Elem<TYPE>::val V;
@@ -182,7 +181,7 @@ __global__ __launch_bounds__(MXT) void quantize_cols_kernel(const typename Elem<
         V x[MX4_BLOCK];
         if (c0 + MX4_BLOCK <= Q.cols) {
 #pragma unroll
-            for (int i = 0; i < MX4_BLOCK; ++i) x[i] = (V)p[i * ld];
+            for (int i = 0; i < MX4_BLOCK; ++i) x[i] = (V)(NT ? __builtin_nontemporal_load(p + i * ld) : p[i * ld]);
         } else {
 #pragma unroll
             for (int i = 0; i < MX4_BLOCK; ++i) x[i] = c0 + i < Q.cols ? (V)p[i * ld] : (V)0;
@@ -230,30 +229,32 @@ template <int TYPE>
 __global__ __launch_bounds__(MXT) void dequantize_rows_kernel(Mx4View Q, typename Elem<TYPE>::mem *__restrict__ A,
                                                                int64_t ld, FastDiv nb, uint32_t units, int64_t row0) {
     typedef typename Elem<TYPE>::mem M;
-    typedef M m8_t __attribute__((ext_vector_type(8)));
+    constexpr int E = 16 / sizeof(M), UB = MX4_BLOCK / E;   // elements a lane, lanes a block: 16 bytes a lane, side by side
+    typedef M any_t __attribute__((ext_vector_type(E), aligned(sizeof(M))));
     const uint32_t u = blockIdx.x * (uint32_t)MXT + threadIdx.x;
     if (u >= units) return;
-    const uint32_t ub = u >> 2, q = u & 3u;
+    const uint32_t ub = u / UB, q = u % UB;
     const uint32_t rr = ub / nb, b = ub - rr * nb.d;
-    const int64_t r = row0 + rr, c = (int64_t)b * MX4_BLOCK + 8 * q;
+    const int64_t r = row0 + rr, c = (int64_t)b * MX4_BLOCK + E * q;
     if (c >= Q.cols) return;
-    const uint32_t w = *reinterpret_cast<const uint32_t *>(Q.codes + r * Q.ldq + (int64_t)b * 16 + 4 * q);
+    const uint8_t *from = Q.codes + r * Q.ldq + (int64_t)b * 16 + E / 2 * q;
+    const uint32_t w = E == 8 ? *reinterpret_cast<const uint32_t *>(from) : E == 4 ? *reinterpret_cast<const uint16_t *>(from) : *from;
     M o[8];
     decode8<TYPE>(w, scale_f32(Q.scales[r * Q.lds + b]), o);
     M *p = A + r * ld + c;
-    if (c + 8 <= Q.cols) {
-        m8_t m;
+    if (c + E <= Q.cols) {
+        any_t m;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) m[i] = o[i];
-        __builtin_memcpy(p, &m, sizeof m);   // wide at any multiple of an element, as the loads above
+        for (int i = 0; i < E; ++i) m[i] = o[i];
+        __builtin_nontemporal_store(m, (any_t *)p);   // the caches keep what is read (8192 x 16384 f32 and back 211 us, without 255)
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i)
+        for (int i = 0; i < E; ++i)
             if (c + i < Q.cols) p[i] = o[i];
     }
 }
 
-template <int TYPE>
+template <int TYPE, bool NT>
 __global__ __launch_bounds__(MXT) void dequantize_cols_kernel(Mx4View Q, typename Elem<TYPE>::mem *__restrict__ A,
                                                                int64_t ld, int64_t nb) {
     typedef typename Elem<TYPE>::mem M;
@@ -271,7 +272,10 @@ __global__ __launch_bounds__(MXT) void dequantize_cols_kernel(Mx4View Q, typenam
         M *p = A + r + c0 * ld;
 #pragma unroll
         for (int i = 0; i < MX4_BLOCK; ++i)
-            if (c0 + i < Q.cols) p[i * ld] = o[i];
+            if (c0 + i < Q.cols) {
+                if constexpr (NT) __builtin_nontemporal_store(o[i], p + i * ld);
+                else p[i * ld] = o[i];
+            }
     }
 }
 
@@ -295,17 +299,21 @@ hipError_t quantize_t(const Mx4Dense &A, const Mx4View &Q, const Mx4Random &rnd,
     typedef typename Elem<TYPE>::mem M;
     const M *a = (const M *)A.ptr;
     const int64_t nb = mx4_blocks(Q.cols);
+    // What the last-level cache (256 MB) cannot hold passes it by: 8192 x 16384 f32 225 and 250 us with the way back,
+    // 4096 x 8192 f64 across memory 104 and 121, but 3412 x 5730 f32, which it can hold, 36 and 32
+    const bool past = Q.rows * Q.cols * (int64_t)sizeof(M) >= ((int64_t)1 << 28);
     if (A.sc == 1) {
         return row_chunks(Q.rows, nb * 4, [&](int64_t r0, int64_t rows) {
             const uint32_t units = (uint32_t)(rows * nb * 4);
-            hipLaunchKernelGGL((quantize_rows_kernel<TYPE, SR>), dim3((units + MXT - 1) / MXT), dim3(MXT), 0, s, a,
-                               A.sr, Q, fast_div((uint32_t)nb), units, r0, rnd);
+            auto go = [&](auto kernel) {
+                hipLaunchKernelGGL(kernel, dim3((units + MXT - 1) / MXT), dim3(MXT), 0, s, a, A.sr, Q, fast_div((uint32_t)nb), units, r0, rnd);
+            };
+            past ? go(quantize_rows_kernel<TYPE, SR, true>) : go(quantize_rows_kernel<TYPE, SR, false>);
             return hipGetLastError();
         });
     }
-    hipLaunchKernelGGL((quantize_cols_kernel<TYPE, SR>),
-                       cols_grid(Q.rows, nb), dim3(MXT), 0, s,
-                       a, A.sc, Q, nb, rnd);
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, cols_grid(Q.rows, nb), dim3(MXT), 0, s, a, A.sc, Q, nb, rnd); };
+    past ? go(quantize_cols_kernel<TYPE, SR, true>) : go(quantize_cols_kernel<TYPE, SR, false>);
     return hipGetLastError();
 }
 
@@ -314,16 +322,18 @@ template <int TYPE> hipError_t dequantize_t(const Mx4View &Q, const Mx4Dense &A,
     M *a = (M *)const_cast<void *>(A.ptr);
     const int64_t nb = mx4_blocks(Q.cols);
     if (A.sc == 1) {
-        return row_chunks(Q.rows, nb * 4, [&](int64_t r0, int64_t rows) {
-            const uint32_t units = (uint32_t)(rows * nb * 4);
+        constexpr int a_block = MX4_BLOCK * sizeof(M) / 16;
+        return row_chunks(Q.rows, nb * a_block, [&](int64_t r0, int64_t rows) {
+            const uint32_t units = (uint32_t)(rows * nb * a_block);
             hipLaunchKernelGGL((dequantize_rows_kernel<TYPE>), dim3((units + MXT - 1) / MXT), dim3(MXT), 0, s, Q, a, A.sr,
                                fast_div((uint32_t)nb), units, r0);
             return hipGetLastError();
         });
     }
-    hipLaunchKernelGGL((dequantize_cols_kernel<TYPE>),
-                       cols_grid(Q.rows, nb), dim3(MXT), 0, s, Q,
-                       a, A.sc, nb);
+    // Past the caches only where a wave writes whole lines: 16384 x 16384 f32 547 and 572 us with the way there, 4097 x
+    // 8191 bf16 82 and 61
+    auto go = [&](auto kernel) { hipLaunchKernelGGL(kernel, cols_grid(Q.rows, nb), dim3(MXT), 0, s, Q, a, A.sc, nb); };
+    (uintptr_t)a % 128 == 0 && A.sc * (int64_t)sizeof(M) % 128 == 0 ? go(dequantize_cols_kernel<TYPE, true>) : go(dequantize_cols_kernel<TYPE, false>);
     return hipGetLastError();
 }
 

@@ -205,6 +205,29 @@ def test_large_offsets(cuda):
     assert not a[: cols].any()
 
 
+@pytest.mark.parametrize("t,rows,cols", [("f32", 8192, 8200), ("f64", 4096, 8193), ("bf16", 64, 40), ("f16", 128, 100)])
+def test_across_memory_as_along_it(cuda, t, rows, cols):
+    """Matrices above and below 256 MB, whole lines across memory: the same codes and values as along it."""
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    a = torch.randn(rows, cols, generator=g, device=cuda, dtype=TORCH["f32"]).to(TORCH[t])
+    across = a.t().contiguous()
+    P, Q = rb.mx4_empty(rows, cols, device=cuda), rb.mx4_empty(rows, cols, device=cuda)
+    rb.mx4_quantize("R", "N", rows, cols, a.view(-1), cols, P)
+    rb.mx4_quantize("C", "N", rows, cols, across.view(-1), rows, Q)
+    nb = (cols + 31) // 32
+    assert torch.equal(P.codes, Q.codes) and torch.equal(P.scales[:, :nb], Q.scales[:, :nb])
+    pick = torch.arange(0, rows, max(1, rows // 8), device=cuda)
+    code, scale = R.quantize(a[pick].cpu().double().numpy())
+    assert np.array_equal(Q.codes[pick].cpu().numpy(), R.pack(code)) and np.array_equal(Q.scales[pick, :nb].cpu().numpy(), scale)
+    a.fill_(7.0)
+    across.fill_(7.0)
+    rb.mx4_dequantize("R", "N", rows, cols, P, a.view(-1), cols)
+    rb.mx4_dequantize("C", "N", rows, cols, P, across.view(-1), rows)
+    assert torch.equal(a, across.t())
+    exp = torch.from_numpy(R.values(R.pack(code), scale, cols)).to(TORCH[t])
+    assert torch.equal(a[pick].cpu(), exp)
+
+
 # ---------------------------------------------------------------------------------------------
 # products
 # ---------------------------------------------------------------------------------------------
