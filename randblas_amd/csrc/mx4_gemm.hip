@@ -226,8 +226,8 @@ __device__ __forceinline__ void store_rows(const Out &o, const float *from, int 
 // blocks are kept at place block ^ (row / 2 & 7), which spreads the 16 rows that an access takes at once over
 // all banks (the lane that fills a place loads the block that belongs there). The packed scales lie behind
 // the codes.
-// Bound by the power of the products (fed from registers alone 6.5 PFLOP/s): 8192^3 bf16 271 us with the scales' pass,
-// 4.05 PFLOP/s. Short contractions are bound by the results' way to memory: 4096 x 4096 x 1024 f32 24 us, 2.9 TB/s.
+// Bound by the power of the products (fed from registers alone 6.5 PFLOP/s): 8192^3 bf16 259 us with the scales' pass,
+// 4.24 PFLOP/s. Short contractions are bound by the results' way to memory: 4096 x 4096 x 1024 f32 24 us, 2.9 TB/s.
 template <typename T, int BP, int BO, int WP, int WO>
 __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kernel(Mx4View P, Mx4View O, const uint8_t *ps, const uint8_t *os,
                                                                                   int nb, int steps_z, Out out, float *partial) {
@@ -562,8 +562,8 @@ template <int PL, int BD, int NT, bool SPREAD> struct DenseTile {
 // where LDS is short), the next ones a part of the rows a step; 16-byte blocks at place
 // block ^ (row / 2), the rows' scales behind them.
 //
-// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 204 us, 1.35 PFLOP/s, the rate of a
-// large bf16 product by the library; 4096 x 1001 x 8192 f32, three planes, 173 us with their pass, 1.16.
+// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 197 us, 1.39 PFLOP/s (a
+// large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 172 us with their pass, 1.17.
 template <typename T, int PL, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
@@ -667,7 +667,7 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 // steps ahead (one where LDS is short), and the wait of a step leaves its own loads on their way.
 // Scales go to LDS through registers, a block's after each other; the decoding instruction looks at a float's exponent
 // only, so a shift of the word brings a scale there.
-// 2048 x 4096 x 8192 bf16 (256 x 128 tiles) 120 us, 1.14 PFLOP/s, without the operands ahead and with 8 bytes' scales by
+// 2048 x 4096 x 8192 bf16 (256 x 128 tiles) 122 us, 1.13 PFLOP/s, without the operands ahead and with 8 bytes' scales by
 // two reads 146; bound by the decoding beside the products and the reads from LDS.
 template <typename T, int PL, int BQ, int BD, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
