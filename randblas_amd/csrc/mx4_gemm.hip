@@ -411,41 +411,81 @@ template <int PL> __device__ __forceinline__ void split(float x, uint32_t *b) {
 }
 __device__ __forceinline__ uint32_t bf16_bits(__bf16 x) { return __builtin_bit_cast(unsigned short, x); }
 
+// 8 elements of a row as 16 bytes of each plane
+template <typename T> __device__ __forceinline__ void to_planes(const T (&v)[8], v4u (&w)[Planes<T>::N]) {
+    constexpr int PL = Planes<T>::N;
+    uint32_t b[8][PL];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        if constexpr (PL == 1) b[i][0] = bf16_bits(v[i]);
+        else split<PL>((float)v[i], b[i]);
+    }
+#pragma unroll
+    for (int q = 0; q < PL; ++q)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[q][i] = b[2 * i][q] | b[2 * i + 1][q] << 16;
+}
 // The planes of a dense factor in a workspace: plane i of element (r, c) at out[(i * rows + r) * ld + c], ld a
-// multiple of 64, zeros behind the last column. One thread makes 8 columns of a row; with COLS the rows
-// are contiguous in memory, and lanes go along them.
-// Bound by HBM: 1001 x 8192 f32 20 us, 4.1 TB/s.
-template <typename T, bool COLS>
+// multiple of 64, zeros behind the last column. One thread makes 8 columns of a row. Bound by HBM: 1001 x 8192 f32
+// 13.5 us, 6.1 TB/s (with loads of single elements 20).
+template <typename T>
 __global__ __launch_bounds__(256) void planes_kernel(const T *__restrict__ x, int64_t stride, int64_t rows, int64_t cols,
                                                      int64_t ld, uint16_t *__restrict__ out) {
     constexpr int PL = Planes<T>::N;
-    const int64_t n8 = ld / 8;
-    int64_t r, c8;
-    if (COLS) {
-        r = (int64_t)blockIdx.x * 64 + (threadIdx.x & 63);
-        c8 = (int64_t)blockIdx.y * 4 + (threadIdx.x >> 6);
-    } else {
-        r = blockIdx.y;
-        c8 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    const int64_t c = ((int64_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (c >= ld) return;
+    for (int64_t r = blockIdx.y; r < rows; r += gridDim.y) {
+        T v[8];
+        if (c + 8 <= cols) {
+            typedef T any8 __attribute__((ext_vector_type(8), aligned(sizeof(T))));
+            const any8 m = *(const any8 *)(x + r * stride + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = m[i];
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = c + i < cols ? x[r * stride + c + i] : (T)0.f;
+        }
+        v4u w[PL];
+        to_planes(v, w);
+#pragma unroll
+        for (int q = 0; q < PL; ++q) *(v4u *)(out + ((int64_t)q * rows + r) * ld + c) = w[q];
     }
-    while (r < rows && c8 < n8) {
-        uint32_t b[8][PL];
+}
+// The same for contiguous columns: 64 rows x 64 columns a workgroup, lanes along the rows, turned in LDS so that lines of
+// 128 bytes are written whole (2400 x 7680 f32 31 us, 5.9 TB/s; pieces of 16 bytes to a row 65).
+template <typename T>
+__global__ __launch_bounds__(256) void planes_cols_kernel(const T *__restrict__ x, int64_t stride, int64_t rows, int64_t cols,
+                                                          int64_t ld, uint16_t *__restrict__ out) {
+    constexpr int PL = Planes<T>::N;
+    __shared__ v4u tile[PL * 64 * 8];   // row's piece p at place p ^ row
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r0 = (int64_t)blockIdx.x * 64, r = r0 + lane;
+    for (int64_t c0 = (int64_t)blockIdx.y * 64; c0 < ld; c0 += (int64_t)gridDim.y * 64) {
+        T v[2][8];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int64_t c = c8 * 8 + i;
-            const T v = c < cols ? (COLS ? x[c * stride + r] : x[r * stride + c]) : (T)0.f;
-            if constexpr (PL == 1) b[i][0] = bf16_bits(v);
-            else split<PL>((float)v, b[i]);
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t c = c0 + (wave + 4 * h) * 8 + i;
+                v[h][i] = r < rows && c < cols ? x[c * stride + r] : (T)0.f;
+            }
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v4u w[PL];
+            to_planes(v[h], w);
+#pragma unroll
+            for (int q = 0; q < PL; ++q) tile[(q * 64 + lane) * 8 + ((wave + 4 * h) ^ (lane & 7))] = w[q];
         }
+        __syncthreads();
+        const int piece = threadIdx.x & 7;
 #pragma unroll
-        for (int q = 0; q < PL; ++q) {
-            v4u w;
+        for (int q = 0; q < PL; ++q)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) w[i] = b[2 * i][q] | b[2 * i + 1][q] << 16;
-            *(v4u *)(out + ((int64_t)q * rows + r) * ld + c8 * 8) = w;
-        }
-        if (COLS) c8 += (int64_t)gridDim.y * 4;
-        else r += gridDim.y;
+            for (int h = 0; h < 2; ++h) {
+                const int row = (threadIdx.x >> 3) + 32 * h;
+                if (r0 + row < rows) *(v4u *)(out + ((int64_t)q * rows + r0 + row) * ld + c0 + piece * 8) = tile[(q * 64 + row) * 8 + (piece ^ (row & 7))];
+            }
+        __syncthreads();
     }
 }
 
@@ -1425,11 +1465,10 @@ template <int TYPE> hipError_t mixed_t(const Mx4Product &q, uint8_t *work, hipSt
         const T *x = (const T *)p.X.ptr;
         const int64_t n8 = m.ld / 8;
         if (p.X.sc == 1)
-            hipLaunchKernelGGL((planes_kernel<T, false>), dim3((unsigned)((n8 + 255) / 256), (unsigned)(p.M < 65535 ? p.M : 65535)),
+            hipLaunchKernelGGL((planes_kernel<T>), dim3((unsigned)((n8 + 255) / 256), (unsigned)(p.M < 65535 ? p.M : 65535)),
                                dim3(256), 0, s, x, p.X.sr, p.M, p.K, m.ld, planes);
         else
-            hipLaunchKernelGGL((planes_kernel<T, true>),
-                               dim3((unsigned)((p.M + 63) / 64), (unsigned)((n8 + 3) / 4 < 65535 ? (n8 + 3) / 4 : 65535)), dim3(256), 0, s, x,
+            hipLaunchKernelGGL((planes_cols_kernel<T>), dim3((unsigned)((p.M + 63) / 64), (unsigned)(n8 / 8 < 65535 ? n8 / 8 : 65535)), dim3(256), 0, s, x,
                                p.X.sc, p.M, p.K, m.ld, planes);
         e = hipGetLastError();
         if (e != hipSuccess) return e;
