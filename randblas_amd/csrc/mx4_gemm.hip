@@ -1381,11 +1381,12 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     // enough that those are fewer bytes than its codes, and more where that still makes a workgroup for every
     // compute unit. The contraction is cut until there are 256 workgroups. More rows too where that makes
     // no more than a workgroup for each compute unit (64 x 8192 x 4096 bf16 16.5 us, in tiles 20.6; 88 x 59 x 812
-    // f32 14.5 and 27.8), except for one or two planes with blocks across (64 x 4096 x 4096 25.0 and 19.9).
+    // f32 14.5 and 27.8), except for one or two planes with blocks across more than 128 columns (64 x 4096 x 4096 25.0 and
+    // 19.9; but 426 x 28 x 12096 15.9 and 17.8).
     const int df = p.M <= 16 || pl == 3 ? 1 : 2;
     const int64_t dgroups = (p.M + 16 * df - 1) / (16 * df);
     const int64_t widest = p.yt ? 256 : 64;
-    if (p.M <= 16 * df || ((!p.yt || pl == 3) && (p.N + widest - 1) / widest * dgroups <= 256)) {
+    if (p.M <= 16 * df || ((!p.yt || pl == 3 || p.N <= 128) && (p.N + widest - 1) / widest * dgroups <= 256)) {
         m.rows = df;
         m.bq = (int)widest;
         if (!p.yt)
@@ -1406,6 +1407,9 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     // one plane: two tiles of 128 x 128 fit a compute unit (533 x 4231 x 5056: cut to 512 workgroups 51.5 us, to 256 59.0)
     int64_t z = 1;
     while (t * z * 2 <= (pl == 1 && m.bq == 128 ? 512 : 256) && steps / (z * 2) >= 8) z *= 2;
+    // few tiles: shorter slices (300 x 300 x 1000 f16 16.9 us, without 19.8; with 128 workgroups no longer, 512 x 512 x 2048
+    // bf16 15.8 and 15.3)
+    while (t * z * 2 <= 64 && steps / (z * 2) >= 4) z *= 2;
     m.steps_z = (int)((steps + z - 1) / z + 3) / 4 * 4;   // codes come by 4 steps
     m.slices = (int)((steps + m.steps_z - 1) / m.steps_z);
     if (m.slices > 1) m.partials = round256((size_t)m.slices * p.M * p.N * 4);

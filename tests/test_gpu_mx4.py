@@ -378,6 +378,9 @@ def test_few_rows_exact(cuda, opB, t, m, n, k):
     ("right", "f16", "T", "C", 75, 900, 5000, 0),
     ("left", "f32", "T", "R", 64, 100, 3000, 1),
     ("right", "f32", "N", "R", 100, 600, 3000, 2),
+    ("right", "bf16", "N", "R", 100, 90, 3000, 1),
+    ("left", "f16", "T", "C", 100, 75, 2000, 3),
+    ("right", "f16", "N", "C", 300, 300, 1000, 0),      # few tiles
     ("both", "f32", "T", "R", 4100, 4099, 300, 1),      # 256 x 256
     ("both", "bf16", "T", "C", 4099, 4100, 520, 0),
     ("both", "f16", "T", "R", 1050, 1060, 4500, 2),     # 128 x 128, the contraction cut
