@@ -603,7 +603,7 @@ template <int PL, int BD, int NT, bool SPREAD> struct DenseTile {
 // block ^ (row / 2), the rows' scales behind them.
 //
 // 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 197 us, 1.39 PFLOP/s (a
-// large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 172 us with their pass, 1.17.
+// large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 167 us with their pass, 1.21.
 template <typename T, int PL, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
