@@ -1377,20 +1377,22 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     m.ld = (p.K + 63) / 64 * 64;
     if (!m.direct) m.planes = round256((size_t)pl * p.M * m.ld * 2);
     // The kernel for few rows, 16 or 32 of them (3 planes of 32: more than LDS, or with blocks across the
-    // registers, hold) and 16 to 64 columns (256) a workgroup. Columns: each workgroup reads its dense rows whole, so
-    // enough that those are fewer bytes than its codes, and more where that still makes a workgroup for every
-    // compute unit. The contraction is cut until there are 256 workgroups. More rows too where that makes
+    // registers, hold) and 16 to 64 columns (256) a workgroup. Columns: as many as leave a workgroup for every compute
+    // unit, since the sum of slices is a launch of its own (16 x 8192 x 8192 bf16 in a graph, 32 columns 13.8 us, 64 and
+    // slices 16.3; 16 x 4096 x 4096, 16 columns 6.9 and 11.6). But each workgroup reads its dense rows whole: where those
+    // are 512 KB, enough columns that their codes are more (16 x 4096 x 16384, 64 columns 15.4 us, 16 17.0). The
+    // contraction is cut until there are 256 workgroups. More rows too where that makes
     // no more than a workgroup for each compute unit (64 x 8192 x 4096 bf16 16.5 us, in tiles 20.6; 88 x 59 x 812
     // f32 14.5 and 27.8), except for one or two planes with blocks across more than 128 columns (64 x 4096 x 4096 25.0 and
     // 19.9; but 426 x 28 x 12096 15.9 and 17.8).
     const int df = p.M <= 16 || pl == 3 ? 1 : 2;
-    const int64_t dgroups = (p.M + 16 * df - 1) / (16 * df);
+    const int64_t dgroups = (p.M + 16 * df - 1) / (16 * df), rows = p.M < 16 * df ? p.M : 16 * df;
     const int64_t widest = p.yt ? 256 : 64;
     if (p.M <= 16 * df || ((!p.yt || pl == 3 || p.N <= 128) && (p.N + widest - 1) / widest * dgroups <= 256)) {
         m.rows = df;
         m.bq = (int)widest;
         if (!p.yt)
-            for (m.bq = 16; m.bq < 64 && (m.bq < 4 * pl * (p.M < 16 * df ? p.M : 16 * df) || p.N * dgroups >= 512 * m.bq);) m.bq *= 2;
+            for (m.bq = 16; m.bq < 64 && ((rows * pl * 2 * p.K >= 512 << 10 && m.bq < 4 * pl * rows) || p.N * dgroups >= 512 * m.bq);) m.bq *= 2;
         const int64_t groups = (p.N + m.bq - 1) / m.bq * dgroups, units = p.yt ? (p.K + 31) / 32 : (p.K + 255) / 256;
         m.slices = 1;
         while (groups * m.slices < 256 && units / (m.slices * 2) >= (p.yt ? 2 * ROWS_WAVES : dense_waves(pl * m.rows))) m.slices *= 2;
