@@ -172,6 +172,7 @@ for _t, _ct in (("f64", ctypes.c_double), ("f32", ctypes.c_float)):
         getattr(lib, f"rbh_sketch_symmetric_{_t}").argtypes[:-1] + [P(OptionsC), c_vp]
     getattr(lib, f"rbh_sksy_tri_ex_{_t}").argtypes = getattr(lib, f"rbh_sksy_tri_{_t}").argtypes[:-1] + [P(OptionsC), c_vp]
 
+lib.hipStreamIsCapturing.argtypes = [c_vp, P(ctypes.c_int)]   # of the HIP runtime that the library is linked to
 for _t in ("f64", "f32", "f16", "bf16"):
     getattr(lib, f"rbh_mx4_quantize_{_t}").argtypes = [c_char, c_char, c_i64, c_i64, c_vp, c_i64, P(MX4MatrixC),
                                                        ctypes.c_int, P(RNGStateC), P(RNGStateC), c_vp]
@@ -742,6 +743,12 @@ def _mx4_stream(x, stream):
     return stream
 
 
+def _captures(stream) -> bool:
+    """Whether a graph captures the stream (a handle), whichever stream and device are the current ones."""
+    status = ctypes.c_int()
+    return lib.hipStreamIsCapturing(stream, ctypes.byref(status)) == 0 and status.value != 0
+
+
 def _bytes_2d(x, name, rows, width):
     """Address of, and bytes between the rows of, a uint8 array of at least rows x width, checked."""
     if x.dtype not in _MX4_BYTES or x.ndim != 2:
@@ -825,8 +832,8 @@ def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
     factors need opA = "N" and opB = "T" (blocks along the contraction). The gradient of the dense
     factor is the product of C's gradient with op flipped on the 4-bit one.
 
-    On a stream that a graph captures, a call that needs a workspace allocates it from the graph's own
-    memory (torch's allocator), so captured calls share none."""
+    On a stream that torch captures into a graph, a call that needs a workspace allocates it on that stream,
+    from the graph's own memory (torch's allocator), so captured calls share none."""
     if isinstance(X, MX4Matrix):
         ro_a, co_a = x_off_r, x_off_c_or_ld
         if isinstance(Y, MX4Matrix):
@@ -846,13 +853,15 @@ def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
         raise TypeError("mxmm: C and the dense factor must both be f32, both f16 or both bf16")
     fn, st = _MXMM[side, t], _mx4_stream(C, stream)
     head = (_b(layout), _b(opA), _b(opB), m, n, k, alpha, *factors, beta, _ptr(C), ldc)
-    if torch is None or not getattr(C, "is_cuda", False) or not torch.cuda.is_current_stream_capturing():
+    if not getattr(C, "is_cuda", False) or not _captures(st):
         return _check(fn(*head, None, st))
     work = WorkC()
     _check(fn(*head, ctypes.byref(work), st))
     if work.bytes == 0:
         return _check(fn(*head, None, st))
-    block = torch.empty(work.bytes, dtype=torch.uint8, device=C.device)
+    # the call's own stream's: the next block of another stream may be the same bytes, unordered to this call
+    with torch.cuda.stream(torch.cuda.ExternalStream(st, device=C.device)):
+        block = torch.empty(work.bytes, dtype=torch.uint8, device=C.device)
     work.ptr = block.data_ptr()
     _check(fn(*head, ctypes.byref(work), st))
 

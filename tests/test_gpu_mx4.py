@@ -658,6 +658,73 @@ def test_captured_and_replayed(cuda, side, t, opB, m):
             c.check_bitwise()
 
 
+@pytest.mark.parametrize("side,t,opB,m", [("right", "f32", "T", 150), ("right", "f16", "N", 150), ("right", "f32", "N", 9),
+                                          ("both", "bf16", "T", 150)])
+def test_captured_on_a_stream_of_the_callers(cuda, side, t, opB, m):
+    """A capture that forks to a stream passed as stream=: the product's workspace is that stream's, so what the
+    capturing stream allocates and writes beside the product does not meet it."""
+    st, fork = torch.cuda.Stream(), torch.cuda.Stream()
+    cases = [Case(cuda, side, m, 260, 1056, t, "R", "N", opB, s, True) for s in (1, 2)]
+    for c in cases:
+        c.run(stream=fork.cuda_stream)
+        c.run(stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        ahead = torch.zeros(1 << 26, dtype=torch.uint8, device=cuda)   # so that the fork's calls start beside the fills
+        fork.wait_stream(torch.cuda.current_stream())
+        cases[0].run(stream=fork.cuda_stream)
+        beside = [torch.empty(n, dtype=torch.uint8, device=cuda).fill_(0xFF)
+                  for n in (1 << 12, 1 << 14, 1 << 16, 1 << 18, 1 << 20, 1 << 22) for _ in range(4)]
+        cases[1].run()
+        again = [torch.empty_like(b).fill_(0xFE) for b in beside]
+        cases[0].run(stream=fork.cuda_stream)
+        torch.cuda.current_stream().wait_stream(fork)
+    for rep in range(4):
+        for c in cases:
+            c.C.view(-1, c.ldc).fill_(float("nan") if rep % 2 else 3.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        for c in cases:
+            c.check_bitwise()
+            c.run()
+            c.check_bitwise()
+        assert all(bool((b == 0xFF).all()) for b in beside) and all(bool((b == 0xFE).all()) for b in again)
+        assert not ahead.any()
+
+
+def test_capturing_stream_is_the_calls(cuda):
+    """stream= captures and the current stream does not: a workspace of the graph's. The other way round, an eager
+    call during a capture: the arena of its own stream."""
+    st, eager = torch.cuda.Stream(), torch.cuda.Stream()
+    a, b = (Case(cuda, "right", 150, 260, 1056, "f32", "R", "N", "T", s, True) for s in (1, 2))
+    for c in (a, b):
+        for s in (st, eager):
+            c.run(stream=s.cuda_stream)
+    torch.cuda.synchronize()
+    a.new(cuda)
+    b.new(cuda)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=st):
+        b.run(stream=eager.cuda_stream)
+        with torch.cuda.stream(eager):
+            a.run(stream=st.cuda_stream)
+    torch.cuda.synchronize()
+    b.check_bitwise()
+    for rep in range(3):
+        a.C.fill_(9.0)
+        b.C.fill_(9.0)
+        torch.cuda.synchronize()
+        g.replay()
+        torch.cuda.synchronize()
+        a.check_bitwise()
+        assert bool((b.C == 9.0).all())   # no part of the graph
+        b.run()
+        b.check_bitwise()
+
+
 def test_captured_call_without_a_workspace_is_refused(cuda):
     """The C ABI without a caller's workspace, where the call needs one: an error, and the capture ends well."""
     import ctypes
