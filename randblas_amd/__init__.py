@@ -736,10 +736,14 @@ def _mx4_tag(x) -> str:
     return tag
 
 
-def _mx4_stream(x, stream):
-    """_stream without the objects it makes on the way: these calls may take less time than they do."""
-    if stream is None and getattr(x, "is_cuda", False):
-        return torch._C._cuda_getCurrentRawStream(x.device.index)
+def _mx4_stream(stream, *arrays):
+    """The given stream, or the current one of the arrays' device: any of them may be the one that is on a device,
+    and its contents are ordered by that stream. (_stream without the objects it makes on the way: these calls may
+    take less time than they do.)"""
+    if stream is None:
+        for x in arrays:
+            if getattr(x, "is_cuda", False):
+                return torch._C._cuda_getCurrentRawStream(x.device.index)
     return stream
 
 
@@ -812,7 +816,7 @@ def mx4_quantize(layout, op, n_rows, n_cols, A, lda, Q: MX4Matrix, rounding="nea
     if rounding == "stochastic":
         state, nxt = seed.c(), RNGStateC()
     _check(_MX4_QUANTIZE[_mx4_tag(A)](_b(layout), _b(op), n_rows, n_cols, _ptr(A), lda, Q._c, ROUNDINGS[rounding], state,
-                                      nxt, _mx4_stream(A, stream)))
+                                      nxt, _mx4_stream(stream, A, Q.codes, Q.scales)))
     return RNGState.from_c(nxt) if nxt is not None else None
 
 
@@ -820,7 +824,7 @@ def mx4_dequantize(layout, op, n_rows, n_cols, Q: MX4Matrix, A, lda, ro=0, co=0,
     """op(A) = submat(Q), n_rows x n_cols at (ro, co), co a multiple of 32 (rbh_mx4_dequantize). Exact in
     every type but f16, which rounds to nearest even."""
     _check(_MX4_DEQUANTIZE[_mx4_tag(A)](_b(layout), _b(op), n_rows, n_cols, Q._c, ro, co, _ptr(A), lda,
-                                        _mx4_stream(A, stream)))
+                                        _mx4_stream(stream, A, Q.codes, Q.scales)))
 
 
 def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, stream=None) -> None:
@@ -839,19 +843,22 @@ def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
         if isinstance(Y, MX4Matrix):
             side, (ro_b, co_b, beta, C, ldc) = "both", args
             factors, dense = [X._c, ro_a, co_a, Y._c, ro_b, co_b], None
+            arrays = C, X.codes, X.scales, Y.codes, Y.scales
         else:
             side, (ldb, beta, C, ldc) = "left", args
             factors, dense = [X._c, ro_a, co_a, _ptr(Y), ldb], Y
+            arrays = C, Y, X.codes, X.scales
     else:
         A, lda, B = X, x_off_r, x_off_c_or_ld
         if not isinstance(B, MX4Matrix):
             raise TypeError("mxmm needs an MX4Matrix")
         side, (ro_b, co_b, beta, C, ldc) = "right", (Y,) + args
         factors, dense = [_ptr(A), lda, B._c, ro_b, co_b], A
+        arrays = C, A, B.codes, B.scales
     t = _mx4_tag(C)
     if t == "f64" or (dense is not None and dense.dtype != C.dtype):
         raise TypeError("mxmm: C and the dense factor must both be f32, both f16 or both bf16")
-    fn, st = _MXMM[side, t], _mx4_stream(C, stream)
+    fn, st = _MXMM[side, t], _mx4_stream(stream, *arrays)
     head = (_b(layout), _b(opA), _b(opB), m, n, k, alpha, *factors, beta, _ptr(C), ldc)
     if not getattr(C, "is_cuda", False) or not _captures(st):
         return _check(fn(*head, None, st))

@@ -773,6 +773,48 @@ def test_host_arrays(cuda):
     assert np.array_equal(out.T, v)
 
 
+def test_host_and_device_arrays_in_order(cuda):
+    """On a stream of its own, behind a queue of work: what a host array is made from, or goes into, is on the device,
+    and the call takes its turn there."""
+    rng = np.random.default_rng(1)
+    n, cols = 600, 2080
+    a = torch.from_numpy(rng.integers(-6, 7, (n, cols)).astype(np.float32))
+    a[:, ::32] = 6.0   # every block's scale is 1, every integer but 5 a value of its own
+    a[a.abs() == 5] = 4.0
+    there = a.to(cuda)
+    x = rng.integers(-3, 4, (5, cols)).astype(np.float32)
+    work = torch.randn(4096, 4096, device=cuda)
+    late = torch.zeros_like(there)
+    Q, P = rb.mx4_empty(n, cols, device=cuda), rb.mx4_empty(n, cols, device=cuda)
+    Q.codes.zero_()
+    Q.scales.zero_()
+    P.codes.zero_()
+    P.scales.zero_()
+    torch.cuda.synchronize()
+    out, C = np.zeros(n * cols, np.float32), np.zeros(5 * n, np.float32)
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        for _ in range(20):
+            work = torch.tanh(work @ work)
+        late.copy_(there)
+        rb.mx4_quantize("R", "N", n, cols, late.view(-1), cols, Q)
+        rb.mx4_dequantize("R", "N", n, cols, Q, out, cols)   # device to host
+        for _ in range(20):
+            work = torch.tanh(work @ work)
+        P.codes.fill_(0x11)
+        P.scales.fill_(1)
+        rb.mx4_quantize("R", "N", n, cols, a.numpy().ravel(), cols, P)   # host to device, behind the fills
+        for _ in range(20):
+            work = torch.tanh(work @ work)
+        Q.codes.copy_(P.codes ^ 0x88)   # the signs
+        rb.mxmm("R", "N", "T", 5, n, cols, 1.0, x.ravel(), cols, Q, 0, 0, 0.0, C, n)
+    torch.cuda.synchronize()
+    assert np.array_equal(out.reshape(n, cols), a.numpy())
+    code, scale = R.quantize(a.double().numpy())
+    assert np.array_equal(P.codes.cpu().numpy(), R.pack(code)) and np.array_equal(P.scales[:, : cols // 32].cpu().numpy(), scale)
+    assert np.array_equal(C.reshape(5, n), -(x @ a.numpy().T))
+
+
 @pytest.mark.parametrize("opB", ["T", "N"])
 def test_gradient_of_the_dense_factor(cuda, opB):
     """C = A op(B): with G the gradient of C, A's is G op(B)^T, the product with op flipped. C is linear in

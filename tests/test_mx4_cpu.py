@@ -154,6 +154,55 @@ def test_product_refusals():
         mm("R", "N", "T", 5, 9, 64, 1.0, A, 64, A, 0, 0, 0.0, C, 9)
 
 
+class OnDevice:
+    """What the calls ask of a tensor on device 3 (never read: the C entry is replaced)."""
+
+    is_cuda = True
+    device = type("device", (), {"index": 3})
+
+    def __init__(self, dtype):
+        self.dtype = dtype
+
+    def data_ptr(self):
+        return 1 << 40
+
+
+@pytest.mark.parametrize("place", range(5))
+def test_stream_is_that_of_any_device_array(monkeypatch, place):
+    """Host and device arrays in one call: the current stream of the device array's device, whichever it is."""
+    torch = pytest.importorskip("torch")
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda i: 1000 + i, raising=False)
+    seen = []
+    entry = lambda *args: seen.append(args[-1]) or 0
+    monkeypatch.setattr(rb, "_captures", lambda stream: False, raising=False)
+    for table in (rb._MX4_QUANTIZE, rb._MX4_DEQUANTIZE, rb._MXMM):
+        for key in table:
+            monkeypatch.setitem(table, key, entry)
+
+    def matrix(codes, scales):
+        Q = handle(9, 64)
+        object.__setattr__(Q, "codes", OnDevice(torch.uint8) if codes else Q.codes)
+        object.__setattr__(Q, "scales", OnDevice(torch.uint8) if scales else Q.scales)
+        return Q
+
+    def dense(here):
+        return OnDevice(torch.float32) if here else torch.zeros(9 * 64)
+
+    at = [i == place for i in range(5)]
+    if place < 3:
+        rb.mx4_quantize("R", "N", 9, 64, dense(at[0]), 64, matrix(at[1], at[2]))
+        rb.mx4_dequantize("R", "N", 9, 64, matrix(at[1], at[2]), dense(at[0]), 64)
+    if place < 4:
+        rb.mxmm("R", "N", "T", 5, 9, 64, 1.0, dense(at[1]), 64, matrix(at[2], at[3]), 0, 0, 0.0, dense(at[0]), 9)
+        rb.mxmm("R", "N", "N", 9, 5, 64, 1.0, matrix(at[2], at[3]), 0, 0, dense(at[1]), 5, 0.0, dense(at[0]), 5)
+    rb.mxmm("R", "N", "T", 9, 9, 64, 1.0, matrix(at[1], at[2]), 0, 0, matrix(at[3], at[4]), 0, 0, 0.0, dense(at[0]), 9)
+    assert seen and seen == [1003] * len(seen)
+    rb.mx4_dequantize("R", "N", 9, 64, matrix(True, True), dense(False), 64, stream=7)
+    assert seen[-1] == 7
+    rb.mx4_dequantize("R", "N", 9, 64, matrix(False, False), dense(False), 64)
+    assert seen[-1] is None
+
+
 def test_null_result_is_refused():
     A, B = np.zeros(5 * 64, np.float32), handle(9, 64)
     refused("C != nullptr", rb.mxmm, "R", "N", "T", 5, 9, 64, 1.0, A, 64, B, 0, 0, 0.0, Null(np.float32), 9)
