@@ -496,6 +496,109 @@ struct Dense16 {
     int chunks;
 };
 
+// 4-bit values of 2^128 or more are infinities, as in other products of 32 bits. Where the dense factor is several planes,
+// most numbers' lower ones are 0, and 0 times an infinity makes a NaN of a sum that is infinite. Every sum that this
+// touches is a NaN, so the kernels look for one among their complete sums, then for scales under which infinities can
+// be, and form those sums once more: with 0 for the infinite values of every plane but the first, which is 0 only with
+// the number. That reads its operands from memory as they are needed: with an infinity in every sum 512 x 4096 x 4096 f32
+// takes 690 us instead of 68, 16 x 4096 x 4096 81 and 17, with NaNs from elsewhere 63 and 17. Without a NaN the look
+// at the sums is all that is added (-1 to 1.7 % over 36 sizes).
+//
+// Operands' places: a lane's row (yt: column) of the 4-bit factor is q, of the dense one d.
+//
+// The factors come from the kernel's arguments, which are read again for it: kept in scalar registers beside the loop
+// they push others' loads behind it (some kernels 1 us longer).
+struct Factors {   // how the arguments of every kernel that has planes begin
+    Dense16 D;
+    Mx4View Y;
+};
+static_assert(sizeof(Dense16) % alignof(Mx4View) == 0, "arguments lie as the members do");
+__device__ __forceinline__ const Factors &factors_again() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return *(const Factors *)(const void *)p;
+}
+__device__ __forceinline__ v4u finite_or_0(v4u q) {
+    v4u r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        r[i] = (q[i] & 0x7F80u) == 0x7F80u ? q[i] & 0xFFFF0000u : q[i];
+        r[i] = (q[i] & 0x7F800000u) == 0x7F800000u ? r[i] & 0xFFFFu : r[i];
+    }
+    return r;
+}
+// sum += q d over k0 <= k < k1, k0 a multiple of 32
+template <bool YT, bool QFIRST, int PL>
+__device__ __forceinline__ v4f add_finite(v4f sum, const Factors &x, int64_t q, int64_t d, int64_t k0, int64_t k1, int g) {
+    const Mx4View &Y = x.Y;
+    const Dense16 &D = x.D;
+#pragma unroll 1
+    for (int64_t k = k0; k < k1; k += 32) {   // lane group g: elements k + 8 g .. + 7
+        v4u w{};
+        if constexpr (YT) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t row = k + 8 * g + j;
+                const bool in = row < k1 && q < Y.cols;
+                const uint8_t *const code = Y.codes + (in ? row * Y.ldq + q / 2 : 0), *const scale = Y.scales + (in ? row * Y.lds + q / 32 : 0);
+                const uint32_t v = decode_bf16_4((uint32_t)*code >> (q % 2 * 4), __builtin_bit_cast(float, (uint32_t)*scale << 23))[0];
+                w[j / 2] |= (in ? v & 0xFFFFu : 0u) << (j % 2 * 16);
+            }
+        } else if (q < Y.rows && k < Y.cols) {
+            const uint32_t scale = Y.scales[q * Y.lds + k / 32];
+            w = decode_bf16(*(const uint32_t *)(Y.codes + q * Y.ldq + k / 2 + 4 * g), __builtin_bit_cast(float, scale << 23));
+        }
+        const int64_t piece = k / 8 + g;
+#pragma unroll
+        for (int p = 0; p < PL; ++p) {
+            const v4u v = d < D.rows && piece < D.chunks ? *(const v4u *)(D.ptr + p * D.plane + d * D.ld + piece * 8) : v4u{};
+            const v4u wp = p ? finite_or_0(w) : w;
+            sum = QFIRST ? mfma_bf16(wp, v, sum) : mfma_bf16(v, wp, sum);
+        }
+    }
+    return sum;
+}
+// Whether a scale of 2^126 or 2^127 is among those of `count` rows (columns) of the 4-bit factor from q0, k0 <= k < k1 of
+// the contraction; q0 (across) or k0 is a multiple of 128, scales are read by words of 4
+template <bool YT> __device__ __forceinline__ bool infinities(const Mx4View &Y, int64_t q0, int count, int64_t k0, int64_t k1, int lane) {
+    uint32_t found = 0;
+    const int64_t q1 = q0 + count, rows = YT ? k1 : q1 < Y.rows ? q1 : Y.rows, cols = YT ? (q1 < Y.cols ? q1 : Y.cols) : k1;
+    auto has_0 = [](uint32_t w) { return (w - 0x01010101u) & ~w & 0x80808080u; };   // not 0 if a byte is
+    for (int64_t r = (YT ? k0 : q0) + lane; r < rows; r += 64)
+#pragma unroll 8
+        for (int64_t b = (YT ? q0 : k0) / 32; b < mx4_blocks(cols); b += 4) {
+            const uint32_t w = *(const uint32_t *)(Y.scales + r * Y.lds + b);
+            found |= has_0(w ^ 0xFDFDFDFDu) | has_0(w ^ 0xFEFEFEFEu);
+        }
+    return __any(found != 0);
+}
+__device__ __forceinline__ bool any_nan(v4f x, bool counts) {
+    const float sum = (x[0] + x[1]) + (x[2] + x[3]);   // a NaN if one of them is
+    return __builtin_expect(__any(sum != sum && counts), 0);
+}
+// A wave's operands of a tile: those of the 4-bit factor are qf apart, a lane's row (column) of one is ql times r16
+template <bool YT, bool QFIRST, int PL, int FQ, int FD>
+__device__ __forceinline__ void mend_tile(v4f (&acc)[FQ][FD], int64_t q0, int qf, int ql, int64_t d0, int64_t k0,
+                                          int64_t k1, int lane) {
+    v4f total = acc[0][0];
+#pragma unroll
+    for (int i = 1; i < FQ * FD; ++i) total += acc[i / FD][i % FD];
+    if (!any_nan(total, true)) return;
+    const Factors &x = factors_again();
+    // (blocks across: the words that a wave's two blocks are in)
+    if (!infinities<YT>(x.Y, YT ? q0 & -128 : q0, YT ? 128 : FQ * 16, k0, k1, lane)) return;
+#pragma unroll 1
+    for (int i = 0; i < FQ * FD; ++i) {
+        v4f old = acc[0][0];
+#pragma unroll
+        for (int j = 1; j < FQ * FD; ++j) old = i == j ? acc[j / FD][j % FD] : old;
+        if (!any_nan(old, true)) continue;
+        const v4f sum = add_finite<YT, QFIRST, PL>(v4f{}, x, q0 + i / FD * qf + (lane & 15) * ql, d0 + i % FD * 16 + (lane & 15), k0, k1, lane >> 4);
+#pragma unroll
+        for (int j = 0; j < FQ * FD; ++j) acc[j / FD][j % FD] = i == j ? sum : acc[j / FD][j % FD];
+    }
+}
+
 // A wave's part of the result to memory by way of LDS (16 rows of the second index at a time, `rows` this wave's
 // place), q0 and d0 its first entry. Entry i of a lane's 4 is row 4 g + i of the first operand; with YT the 4-bit
 // index of row r of operand f is 4 r + f.
@@ -692,6 +795,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
         arrive();
     }
     if (st < s1) compute(st, lds0);
+    if constexpr (PL > 1)
+        mend_tile<false, QFIRST, PL>(acc, q0 + wq * WQ, 16, 1, d0 + wd * WD, s0 * 64, s1 * 64 < K ? s1 * 64 : K, lane);
     __syncthreads();
     store_wave<T, false, QFIRST>(acc, (float *)lds + wave * (STORE / NW / 4), out, partial, q0 + wq * WQ, d0 + wd * WD, lane);
 }
@@ -736,7 +841,10 @@ __global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_k
     const uint32_t vq = qpart < nb ? (uint32_t)((wave * (64 / PR) + lane / PR) * Y.ldq) + qpart * 16 : OUTSIDE;
     const uint32_t vs = wave * 4 < nb ? (uint32_t)(lane * Y.lds) + wave * 4 : OUTSIDE;
     uint32_t sreg = 0;   // a row's scales of 4 blocks on their way to LDS
+    // behind the last block 0, whatever is there: sums that are not stored are to be no NaN for that
+    const uint32_t keep = nb - wave * 4 >= 4 ? ~0u : nb > wave * 4 ? (1u << (8 * (nb - wave * 4))) - 1 : 0u;
     auto put_scales = [&](uint8_t *to) {
+        if constexpr (PL > 1) sreg &= keep;
 #pragma unroll
         for (int i = 0; i < 4; ++i) to[Dense::BYTES + CW * PITCH + (wave * 4 + i) * 64 + lane] = (uint8_t)(sreg >> (8 * i));
     };
@@ -849,6 +957,8 @@ __global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_k
         at = at == (DS - 1) * STAGE ? 0 : at + STAGE;
         half(b, a, lds + at, 0, st + DS, lds + last);
     }
+    if constexpr (PL > 1)
+        mend_tile<true, QFIRST, PL>(acc, q0 + wq * 64, 1, 4, d0 + wd * WD, s0 * 64, s1 * 64 < K ? s1 * 64 : K, lane);
     arrive();   // nothing is on its way to LDS any more
     store_wave<T, true, QFIRST>(acc, (float *)lds + wave * (STORE / NW / 4), out, partial, q0 + wq * 64, d0 + wd * WD, lane);
 }
@@ -1022,6 +1132,14 @@ __global__ __launch_bounds__(dense_waves(Planes<T>::N * (RG > 4 ? 2 : 1)) * 64, 
     }
     arrive();   // nothing is on its way to LDS any more
     add_waves<W, NF * DF>(acc, (v4f *)half0, lane, wave, [&](int i, int l, v4f v) {
+        if constexpr (PL > 1)
+            if (any_nan(v, i % DF * 16 + (l & 15) < rows))
+                if (const Factors &x = factors_again(); infinities<false>(x.Y, q0 + i / DF * 16, 16, 0, x.Y.cols, l)) {
+                    v = v4f{};
+                    for (int64_t k = blockIdx.y * W * 256; k < x.Y.cols; k += stride * 256)
+                        v = add_finite<false, true, PL>(v, x, q0 + i / DF * 16 + (l & 15), d0 + i % DF * 16 + (l & 15), k,
+                                                        k + W * 256 < x.Y.cols ? k + W * 256 : x.Y.cols, l >> 4);
+                }
 #pragma unroll
         for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (i / DF) * 16 + 4 * (l >> 4) + j, d0 + (i % DF) * 16 + (l & 15), v[j]);
     });
@@ -1107,6 +1225,9 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
         uint32_t s;
         v4u d[DF][PL];
     };
+    // behind the last block 0, whatever is there: sums that are not stored are to be no NaN for that
+    const int mine = tile_nb - (lane & 1) * 4;
+    const uint32_t keep = mine >= 4 ? ~0u : mine > 0 ? (1u << (8 * mine)) - 1 : 0u;
     auto load = [&](int u, Codes &x) {
         const int left = K - u * 32 < 32 ? K - u * 32 : 32;
         const int64_t k0 = left > 0 ? (int64_t)u * 32 : 0;   // past the last unit the ranges are empty
@@ -1117,6 +1238,7 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
         // lane: row lane / 2, 4 blocks
         const int b = (lane & 1) * 4;
         x.s = load4(sb, b < nb ? (uint32_t)((lane >> 1) * Y.lds) + b : OUTSIDE, 0);
+        if constexpr (PL > 1) x.s &= keep;
         dense(u * 4 + g, x.d);
     };
     v4f acc[16 * DF];
@@ -1163,7 +1285,24 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense
         compute(b);
         __builtin_amdgcn_sched_barrier(0);
     }
+    // whether f is true for one of the parts of the contraction that the workgroup's waves took together
+    auto in_parts = [&](auto f) {
+        bool any = false;
+        for (int64_t k = blockIdx.y * ROWS_WAVES * 32; k < K; k += stride * 32) any |= f(k, k + ROWS_WAVES * 32 < K ? k + ROWS_WAVES * 32 : K);
+        return any;
+    };
     add_waves<ROWS_WAVES, 16 * DF>(acc, sums, lane, wave, [&](int i, int l, v4f v) {
+        if constexpr (PL > 1)
+            if (any_nan(v, i % DF * 16 + (l & 15) < rows)) {
+                const Factors &x = factors_again();
+                if (in_parts([&](int64_t k, int64_t end) { return infinities<true>(x.Y, q0, 256, k, end, l); })) {
+                    v = v4f{};
+                    in_parts([&](int64_t k, int64_t end) {
+                        v = add_finite<true, true, PL>(v, x, q0 + (l & 15) * 16 + i / DF, d0 + i % DF * 16 + (l & 15), k, end, l >> 4);
+                        return false;
+                    });
+                }
+            }
 #pragma unroll
         for (int j = 0; j < 4; ++j) put1<T>(out, q0 + (4 * (l >> 4) + j) * 16 + i / DF, d0 + (i % DF) * 16 + (l & 15), v[j]);
     });

@@ -564,6 +564,80 @@ def test_products_of_extreme_scales(cuda, m, side, opB):
     assert np.array_equal(C.cpu().numpy().reshape(m, n), exp)
 
 
+def infinite_case(rng, m, n, k, t, opB):
+    """A dense m x k, codes and scales of a 4-bit k x n (after op): one code that counts a column, under a scale of
+    2^123 .. 2^127; the dense entry it meets has one plane, all planes, or is 0 or an infinity."""
+    special = np.array([1.0, -1.0, 0.0, 3.0, -0.75, 1.0 + 2.0 ** -10, -1.5 - 2.0 ** -9, np.inf, -np.inf, np.nan, 2.0 ** -14])
+    if t == "f32":
+        special = np.concatenate((special, [1.0 + 2.0 ** -23, -3.14159274, 2.0 ** -100, -2.0 ** -120]))
+    x = rng.integers(-2, 3, (m, k)).astype(np.float64)
+    at = rng.integers(0, k, n)
+    x[:, np.unique(at)] = rng.choice(special, (m, len(np.unique(at))))
+    for r in range(m):   # an infinity or a NaN meets every column of its row: in some rows only
+        if r % 3:
+            x[r, ~np.isfinite(x[r])] = 2.0
+    code = np.zeros((k, n), np.uint8)
+    code[at, np.arange(n)] = rng.integers(0, 16, n)
+    q = np.ascontiguousarray(code if opB == "N" else code.T)
+    scales = rng.integers(250, 255, (q.shape[0], (q.shape[1] + 31) // 32)).astype(np.uint8)
+    return torch.from_numpy(x).to(TORCH[t]), R.pack(np.pad(q, ((0, 0), (0, -q.shape[1] % 32)))), scales
+
+
+@pytest.mark.parametrize("side", ["right", "left"])
+@pytest.mark.parametrize("opB", ["T", "N"])
+@pytest.mark.parametrize("t", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 64), (2, 16390, 100), (3, 300, 500), (16, 70, 4100), (30, 600, 333), (40, 200, 9000), (150, 260, 1000),
+                                   (300, 700, 5000), (2100, 4100, 264)])
+def test_infinite_values_of_a_4_bit_factor(cuda, m, n, k, t, opB, side):
+    """4-bit values of 2^128 or more enter as infinities whatever the dense factor's type: infinite sums where 32-bit
+    arithmetic has them, NaN where it multiplies them with 0. One product a sum that is not 0, so sums are exact."""
+    rng = np.random.default_rng(m + n + k)
+    x, codes, scales = infinite_case(rng, m, n, k, t, opB)
+    Q = rb.MX4Matrix(codes.shape[0], n if opB == "N" else k, torch.from_numpy(codes).to(cuda), torch.from_numpy(scales).to(cuda))
+    v = torch.from_numpy(R.values(codes, scales, Q.n_cols)).float()   # 2^128 and more: infinite
+    v = (v if opB == "N" else v.t()).double().to(cuda)
+    xd = x.double().to(cuda)
+    code_at = (v != 0).double()
+    # the one product that counts; a code of 0 counts where the dense entry is not finite
+    bad = ((~xd.isfinite()).double() @ (1 - code_at)) > 0
+    pick, col = code_at.max(0).values > 0, code_at.argmax(0)
+    one = xd[:, col] * v[col, torch.arange(n, device=cuda)]
+    exp = torch.where(pick, one, torch.zeros_like(one))
+    exp[bad] = float("nan")
+    exp = exp.float().to(TORCH[t])
+    C = torch.full((m * n,), 5.0, dtype=TORCH[t], device=cuda)
+    if side == "right":
+        rb.mxmm("R", "N", opB, m, n, k, 1.0, x.to(cuda).view(-1), k, Q, 0, 0, 0.0, C, n)
+    else:   # C^T = op(B)^T A^T
+        rb.mxmm("R", "T" if opB == "N" else "N", "T", n, m, k, 1.0, Q, 0, 0, x.to(cuda).view(-1), k, 0.0, C, m)
+    got = C.view(m, n) if side == "right" else C.view(n, m).t()
+    wrong = ~((got == exp) | (got.isnan() & exp.isnan()))
+    at = wrong.nonzero()[:5].tolist()
+    assert not at, (int(wrong.sum()), [(i, j, float(got[i, j]), float(exp[i, j]), float(xd[i, col[j]]), float(v[col[j], j])) for i, j in at])
+    assert m == 1 or bool(exp.isinf().any())   # row 0 keeps its infinities and NaN
+
+
+@pytest.mark.parametrize("m,n,k", [(3, 144, 64), (150, 300, 500), (700, 1030, 300), (1050, 1060, 4500)])
+def test_two_factors_of_extreme_scales(cuda, m, n, k):
+    """Two 4-bit factors up to 2^127: products are exact, those of 2^128 or more infinite as 32-bit results, and those
+    of a value of 2^128 or more and a small one finite."""
+    rng = np.random.default_rng(k)
+    code = np.zeros((n, -(-k // 32) * 32), np.uint8)
+    at = rng.integers(0, k, n)
+    code[np.arange(n), at] = rng.integers(0, 16, n)
+    scales = rng.integers(250, 255, (n, code.shape[1] // 32)).astype(np.uint8)
+    Q = rb.MX4Matrix(n, k, torch.from_numpy(R.pack(code)).to(cuda), torch.from_numpy(scales).to(cuda))
+    small = rng.choice(np.array([100, 126, 127], np.uint8), (m, code.shape[1] // 32))
+    ones = np.zeros((m, code.shape[1]), np.uint8)
+    ones[:, :k] = 2
+    P = rb.MX4Matrix(m, k, torch.from_numpy(R.pack(ones)).to(cuda), torch.from_numpy(small).to(cuda))
+    C = torch.full((m * n,), 5.0, device=cuda)
+    rb.mxmm("R", "N", "T", m, n, k, 1.0, P, 0, 0, Q, 0, 0, 0.0, C, n)
+    with np.errstate(over="ignore"):
+        exp = (R.values(R.pack(ones), small, k) @ R.values(R.pack(code), scales, k).T).astype(np.float32)
+    assert np.array_equal(C.cpu().numpy().reshape(m, n), exp) and np.isinf(exp).any()
+
+
 def test_two_streams_at_once(cuda):
     """Calls that need workspaces, in flight on two streams together, keep apart."""
     cases = [Case(cuda, "right", 150, 700, 2100, "f32", "R", "N", "T", 1, True, low=126, high=127),
