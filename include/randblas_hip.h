@@ -464,10 +464,11 @@ int rbh_mx4_dequantize_bf16(char layout, char op, int64_t n_rows, int64_t n_cols
  * (ro_b, co_b), as the sparse factor of rbh_spmm_right_*; left: A is; both: both are, and their blocks
  * have to lie along the contraction (opA = 'N', opB = 'T'). Column offsets are multiples of 32; a window
  * that ends inside a block of a wider matrix is copied first where its further codes would count. The
- * dense factor and C have one type, m and n are at most 2^28, k at most 2^21; the dense factor enters the
- * sums with all its bits, 4-bit values of 2^128 or more next to one as infinities (sums with such a value may
- * take some 10 times as long); products of two 4-bit values are exact. The gradient of a product's dense
- * factor is the product of C's gradient with op flipped on the 4-bit one. C overlaps no other array. */
+ * dense factor and C have one type, m and n are at most 2^28, k at most 2^21. The dense factor enters the
+ * sums with all its bits, but for those of an f32 below 2^-133 (which numbers under 2^-110 have); 4-bit values
+ * of 2^128 or more enter next to one as infinities (sums with such a value may take 10 to 20 times as
+ * long). Products of two 4-bit values are exact. The gradient of a product's dense factor is the product
+ * of C's gradient with op flipped on the 4-bit one. C overlaps no other array. */
 int rbh_mxmm_right_f32(char layout, char opA, char opB, int64_t m, int64_t n, int64_t k, float alpha, const float *A,
                        int64_t lda, const rbh_mx4 *B, int64_t ro_b, int64_t co_b, float beta, float *C, int64_t ldc,
                        rbh_work *work, void *stream);

@@ -832,7 +832,8 @@ def mxmm(layout, opA, opB, m, n, k, alpha, X, x_off_r, x_off_c_or_ld, Y, *args, 
       mxmm(layout, opA, opB, m, n, k, alpha, A_mx4, ro_a, co_a, B, ldb, beta, C, ldc)
       mxmm(layout, opA, opB, m, n, k, alpha, A, lda, B_mx4, ro_b, co_b, beta, C, ldc)
       mxmm(layout, opA, opB, m, n, k, alpha, A_mx4, ro_a, co_a, B_mx4, ro_b, co_b, beta, C, ldc)
-    The dense factor and C are of one type, f32, f16 or bf16; sums are formed in 32 bits. Two 4-bit
+    The dense factor and C are of one type, f32, f16 or bf16; sums are formed in 32 bits (of the dense factor's
+    bits those below 2^-133, which a f32 under 2^-110 has, are left out). Two 4-bit
     factors need opA = "N" and opB = "T" (blocks along the contraction). The gradient of the dense
     factor is the product of C's gradient with op flipped on the 4-bit one.
 

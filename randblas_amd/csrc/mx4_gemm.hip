@@ -367,7 +367,8 @@ hipError_t launch_both_tile(const Mx4View &P, const Mx4View &O, uint8_t *work, i
 // A product of E2M1 and a power of two is a bf16 number, so the 4-bit factor enters exactly. The dense one
 // enters as a sum of bf16 planes with all its bits: bf16 is one plane, f16 two (11 bits), f32 three (24
 // bits, cut off from the top 8 at a time: each remainder is exact, and 3 bf16 products at 2.5 PFLOP/s are
-// 5 times the f32 instruction's rate). Sums are f32.
+// 5 times the f32 instruction's rate). The smallest bf16 is 2^-133, and what a f32 under 2^-110 has below that is
+// left out. Sums are f32.
 typedef __bf16 v8bf __attribute__((ext_vector_type(8)));
 
 __device__ __forceinline__ v4f mfma_bf16(v4u a, v4u b, v4f c) {
@@ -395,7 +396,7 @@ template <typename T> struct Planes { static constexpr int N = 1; };
 template <> struct Planes<_Float16> { static constexpr int N = 2; };
 template <> struct Planes<float> { static constexpr int N = 3; };
 
-// x as a sum of bf16 numbers (their bits); an infinity or a NaN is the first one alone
+// x as a sum of bf16 numbers (their bits), without its bits below 2^-133; an infinity or a NaN is the first one alone
 template <int PL> __device__ __forceinline__ void split(float x, uint32_t *b) {
     const uint32_t u = __builtin_bit_cast(uint32_t, x);
     const bool finite = (u & 0x7F800000u) != 0x7F800000u;

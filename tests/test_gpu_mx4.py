@@ -436,6 +436,32 @@ def test_all_bits_of_the_dense_factor(cuda, m, opB):
         assert np.isinf(got[1, 5]) and np.all(np.isnan(np.delete(got[1], 5)))
 
 
+@pytest.mark.parametrize("opB", ["T", "N"])
+@pytest.mark.parametrize("m", [1, 20, 150, 600])
+def test_smallest_numbers_of_the_dense_factor(cuda, m, opB):
+    """f32 from the smallest subnormal to 2^-100, each times one +-2^90: what a number has from 2^-133 on arrives, cut
+    towards 0. So all its bits from 2^-110 on, and below that the sum is off by less than 2^-133 times the 4-bit value."""
+    k = n = 96
+    rng = np.random.default_rng(m)
+    code = np.zeros((k, n), np.uint8)
+    perm = rng.permutation(k)
+    sign = rng.integers(0, 2, n)
+    code[perm, np.arange(n)] = 2 + 8 * sign
+    q = np.ascontiguousarray(code if opB == "N" else code.T)
+    Q = rb.MX4Matrix(*q.shape, torch.from_numpy(R.pack(q)).to(cuda), torch.from_numpy(np.full((q.shape[0], 3), 127 + 90, np.uint8)).to(cuda))
+    x = rng.integers(1, 27 << 23, (m, k)).astype(np.uint32).view(np.float32)   # exponents to 2^-101
+    x[:, ::5] = rng.integers(1, 1 << 23, (m, len(range(0, k, 5)))).astype(np.uint32).view(np.float32)   # subnormals
+    x[rng.random((m, k)) < 0.5] *= np.float32(-1)
+    C = torch.empty(m * n, dtype=torch.float32, device=cuda)
+    rb.mxmm("R", "N", opB, m, n, k, 1.0, torch.from_numpy(x).to(cuda).view(-1), k, Q, 0, 0, 0.0, C, n)
+    got = C.cpu().double().numpy().reshape(m, n)
+    value = np.where(sign, -1.0, 1.0) * 2.0 ** 90
+    exact, kept = x.astype(np.float64)[:, perm] * value, np.trunc(x.astype(np.float64)[:, perm] * 2.0 ** 133) * 2.0 ** -133 * value
+    assert np.array_equal(got, kept)
+    assert np.array_equal(got[np.abs(x[:, perm]) >= 2.0 ** -110], exact[np.abs(x[:, perm]) >= 2.0 ** -110])
+    assert np.all(np.abs(got - exact) < 2.0 ** -133 * 2.0 ** 90)
+
+
 @pytest.mark.parametrize("side,opB", [("right", "T"), ("right", "N"), ("both", "T")])
 @pytest.mark.parametrize("m", [3, 140])
 def test_nan_scale_reaches_its_outputs_only(cuda, m, side, opB):
