@@ -157,6 +157,26 @@ def test_dequantize(cuda, rows, cols, ro, co, pad, t, layout, op):
     assert torch.all(padding == 7.0)
 
 
+@pytest.mark.parametrize("layout,op", [("R", "N"), ("R", "T"), ("C", "N"), ("C", "T")])
+@pytest.mark.parametrize("t", ["f64", "f32", "f16", "bf16"])
+@pytest.mark.parametrize("rows,cols", [(1, 1), (1, 16), (40, 70), (33, 129)])
+def test_signs_of_dequantized_values(cuda, rows, cols, t, layout, op):
+    """Every sign, of zeros too, those that a small scale rounds to 0 in f16 among them; a NaN block's have none."""
+    rng = np.random.default_rng(rows + cols)
+    codes, scales = R.random_mx4(rng, rows, cols, 90 if t == "f16" else 0, 140 if t == "f16" else 252)
+    codes[0, 0] = 0x98 if cols > 1 else 0x08   # -0 first, then -0.5
+    if cols > 32:
+        scales[0, 1] = 255
+    Q = rb.MX4Matrix(rows, cols, torch.from_numpy(codes).to(cuda), torch.from_numpy(scales).to(cuda))
+    exp = torch.from_numpy(R.values(codes, scales, cols)).to(TORCH[t])
+    buf, lda = stored(torch.zeros(rows, cols, dtype=TORCH[t]), layout, op, 0, cuda)
+    rb.mx4_dequantize(layout, op, rows, cols, Q, buf, lda)
+    got, _ = unstored(buf, lda, rows, cols, layout, op)
+    nan = torch.isnan(exp)
+    assert torch.equal(torch.isnan(got), nan) and torch.equal(got[~nan], exp[~nan])
+    assert torch.equal(torch.signbit(got)[~nan], torch.signbit(exp)[~nan]) and bool(torch.signbit(got[0, 0])) and got[0, 0] == 0
+
+
 @pytest.mark.parametrize("offset,pad", [(1, 0), (3, 5), (8, 8)])
 @pytest.mark.parametrize("layout", ["R", "C"])
 @pytest.mark.parametrize("t", ["f64", "f32", "f16", "bf16"])
