@@ -58,6 +58,22 @@ def test_reference_stochastic_rounding_has_the_right_mean():
     assert np.all(np.abs(mean - row) <= 6 * gap / 2 / 64)
 
 
+def test_two_stochastic_roundings_have_the_right_mean_of_squares():
+    """The mean of q1 q2 is x^2 for two roundings with words of their own; q1 q1 has the variance besides. Means of 4096
+    rows within 6 standard deviations of the differences from x^2, at most those of gap / 2 times twice the value and gap."""
+    rows, row = 4096, np.random.default_rng(2).standard_normal(32)
+    x = np.tile(row, (rows, 1))
+    q1, q2 = (R.values(R.pack(c), s, 32) for c, s in (R.quantize(x, R.philox_words(rows, 32, 5, at)) for at in (0, rows * 8)))
+    unit = 2.0 ** np.floor(np.log2(np.abs(row).max() / 6) + 1)
+    gap = np.where(np.abs(row) / unit < 2, 0.5, np.where(np.abs(row) / unit < 4, 1.0, 2.0)) * unit
+    low = np.floor(np.abs(row) / gap) * gap
+    variance = (np.abs(row) - low) * (low + gap - np.abs(row))
+    off = 6 * (np.abs(row) * gap + gap * gap) / np.sqrt(rows)
+    assert np.all(np.abs((q1 * q2).mean(0) - row * row) <= off)
+    assert np.all(np.abs((q1 * q1).mean(0) - row * row - variance) <= off)
+    assert ((q1 * q1).mean(0) - row * row).sum() > 0.9 * variance.sum() > 0.01 * (row * row).sum()
+
+
 @pytest.mark.parametrize("t", ["f64", "f32"])
 def test_quantize_refusals(t):
     dt = np.float64 if t == "f64" else np.float32
