@@ -72,7 +72,8 @@ template <typename T> struct Four {
         }
     }
     // NT: past the caches, for results that fill them (8192 x 8192 x 1024 f32 82 us, 87 without; 4096 x 8192 x 512
-    // bf16 42 and 45; f32 from planes, which lie there too, 109 and 103)
+    // bf16 42 and 45; f32 from planes, which lie there too, 109 and 103). Measured on products in a row, whose results
+    // nobody reads; a reader of a result that would have stayed in the caches is not measured
     template <bool NT> __device__ __forceinline__ void store(const Out &o, v4f v) {
         t4 r;
 #pragma unroll
@@ -226,8 +227,8 @@ __device__ __forceinline__ void store_rows(const Out &o, const float *from, int 
 // blocks are kept at place block ^ (row / 2 & 7), which spreads the 16 rows that an access takes at once over
 // all banks (the lane that fills a place loads the block that belongs there). The packed scales lie behind
 // the codes.
-// Bound by the power of the products (fed from registers alone 6.5 PFLOP/s): 8192^3 bf16 259 us with the scales' pass,
-// 4.24 PFLOP/s. Short contractions are bound by the results' way to memory: 4096 x 4096 x 1024 f32 24 us, 2.9 TB/s.
+// Bound by the power of the products (fed from registers alone 6.5 PFLOP/s): 8192^3 bf16 259 - 271 us on three cards with the
+// scales' pass, 4.06 - 4.24 PFLOP/s. Short contractions are bound by the results' way to memory: 4096 x 4096 x 1024 f32 24 us, 2.9 TB/s.
 template <typename T, int BP, int BO, int WP, int WO>
 __global__ __launch_bounds__((BP / WP) * (BO / WO) * 64, 2) void both_tile_kernel(Mx4View P, Mx4View O, const uint8_t *ps, const uint8_t *os,
                                                                                   int nb, int steps_z, Out out, float *partial) {
@@ -706,8 +707,8 @@ template <int PL, int BD, int NT, bool SPREAD> struct DenseTile {
 // where LDS is short), the next ones a part of the rows a step; 16-byte blocks at place
 // block ^ (row / 2), the rows' scales behind them.
 //
-// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 197 us, 1.39 PFLOP/s (a
-// large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 167 us with their pass, 1.21.
+// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 197 - 206 us on several cards, 1.33 - 1.39
+// PFLOP/s (a large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 165 - 173 us with their pass, 1.17 - 1.22.
 template <typename T, int PL, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
@@ -807,14 +808,14 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 // between rows; its 4 operands are then columns 4 c + f, and the operand f of the wave is columns f, f + 4, .. --
 // an order of the result's rows or columns that the stores undo.
 //
-// An element costs two instructions in every wave that decodes it, about as long as its products take, so the
-// two have to run at the same time: a wave decodes the next instruction's operands among the present one's
+// The 32 elements of a lane's operands cost 40 instructions in every wave that decodes them (16 conversions, 16 permutations,
+// 8 scales), about as long as their products take, so the two have to run at the same time: a wave decodes the next instruction's operands among the present one's
 // products, also across steps. For that the codes are one step further ahead than the dense rows, which are two
 // steps ahead (one where LDS is short), and the wait of a step leaves its own loads on their way.
 // Scales go to LDS through registers, a block's after each other; the decoding instruction looks at a float's exponent
 // only, so a shift of the word brings a scale there.
-// 2048 x 4096 x 8192 bf16 (256 x 128 tiles) 122 us, 1.13 PFLOP/s, without the operands ahead and with 8 bytes' scales by
-// two reads 146; bound by the decoding beside the products and the reads from LDS.
+// 2048 x 4096 x 8192 bf16 (256 x 128 tiles) 120 - 129 us on several cards, 1.07 - 1.15 PFLOP/s, without the operands ahead and with
+// 8 bytes' scales by two reads 146 beside 122; bound by the decoding beside the products and the reads from LDS.
 template <typename T, int PL, int BQ, int BD, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / 64) * (BD / WD) * 64, 2) void mixed_tile_yt_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                       Out out, float *partial) {
@@ -1198,7 +1199,9 @@ __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void both_rows_kernel(Mx4View Q
 }
 
 // Few dense rows and blocks across the contraction: codes, scales and dense rows from memory to registers, two units on
-// their way. 16 x 8192 x 8192 bf16 20 us, 1.8 TB/s, bound by the decoding (two instructions an element).
+// their way. 16 x 8192 x 8192 bf16 19.5 us: this kernel 15.7, 2.3 TB/s, and the sum of 8 slices 3.8. Bound by the way of its
+// loads: a wave has 4 units and two of them on their way. Vector instructions (2 an element, counted) are a quarter of
+// the kernel's time, matrix instructions a sixteenth, and waves wait for 43 % of theirs.
 template <typename T, int DF>
 __global__ __launch_bounds__(ROWS_WAVES * 64, 2) void mixed_rows_yt_kernel(Dense16 D, Mx4View Y, int K, RowsOut out) {
     constexpr int PL = Planes<T>::N;
@@ -1520,8 +1523,8 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     // registers, hold) and 16 to 64 columns (256) a workgroup. Columns: as many as leave a workgroup for every compute
     // unit, since the sum of slices is a launch of its own (16 x 8192 x 8192 bf16 in a graph, 32 columns 13.8 us, 64 and
     // slices 16.3; 16 x 4096 x 4096, 16 columns 6.9 and 11.6). But each workgroup reads its dense rows whole: where those
-    // are 512 KB, enough columns that their codes are more (16 x 4096 x 16384, 64 columns 15.4 us, 16 17.0). The
-    // contraction is cut until there are 256 workgroups. More rows too where that makes
+    // are 512 KB, enough columns that their codes are more (16 x 4096 x 16384, 64 columns 15.4 us, 16 17.0). Measured at 128,
+    // 256 and 512 KB only: where between the last two the sides meet is not known. The contraction is cut until there are 256 workgroups. More rows too where that makes
     // no more than a workgroup for each compute unit (64 x 8192 x 4096 bf16 16.5 us, in tiles 20.6; 88 x 59 x 812
     // f32 14.5 and 27.8), except for one or two planes with blocks across more than 128 columns (64 x 4096 x 4096 25.0 and
     // 19.9; but 426 x 28 x 12096 15.9 and 17.8).
