@@ -246,7 +246,8 @@ __global__ __launch_bounds__(MXT) void dequantize_rows_kernel(Mx4View Q, typenam
         any_t m;
 #pragma unroll
         for (int i = 0; i < E; ++i) m[i] = o[i];
-        __builtin_nontemporal_store(m, (any_t *)p);   // the caches keep what is read (8192 x 16384 f32 and back 211 us, without 255; no reader of the result measured)
+        // the caches keep what is read (8192 x 16384 f32 and back 211 us, without 255; no reader of the result measured)
+        __builtin_nontemporal_store(m, (any_t *)p);
     } else {
 #pragma unroll
         for (int i = 0; i < E; ++i)

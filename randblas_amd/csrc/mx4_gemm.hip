@@ -587,7 +587,7 @@ __device__ __forceinline__ void mend_tile(v4f (&acc)[FQ][FD], int64_t q0, int qf
     for (int i = 1; i < FQ * FD; ++i) total += acc[i / FD][i % FD];
     if (!any_nan(total, true)) return;
     const Factors &x = factors_again();
-    // (blocks across: the words that a wave's two blocks are in)
+    // blocks across: the words that the wave's two blocks are in
     if (!infinities<YT>(x.Y, YT ? q0 & -128 : q0, YT ? 128 : FQ * 16, k0, k1, lane)) return;
 #pragma unroll 1
     for (int i = 0; i < FQ * FD; ++i) {
@@ -707,8 +707,9 @@ template <int PL, int BD, int NT, bool SPREAD> struct DenseTile {
 // where LDS is short), the next ones a part of the rows a step; 16-byte blocks at place
 // block ^ (row / 2), the rows' scales behind them.
 //
-// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 197 - 206 us on several cards, 1.33 - 1.39
-// PFLOP/s (a large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 165 - 173 us with their pass, 1.17 - 1.22.
+// 256 x 256 tiles are bound by the products and their power: 4096 x 8192 x 4096 bf16 197 - 206 us on several cards, 1.33 -
+// 1.39 PFLOP/s (a large bf16 product by the library: 1.35); 4096 x 1001 x 8192 f32, three planes, 165 - 173 us with
+// their pass, 1.17 - 1.22.
 template <typename T, int PL, int BQ, int BD, int WQ, int WD, bool QFIRST>
 __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kernel(Dense16 D, Mx4View Y, int64_t K, int steps_z,
                                                                                    Out out, float *partial) {
@@ -809,8 +810,8 @@ __global__ __launch_bounds__((BQ / WQ) * (BD / WD) * 64, 2) void mixed_tile_kern
 // an order of the result's rows or columns that the stores undo.
 //
 // The 32 elements of a lane's operands cost 40 instructions in every wave that decodes them (16 conversions, 16 permutations,
-// 8 scales), about as long as their products take, so the two have to run at the same time: a wave decodes the next instruction's operands among the present one's
-// products, also across steps. For that the codes are one step further ahead than the dense rows, which are two
+// 8 scales), about as long as their products take, so the two have to run at the same time: a wave decodes the next
+// instruction's operands among the present one's products, also across steps. For that the codes are one step further ahead than the dense rows, which are two
 // steps ahead (one where LDS is short), and the wait of a step leaves its own loads on their way.
 // Scales go to LDS through registers, a block's after each other; the decoding instruction looks at a float's exponent
 // only, so a shift of the word brings a scale there.
@@ -1524,7 +1525,8 @@ MixedPlan mixed_plan(const Mx4Product &p) {
     // unit, since the sum of slices is a launch of its own (16 x 8192 x 8192 bf16 in a graph, 32 columns 13.8 us, 64 and
     // slices 16.3; 16 x 4096 x 4096, 16 columns 6.9 and 11.6). But each workgroup reads its dense rows whole: where those
     // are 512 KB, enough columns that their codes are more (16 x 4096 x 16384, 64 columns 15.4 us, 16 17.0). Measured at 128,
-    // 256 and 512 KB only: where between the last two the sides meet is not known. The contraction is cut until there are 256 workgroups. More rows too where that makes
+    // 256 and 512 KB only: where between the last two the sides meet is not known. The contraction is cut until
+    // there are 256 workgroups. More rows too where that makes
     // no more than a workgroup for each compute unit (64 x 8192 x 4096 bf16 16.5 us, in tiles 20.6; 88 x 59 x 812
     // f32 14.5 and 27.8), except for one or two planes with blocks across more than 128 columns (64 x 4096 x 4096 25.0 and
     // 19.9; but 426 x 28 x 12096 15.9 and 17.8).
